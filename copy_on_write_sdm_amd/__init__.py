@@ -34,6 +34,14 @@ from .prefill import (
     prefill_sdm_layer,
 )
 from .stack_decode import decode_faithful_sdm_stack, write_dense_cache
+from .attention import (
+    PageTableStep,
+    cache_width,
+    cached_attention,
+    extend_page_tables,
+    prompt_attention,
+    write_kv_cache,
+)
 from .controller import (
     ControllerDecodeGraph,
     ControllerStep,
@@ -52,10 +60,13 @@ __all__ = [
     "SDMPrefill",
     "FaithfulSDMDecodeState",
     "PackedSDMCopyOnWriteState",
+    "PageTableStep",
     "PagedSlotMap",
     "SDMCopyOnWriteStep",
     "SDMStepInputs",
     "allocate_dense_cache",
+    "cache_width",
+    "cached_attention",
     "decode_faithful_sdm_stack",
     "decode_sdm_layer",
     "decode_sdm_layer_controller",
@@ -64,6 +75,7 @@ __all__ = [
     "dense_sdm_sparse_step",
     "dense_sdm_sparse_step_layers",
     "dense_sparse_routes",
+    "extend_page_tables",
     "finish_sdm_step",
     "gated_delta_recurrence",
     "mark_written",
@@ -75,6 +87,8 @@ __all__ = [
     "prefill_sdm_layer",
     "prepare_sdm_step",
     "product_key_routes",
+    "prompt_attention",
     "sdm_recurrence",
     "write_dense_cache",
+    "write_kv_cache",
 ]

@@ -25,7 +25,7 @@ SOURCE_DIR = PACKAGE_DIR / "csrc"
 # one translation unit per step-kernel family so hipcc can run in parallel
 SOURCES = ("cowsdm.hip", "step_i32_packed.hip", "step_i32_dense.hip", "step_i64_packed.hip",
            "step_i64_dense.hip", "trace_plan.hip", "routes.hip", "controller.hip",
-           "recurrence.hip", "route_recurrence.hip")
+           "recurrence.hip", "route_recurrence.hip", "prompt_attention.hip", "kv_cache.hip")
 INCLUDE_DIR = REPO_DIR / "include"
 LIBRARY = PACKAGE_DIR / "lib" / "libcowsdm.so"
 BUILD_DIR = PACKAGE_DIR / "_build"
@@ -298,6 +298,69 @@ class HandoffLayer(ctypes.Structure):
     ]
 
 
+class PromptAttention(ctypes.Structure):
+    """cowsdm_prompt_attention_t."""
+
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("query_row", ctypes.c_int64),
+        ("query_head", ctypes.c_int64),
+        ("key_row", ctypes.c_int64),
+        ("key_head", ctypes.c_int64),
+        ("value_row", ctypes.c_int64),
+        ("value_head", ctypes.c_int64),
+        ("offsets", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("sequences", ctypes.c_int64),
+        ("longest", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("float_type", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class KVCache(ctypes.Structure):
+    """cowsdm_kv_cache_t."""
+
+    _fields_ = [
+        ("pages", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("page_tokens", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("key_codes", ctypes.c_void_p),
+        ("key_scales", ctypes.c_void_p),
+        ("value_codes", ctypes.c_void_p),
+        ("value_scales", ctypes.c_void_p),
+    ]
+
+
+class CachedQuery(ctypes.Structure):
+    """cowsdm_cached_query_t."""
+
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("query_request", ctypes.c_int64),
+        ("query_token", ctypes.c_int64),
+        ("query_head", ctypes.c_int64),
+        ("page_tables", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("requests", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("columns", ctypes.c_int64),
+        ("longest", ctypes.c_int64),
+        ("float_type", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -382,6 +445,18 @@ SIGNATURES: dict[str, tuple] = {
     "cowsdm_check_invariants": (
         _I32, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P]),
     "cowsdm_mark_written": (_I32, [_P, _I64, _I64, _P, _I64, _I32, _P, _P]),
+    "cowsdm_prompt_attention": (_I32, [ctypes.POINTER(PromptAttention), _P]),
+    "cowsdm_page_tables_extend": (
+        _I32, [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "cowsdm_pages_release": (
+        _I32, [_P, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P]),
+    "cowsdm_kv_write": (
+        _I32, [ctypes.POINTER(KVCache), _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _I64,
+               _P]),
+    "cowsdm_cached_attention_workspace_bytes": (
+        _I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "cowsdm_cached_attention": (
+        _I32, [ctypes.POINTER(KVCache), ctypes.POINTER(CachedQuery), _P, _I64, _P]),
     "cowsdm_product_key_routes": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P]),
 }
 

@@ -1,0 +1,342 @@
+"""The attention layers of a stack on the device: whole prompts, and single
+tokens over a paged cache held in 8 bits.
+
+The reference runs its attention layers in its model (CausalSelfAttention,
+copy_on_write_sdm/model.py:47-189) over a dense K/V cache in the activations'
+type; ``prefill_faithful_sdm_stack`` and ``decode_faithful_sdm_stack`` take
+them as the caller's callables.  These are the operators such a callable
+needs:
+
+* ``prompt_attention``    causal attention over packed prompts of different
+                          lengths, with grouped heads;
+* ``extend_page_tables``  the page tables and token slots of a step, from the
+                          requests' lengths and new tokens;
+* ``write_kv_cache``      keys and values into their slots, in 8 bits;
+* ``cached_attention``    each request's newest tokens over the cache.
+
+A page holds ``page_tokens`` tokens of one request in one layer: keys as
+[pages, heads, page_tokens, width], values transposed, [pages, heads, width,
+page_tokens], in float8 (e4m3), with one power of two for each page and head
+by which the codes count, [pages, heads].  The width is a head's, padded with
+zeros to 32, 64, 96, 128, 192 or 256 (``cache_width``).
+
+Kernels: csrc/prompt_attention.hip and csrc/kv_cache.hip.  Float32, float16
+and bfloat16; there is no backward pass and no CPU path.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Sequence
+
+import torch
+
+from . import _native as nat
+
+CODES = torch.float8_e4m3fn
+MAX_REQUESTS = 4_096
+PAGE_TOKENS = (16, 32, 64, 128, 256)
+CACHE_WIDTHS = (32, 64, 96, 128, 192, 256)
+
+
+def cache_width(head_width: int) -> int:
+    """The row width of a cache for heads of ``head_width``."""
+
+    if head_width <= 0 or head_width % 8 or head_width > CACHE_WIDTHS[-1]:
+        raise ValueError("attention head width must be a multiple of 8, at most 256")
+    return next(w for w in CACHE_WIDTHS if w >= head_width)
+
+
+def _need_device(tensor: torch.Tensor, what: str) -> None:
+    if not tensor.is_cuda:
+        raise RuntimeError(f"{what} must be on the GPU: the attention kernels have no CPU path")
+
+
+def _float_type(dtype: torch.dtype) -> int:
+    code = nat.FLOAT_TYPES.get(dtype)
+    if code is None:
+        raise TypeError("attention takes float32, float16 or bfloat16")
+    return code
+
+
+def _scale(scale: float | None, width: int) -> float:
+    if scale is None:
+        return width ** -0.5
+    if not 0.0 < scale < math.inf:
+        raise ValueError("the attention scale must be positive")
+    return scale
+
+
+def _rows(tensor: torch.Tensor) -> torch.Tensor:
+    """``tensor`` itself where its rows can be loaded 16 bytes at a time (a
+    slice of a fused projection can), else a contiguous copy."""
+
+    step = 16 // tensor.element_size()
+    strides = tensor.stride()
+    if strides[-1] == 1 and not tensor.data_ptr() % 16:
+        for s in strides[:-1]:
+            if s % step:
+                break
+        else:
+            return tensor
+    tensor = tensor.contiguous()
+    # contiguous() is the tensor itself where only its address is odd
+    return tensor.clone() if tensor.data_ptr() % 16 else tensor
+
+
+def _int32(tensor: torch.Tensor, shape: tuple[int, ...], what: str) -> None:
+    if tensor.dtype != torch.int32 or tensor.shape != shape or not tensor.is_contiguous():
+        raise ValueError(f"{what} must be contiguous int32 of shape {list(shape)}")
+
+
+@torch.no_grad()
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                     offsets: torch.Tensor, *, longest: int | None = None,
+                     scale: float | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts: query [T, heads, D], key and
+    value [T, kv_heads, D] (any strides between rows and heads; ``heads`` a
+    multiple of ``kv_heads``, query head h reads key head ``h // (heads //
+    kv_heads)``), and int32 offsets [S + 1] on the device: sequence s holds
+    rows offsets[s] to offsets[s + 1] - 1.  Returns [T, heads, D] in the
+    query's type; rows of no sequence are zero.  ``longest`` bounds the
+    sequences' lengths (T when not given) and sizes the launch: a bound that
+    is too small costs time, not correctness.  ``scale`` defaults to
+    D ** -0.5."""
+
+    if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
+        raise ValueError("attention takes query [T,heads,D] and key and value [T,kv_heads,D]")
+    rows, heads, width = query.shape
+    kv_heads = key.shape[1]
+    if key.shape[0] != rows or key.shape[2] != width:
+        raise ValueError("attention query, key and value do not align")
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise ValueError("query heads must be a multiple of the key heads")
+    cache_width(width)
+    code = _float_type(query.dtype)
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise TypeError("attention query, key and value share one type")
+    device = query.device
+    _need_device(query, "attention inputs")
+    if key.device != device or value.device != device or offsets.device != device:
+        raise ValueError("attention inputs must be on one device")
+    if offsets.ndim != 1 or offsets.numel() == 0:
+        raise ValueError("attention offsets must be a vector of sequences + 1")
+    _int32(offsets, offsets.shape, "attention offsets")
+    if longest is not None and longest < 0:
+        raise ValueError("the longest sequence cannot be negative")
+    factor = _scale(scale, width)
+    sequences = offsets.numel() - 1
+    if sequences == 0:
+        return torch.zeros(rows, heads, width, device=device, dtype=query.dtype)
+    out = torch.empty(rows, heads, width, device=device, dtype=query.dtype)
+    if rows == 0:
+        return out
+    query, key, value = _rows(query), _rows(key), _rows(value)
+    a = nat.PromptAttention(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), query.stride(0), query.stride(1),
+        key.stride(0), key.stride(1), value.stride(0), value.stride(1), offsets.data_ptr(),
+        out.data_ptr(), rows, sequences, rows if longest is None else longest, heads, kv_heads,
+        width, code, factor)
+    rc = nat.lib().cowsdm_prompt_attention(a, nat.stream_handle(device))
+    if rc:
+        nat.check(rc, "cowsdm_prompt_attention")
+    return out
+
+
+class PageTableStep(NamedTuple):
+    """What ``extend_page_tables`` returns, all int32 on the device: the
+    requests' new lengths [B], the free pages left [1], the offsets of their
+    new tokens in the packed order [B + 1], each new token's position in its
+    request and its slot [tokens], and whether something ran short [1]."""
+
+    lengths: torch.Tensor
+    free_count: torch.Tensor
+    offsets: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    overflow: torch.Tensor
+
+
+@torch.no_grad()
+def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: torch.Tensor,
+                       free_pages: torch.Tensor, free_count: torch.Tensor, *, page_tokens: int,
+                       tokens: int, out: Sequence[torch.Tensor] | None = None) -> PageTableStep:
+    """Room for ``added`` [B] new tokens of requests that hold ``lengths``
+    [B]: pages popped from the top of the free stack (``free_pages`` [P],
+    ``free_count`` [1]) in request order go into ``page_tables`` [B, columns]
+    in place, and every new token gets its position and slot (page *
+    page_tokens + position % page_tokens).  ``tokens`` is the size of the
+    packed token outputs, at least the sum of ``added``; entries past it are
+    -1.  Where the pages, the columns or ``tokens`` do not suffice, or a count
+    is negative, ``overflow`` is 1, positions and slots are -1 and the tables
+    stay as they were.  ``out``: the tensors to write, in the order of
+    ``PageTableStep``, none of them an input."""
+
+    batch = lengths.numel()
+    if lengths.ndim != 1 or page_tables.ndim != 2 or free_pages.ndim != 1:
+        raise ValueError("page tables take lengths [B], page_tables [B,columns], free_pages [P]")
+    _need_device(lengths, "page tables")
+    _int32(lengths, (batch,), "lengths")
+    _int32(added, (batch,), "added tokens")
+    _int32(page_tables, (batch, page_tables.shape[1]), "page tables")
+    _int32(free_pages, free_pages.shape, "free pages")
+    if free_count.dtype != torch.int32 or free_count.numel() != 1:
+        raise ValueError("the free count must be one int32")
+    if page_tokens not in PAGE_TOKENS:
+        raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
+    if tokens < 0:
+        raise ValueError("the token count cannot be negative")
+    if batch > MAX_REQUESTS:
+        raise ValueError(f"page tables take at most {MAX_REQUESTS} requests")
+    device = lengths.device
+    if out is None:
+        sizes = (batch, 1, batch + 1, tokens, tokens, 1)
+        step = PageTableStep(*torch.empty(sum(sizes), dtype=torch.int32, device=device)
+                             .split(sizes))
+    else:
+        step = PageTableStep(*out)
+        for t, n in zip(step, (batch, 1, batch + 1, tokens, tokens, 1)):
+            _int32(t, (n,), "page table outputs")
+        if batch and (step.lengths.data_ptr() == lengths.data_ptr()):
+            raise ValueError("the new lengths cannot be written over the old")
+        if step.free_count.data_ptr() == free_count.data_ptr():
+            raise ValueError("the new free count cannot be written over the old")
+    for t in (added, page_tables, free_pages, free_count, *step):
+        if t.device != device:
+            raise ValueError("page table tensors must be on one device")
+    rc = nat.lib().cowsdm_page_tables_extend(
+        lengths.data_ptr(), added.data_ptr(), batch, page_tables.data_ptr(),
+        page_tables.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+        page_tokens, tokens, step.lengths.data_ptr(), step.free_count.data_ptr(),
+        step.offsets.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(),
+        step.overflow.data_ptr(), nat.stream_handle(device))
+    if rc:
+        nat.check(rc, "cowsdm_page_tables_extend")
+    return step
+
+
+def _cache(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch.Tensor,
+           value_scales: torch.Tensor, width: int, device: torch.device) -> nat.KVCache:
+    """The C view of one layer's cache, after checking its tensors."""
+
+    if key_pages.ndim != 4:
+        raise ValueError("cache keys must be [pages,heads,page_tokens,width]")
+    pages, heads, page_tokens, padded = key_pages.shape
+    if (value_pages.shape != (pages, heads, padded, page_tokens)
+            or key_scales.shape != (pages, heads) or value_scales.shape != (pages, heads)):
+        raise ValueError("cache tensors do not align")
+    if (key_pages.dtype != CODES or value_pages.dtype != CODES
+            or key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32):
+        raise TypeError("cache codes are float8_e4m3fn and scales float32")
+    if page_tokens not in PAGE_TOKENS:
+        raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
+    if padded != cache_width(width):
+        raise ValueError(f"a cache for heads of {width} is {cache_width(width)} wide")
+    for t in (key_pages, key_scales, value_pages, value_scales):
+        if not t.is_contiguous():
+            raise ValueError("cache tensors must be contiguous")
+        if t.device != device:
+            raise ValueError("cache tensors must be on the inputs' device")
+    return nat.KVCache(pages, heads, page_tokens, padded, key_pages.data_ptr(),
+                       key_scales.data_ptr(), value_pages.data_ptr(), value_scales.data_ptr())
+
+
+@torch.no_grad()
+def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
+                   key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch.Tensor,
+                   value_scales: torch.Tensor) -> None:
+    """Keys and values [T, heads, D] (any strides between rows and heads) into
+    their slots [T] (int32; -1: not written) of one layer's cache, in place.
+
+    A page and head has one scale for its keys and one for its values: the
+    least power of two (from 2^-100 to 2^119) under which every finite
+    magnitude is at most 448.  Writing a page's first token sets it from the
+    tokens of the call; a page that goes on keeps the larger of its own and
+    that one, and where it grows the page's other codes are taken to it,
+    exactly but for the smallest.  Codes round to nearest even; e4m3 has no
+    infinity, so infinities become NaN.  A page's tokens of one call follow
+    one another, as ``extend_page_tables`` gives them."""
+
+    if key.ndim != 3 or value.shape != key.shape:
+        raise ValueError("cache writes take key and value [T,heads,D]")
+    tokens, heads, width = key.shape
+    _need_device(key, "cache writes")
+    device = key.device
+    code = _float_type(key.dtype)
+    if value.dtype != key.dtype:
+        raise TypeError("cache keys and values share one type")
+    if value.device != device or slots.device != device:
+        raise ValueError("cache writes must be on one device")
+    _int32(slots, (tokens,), "cache slots")
+    cache = _cache(key_pages, key_scales, value_pages, value_scales, width, device)
+    if cache.heads != heads:
+        raise ValueError("cache and keys differ in heads")
+    if tokens == 0:
+        return
+    key, value = _rows(key), _rows(value)
+    rc = nat.lib().cowsdm_kv_write(
+        cache, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+        value.stride(1), code, width, slots.data_ptr(), tokens, nat.stream_handle(device))
+    if rc:
+        nat.check(rc, "cowsdm_kv_write")
+
+
+def cached_workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, width: int,
+                           longest: int) -> int:
+    """The workspace of a ``cached_attention`` call: 0 where its launch does
+    not split the cache."""
+
+    return nat.lib().cowsdm_cached_attention_workspace_bytes(batch, tokens, heads, kv_heads,
+                                                             cache_width(width), longest)
+
+
+@torch.no_grad()
+def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: torch.Tensor,
+                     value_pages: torch.Tensor, value_scales: torch.Tensor,
+                     page_tables: torch.Tensor, lengths: torch.Tensor, *,
+                     longest: int | None = None, scale: float | None = None) -> torch.Tensor:
+    """Attention of each request's newest tokens over one layer's cache: query
+    [B, n, heads, D] holds the last n of its ``lengths`` [B] tokens (written
+    before), and row i sees positions 0 to length - n + i.  Grouped heads as
+    in ``prompt_attention``.  Returns [B, n, heads, D] in the query's type; a
+    row that sees nothing is zero.  ``longest`` bounds the lengths (the
+    tables' columns when not given): a bound that is too small costs time, not
+    correctness."""
+
+    if query.ndim != 4:
+        raise ValueError("cached attention takes query [B,n,heads,D]")
+    batch, tokens, heads, width = query.shape
+    _need_device(query, "attention inputs")
+    device = query.device
+    code = _float_type(query.dtype)
+    cache = _cache(key_pages, key_scales, value_pages, value_scales, width, device)
+    if heads == 0 or heads % cache.heads:
+        raise ValueError("query heads must be a multiple of the cache's heads")
+    if page_tables.ndim != 2:
+        raise ValueError("page tables must be [B,columns]")
+    columns = page_tables.shape[1]
+    _int32(page_tables, (batch, columns), "page tables")
+    _int32(lengths, (batch,), "lengths")
+    if page_tables.device != device or lengths.device != device:
+        raise ValueError("attention inputs must be on one device")
+    room = columns * cache.page_tokens
+    if longest is None or longest > room:
+        longest = room
+    if longest < 0:
+        raise ValueError("the longest length cannot be negative")
+    factor = _scale(scale, width)
+    out = torch.empty(batch, tokens, heads, width, device=device, dtype=query.dtype)
+    if out.numel() == 0:
+        return out
+    query = _rows(query)
+    need = cached_workspace_bytes(batch, tokens, heads, cache.heads, width, longest)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    q = nat.CachedQuery(
+        query.data_ptr(), query.stride(0), query.stride(1), query.stride(2),
+        page_tables.data_ptr(), lengths.data_ptr(), out.data_ptr(), batch, tokens, heads, width,
+        columns, longest, code, factor)
+    rc = nat.lib().cowsdm_cached_attention(cache, q, nat.ptr(workspace), need,
+                                     nat.stream_handle(device))
+    if rc:
+        nat.check(rc, "cowsdm_cached_attention")
+    return out

@@ -1,0 +1,644 @@
+// Causal attention over packed prompts with grouped heads.
+//
+// out[i] = sum_{j <= i} softmax_j(scale q_i . k_j) v_j, in one pass over the
+// keys with the running maximum and sum of each row.  Scores are computed
+// transposed, S^T = K Q^T, so that a lane holds keys of one query row and its
+// probabilities are the right operand of O^T = V^T P^T where they stand:
+// neither scores nor probabilities leave the registers.
+
+#include "attention.h"
+
+namespace cowsdm_impl {
+
+constexpr int kPromptWaves = 4;
+constexpr int kPromptThreads = kPromptWaves * kWave;
+
+struct PromptParams {
+  const void* query;
+  const void* key;
+  const void* value;
+  int64_t query_row, query_head, key_row, key_head, value_row, value_head;
+  const int32_t* offsets;
+  void* out;
+  int32_t rows;
+  int32_t sequences;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t width;
+  int32_t blocks;                  // query blocks of a sequence and head in the grid
+  float scale;                     // times log2(e)
+};
+
+// What a workgroup works on: a sequence, a head, and the first of its query
+// blocks (the others are `blocks` further on).
+struct PromptWork {
+  int sequence, head, kv, block;
+};
+
+// The workgroups of one sequence and key head follow one another on one XCD
+// (workgroup n runs on XCD n % 8), so that its keys and values stay in that
+// XCD's L2; later query blocks, which see more keys, come first.
+__device__ __forceinline__ PromptWork prompt_work(const PromptParams& p) {
+  const int group = p.heads / p.kv_heads;
+  const int each = p.blocks * group;
+  const int pairs = p.sequences * p.kv_heads;
+  int id = static_cast<int>(blockIdx.x), pair, rest;
+  if (pairs % 8 == 0) {
+    const int k = id >> 3;
+    pair = (k / each) * 8 + (id & 7);
+    rest = k % each;
+  } else {
+    pair = id / each;
+    rest = id % each;
+  }
+  PromptWork w;
+  w.sequence = pair / p.kv_heads;
+  w.kv = pair - w.sequence * p.kv_heads;
+  w.block = p.blocks - 1 - rest / group;
+  w.head = w.kv * group + rest % group;
+  return w;
+}
+
+// Rows before the first sequence and after the last are 0.
+template <typename T>
+__device__ void zero_rows(const PromptParams& p, const PromptWork& w) {
+  const int first = p.offsets[0], last = p.offsets[p.sequences];
+  auto zero = [&](int from, int to) {
+    for (int r = from + w.block; r < to; r += p.blocks)
+      for (int d = threadIdx.x; d < p.width; d += kPromptThreads)
+        static_cast<T*>(p.out)[(static_cast<int64_t>(r) * p.heads + w.head) * p.width + d] =
+            static_cast<T>(0.0f);
+  };
+  if (w.sequence == 0 && first > 0) zero(0, first < p.rows ? first : p.rows);
+  if (w.sequence == p.sequences - 1 && last < p.rows) zero(last > 0 ? last : 0, p.rows);
+}
+
+__device__ __forceinline__ void sequence_rows(const PromptParams& p, int sequence, int& begin,
+                                              int& length) {
+  const int a = p.offsets[sequence], b = p.offsets[sequence + 1];
+  begin = a < 0 ? 0 : a > p.rows ? p.rows : a;
+  const int end = b < begin ? begin : b > p.rows ? p.rows : b;
+  length = end - begin;
+}
+
+// ------------------------------------------------------------ 16-bit types
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__bf16> {
+  typedef bf16x8 vec;
+  static constexpr uint32_t kExponent = 0x7f807f80u;
+  static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Half<_Float16> {
+  typedef f16x8 vec;
+  static constexpr uint32_t kExponent = 0x7c007c00u;
+  static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+constexpr int kTileKeys = 64;
+
+// The 16-byte chunk of row `row` of a tile in LDS that holds the row's chunk
+// c: chunks are permuted so that the 16 rows of a key read, and the 4 rows by
+// 64 bytes of a transposing value read, fall on different banks.
+template <int DP>
+__device__ __forceinline__ int place(int row, int c) {
+  constexpr int chunks = DP / 8;
+  if constexpr (chunks % 16 == 0) return c ^ (((row & 3) << 2) | ((row >> 2) & 3));
+  else if constexpr (chunks % 8 == 0) return c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+  else return c ^ ((row >> 2) & 3);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+// 16 bytes a lane from `from` bytes past `first` to 16 times the lane past
+// `to` (the wave's), 0 where they lie past the first `bytes`.
+__device__ __forceinline__ void load_to_lds(const void* first, int bytes, uint32_t from,
+                                            lds_char* to) {
+#if defined(__HIP_DEVICE_COMPILE__)   // the host's pass does not know the load's width
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, bytes, 0x00020000),
+      (__attribute__((address_space(3))) void*)to, 16, from, 0, 0, 0);
+#endif
+}
+
+// This thread's chunks of a tile into LDS, a wave's side by side.  Rows past
+// the sequence's end and columns past the width read as 0.
+template <int kLoads>
+__device__ __forceinline__ void load_rows(const void* first, int rows, int64_t stride, int width,
+                                          const uint32_t (&from)[kLoads], lds_char* to) {
+  const int bytes = static_cast<int>((rows - 1) * stride + width) * 2;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+    load_to_lds(first, bytes, from[i], to + i * kPromptThreads * 16);
+}
+
+// One workgroup: four waves of RB * 32 query rows each of one head.  Keys and
+// values come through LDS, 64 at a time, by loads that go to LDS without
+// passing registers; the next tile is on its way while this one is used.
+template <typename T, int DP, int RB>
+__global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParams p) {
+  using vec = typename Half<T>::vec;
+  constexpr int KS = DP / 16;          // products along the width
+  constexpr int DT = DP / 32;          // tiles of the output's width
+  constexpr int kRows = kPromptWaves * RB * 32;
+  constexpr int kTileBytes = kTileKeys * DP * 2;
+  constexpr int kLoads = kTileBytes / (16 * kPromptThreads);
+  extern __shared__ __attribute__((aligned(16))) char s_tiles[];   // [2][keys, values]
+  lds_char* const tiles = (lds_char*)s_tiles;
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int col = lane & 31, half = lane >> 5;
+  const PromptWork w = prompt_work(p);
+  zero_rows<T>(p, w);
+  int begin, length;
+  sequence_rows(p, w.sequence, begin, length);
+  const T* const query = static_cast<const T*>(p.query) + begin * p.query_row +
+                         w.head * p.query_head;
+  const T* const key = static_cast<const T*>(p.key) + begin * p.key_row + w.kv * p.key_head;
+  const T* const value =
+      static_cast<const T*>(p.value) + begin * p.value_row + w.kv * p.value_head;
+  // where this thread's chunks of a tile come from, in bytes from its first row
+  uint32_t key_from[kLoads], value_from[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = i * kPromptThreads + tid;
+    const int row = at / (DP / 8), c = place<DP>(row, at % (DP / 8));
+    const bool inside = c * 8 < p.width;
+    key_from[i] = inside ? row * static_cast<uint32_t>(p.key_row * 2) + c * 16 : 0x80000000u;
+    value_from[i] = inside ? row * static_cast<uint32_t>(p.value_row * 2) + c * 16 : 0x80000000u;
+  }
+  auto load_tile = [&](int tile, int buffer) {
+    const int first = tile * kTileKeys;
+    const int rows = length - first < kTileKeys ? length - first : kTileKeys;
+    lds_char* const to = tiles + buffer * 2 * kTileBytes + wave * kWave * 16;
+    load_rows<kLoads>(key + first * p.key_row, rows, p.key_row, p.width, key_from, to);
+    load_rows<kLoads>(value + first * p.value_row, rows, p.value_row, p.width, value_from,
+                      to + kTileBytes);
+  };
+  // this lane's reads of a tile: keys by row col, values transposed four keys
+  // of 16 columns at a time
+  int key_read[KS], value_read[DT][2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) key_read[s] = col * DP * 2 + place<DP>(col, 2 * s + half) * 16;
+  {
+    const int i = lane & 15, b = (lane >> 4) & 1;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 4 * half + 8 * e + i / 4;
+        value_read[d][e] = row * DP * 2 + place<DP>(row, d * 4 + b * 2 + (i & 3) / 2) * 16 +
+                           (i & 1) * 8;
+      }
+  }
+
+  for (int block = w.block; block * kRows < length; block += p.blocks) {
+    const int q0 = block * kRows + wave * RB * 32;      // this wave's first row
+    vec q[RB][KS];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int row = q0 + r * 32 + col;
+      const T* const src = query + static_cast<int64_t>(row < length ? row : 0) * p.query_row;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = s * 16 + half * 8;
+        q[r][s] = d < p.width ? *reinterpret_cast<const vec*>(src + d) : vec{};
+      }
+    }
+    f32x16 acc[RB][DT];
+    float most[RB], sum[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      most[r] = kMinusInf;
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[r][d][i] = 0.0f;
+    }
+    const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
+    const int count = (seen + kTileKeys - 1) / kTileKeys;
+    __syncthreads();            // the tiles of the block before are used
+    load_tile(0, 0);
+    for (int tile = 0; tile < count; ++tile) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this thread's part has arrived
+      __syncthreads();                         // everyone's; the other buffer is used
+      if (tile + 1 < count) load_tile(tile + 1, (tile + 1) & 1);
+      const int k0 = tile * kTileKeys;
+      if (k0 > q0 + RB * 32 - 1 || q0 >= length) continue;
+      const bool masked = k0 + kTileKeys - 1 > q0;
+      const lds_char* const kt = tiles + (tile & 1) * 2 * kTileBytes;
+      const lds_char* const vt = kt + kTileBytes;
+      f32x16 s[RB][2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[r][kb][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const vec a = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(
+              kt + key_read[k] + kb * 32 * DP * 2);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(a, q[r][k], s[r][kb]);
+        }
+      }
+      vec prob[RB][2][2];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        if (masked) {
+          const int row = q0 + r * 32 + col;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 > row) s[r][kb][i] = kMinusInf;
+        }
+        float top = kMinusInf;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[r][kb][i]);
+        {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top),
+                                                          __float_as_uint(top), false, false);
+          top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * p.scale;
+        }
+        // the running maximum moves only when a row's grows by more than 2^8:
+        // until then its probabilities are at most 2^8, which costs no bits
+        if (__any(top > most[r] + 8.0f)) {
+          const float now = fmaxf(most[r], top);
+          const float keep = now == kMinusInf ? 1.0f : exp2_fast(most[r] - now);
+          most[r] = now;
+          sum[r] *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[r][d][i] *= keep;
+        }
+        const float shift = most[r] == kMinusInf ? 0.0f : most[r];
+        float part = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e = exp2_fast(__builtin_fmaf(s[r][kb][i], p.scale, -shift));
+            part += e;
+            prob[r][kb][i / 8][i % 8] = static_cast<T>(e);
+          }
+        sum[r] += part;
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(vt + value_read[d][0] + (kb * 32 + h * 16) * DP * 2));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(vt + value_read[d][1] + (kb * 32 + h * 16) * DP * 2));
+            struct { s16x4 a, b; } both{lo, hi};
+            vec v = __builtin_bit_cast(vec, both);
+            if (masked) {
+              // A value that is not finite reaches only the rows that see it:
+              // a product with 0 would hand its NaN to the others.  Counted
+              // by products of ones and zeros, it is added by itself.
+              u32x4 bits = __builtin_bit_cast(u32x4, v);
+              uint32_t odd = 0;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                constexpr uint32_t kHigh = Half<T>::kExponent & 0xffff0000u;
+                constexpr uint32_t kLow = Half<T>::kExponent & 0xffffu;
+                odd |= (bits[j] & kHigh) == kHigh || (bits[j] & kLow) == kLow ? 1u : 0u;
+              }
+              if (__any(odd != 0)) {
+                vec kind[3];            // NaN, +inf, -inf
+                vec rest = v;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float x = static_cast<float>(v[j]);
+                  kind[0][j] = static_cast<T>(x != x ? 1.0f : 0.0f);
+                  kind[1][j] = static_cast<T>(x == __builtin_huge_valf() ? 1.0f : 0.0f);
+                  kind[2][j] = static_cast<T>(x == kMinusInf ? 1.0f : 0.0f);
+                  if (!(__builtin_fabsf(x) < __builtin_huge_valf())) rest[j] = static_cast<T>(0.0f);
+                }
+                v = rest;
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                  const int row = q0 + r * 32 + col;
+                  vec sees;
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    const int i = h * 8 + j;
+                    sees[j] = static_cast<T>(
+                        k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 <= row ? 1.0f : 0.0f);
+                  }
+#pragma unroll
+                  for (int n = 0; n < 3; ++n) {
+                    f32x16 c;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+                    c = Half<T>::mfma(kind[n], sees, c);
+                    const float add = n == 0 ? __builtin_nanf("")
+                                             : n == 1 ? __builtin_huge_valf() : kMinusInf;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                      if (c[i] > 0.0f) acc[r][d][i] += add;
+                  }
+                }
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+              acc[r][d] = Half<T>::mfma(v, prob[r][kb][h], acc[r][d]);
+          }
+    }
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[r]),
+                                                      __float_as_uint(sum[r]), false, false);
+      const float inverse = 1.0f / (__uint_as_float(x[0]) + __uint_as_float(x[1]));
+      const int row = q0 + r * 32 + col;
+      if (row >= length) continue;
+      T* const out = static_cast<T*>(p.out) +
+                     ((static_cast<int64_t>(begin) + row) * p.heads + w.head) * p.width;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = d * 32 + i * 8 + half * 4;
+          if (at < p.width)
+            store4(out + at, f32x4{acc[r][d][4 * i], acc[r][d][4 * i + 1], acc[r][d][4 * i + 2],
+                                   acc[r][d][4 * i + 3]} * inverse);
+        }
+    }
+  }
+}
+
+// ----------------------------------------------------------------- float32
+
+constexpr int kFloatKeys = 32;
+
+// Float32 on the float32 matrix instructions: four waves of 16 query rows, 32
+// keys at a time through LDS.
+template <int DP>
+__global__ __launch_bounds__(kPromptThreads) void prompt_float_kernel(PromptParams p) {
+  constexpr int kRows = kPromptWaves * 16;
+  constexpr int KS = DP / 16;
+  constexpr int DT = DP / 16;
+  constexpr int kStride = DP + 4;      // rows of four apart fall on other banks
+  extern __shared__ __attribute__((aligned(16))) char s_tiles[];
+  float* const s_key = reinterpret_cast<float*>(s_tiles);
+  float* const s_value = s_key + kFloatKeys * kStride;
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & (kWave - 1);
+  const int wave = tid / kWave;
+  const int col = lane & 15, quarter = lane >> 4;
+  const PromptWork w = prompt_work(p);
+  zero_rows<float>(p, w);
+  int begin, length;
+  sequence_rows(p, w.sequence, begin, length);
+  const float* const query =
+      static_cast<const float*>(p.query) + begin * p.query_row + w.head * p.query_head;
+  const float* const key =
+      static_cast<const float*>(p.key) + begin * p.key_row + w.kv * p.key_head;
+  const float* const value =
+      static_cast<const float*>(p.value) + begin * p.value_row + w.kv * p.value_head;
+
+  for (int block = w.block; block * kRows < length; block += p.blocks) {
+    const int q0 = block * kRows + wave * 16;
+    const int row = q0 + col;
+    f32x4 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = s * 16 + quarter * 4;
+      q[s] = d < p.width ? *reinterpret_cast<const f32x4*>(
+                               query + static_cast<int64_t>(row < length ? row : 0) *
+                                           p.query_row + d)
+                         : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    f32x4 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float most = kMinusInf, sum = 0.0f;
+    const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
+    for (int k0 = 0; k0 < seen; k0 += kFloatKeys) {
+      __syncthreads();
+      for (int i = tid; i < kFloatKeys * (DP / 4); i += kPromptThreads) {
+        const int r = i / (DP / 4), c = (i % (DP / 4)) * 4;
+        f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
+        if (k0 + r < length && c < p.width) {
+          a = *reinterpret_cast<const f32x4*>(key + (k0 + r) * p.key_row + c);
+          b = *reinterpret_cast<const f32x4*>(value + (k0 + r) * p.value_row + c);
+        }
+        *reinterpret_cast<f32x4*>(s_key + r * kStride + c) = a;
+        *reinterpret_cast<f32x4*>(s_value + r * kStride + c) = b;
+      }
+      __syncthreads();
+      if (k0 > q0 + 15 || q0 >= length) continue;
+      const bool masked = k0 + kFloatKeys - 1 > q0;
+      f32x4 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(s_key + (t * 16 + col) * kStride +
+                                                          k * 16 + quarter * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], q[k][j], s[t], 0, 0, 0);
+        }
+        if (masked)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k0 + t * 16 + quarter * 4 + i > row) s[t][i] = kMinusInf;
+      }
+      float top = kMinusInf;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
+      top = max_over_rows(top) * p.scale;
+      if (__any(top > most)) {
+        const float now = fmaxf(most, top);
+        const float keep = now == kMinusInf ? 1.0f : exp2_fast(most - now);
+        most = now;
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= keep;
+      }
+      const float shift = most == kMinusInf ? 0.0f : most;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], p.scale, -shift));
+          sum += s[t][i];
+        }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v = s_value[(t * 16 + quarter * 4 + i) * kStride + d * 16 + col];
+            if (masked && __any(!(__builtin_fabsf(v) < __builtin_huge_valf()))) {
+              // as in the 16-bit kernel
+              const float sees = k0 + t * 16 + quarter * 4 + i <= row ? 1.0f : 0.0f;
+              const float kind[3] = {v != v ? 1.0f : 0.0f,
+                                     v == __builtin_huge_valf() ? 1.0f : 0.0f,
+                                     v == kMinusInf ? 1.0f : 0.0f};
+              if (!(__builtin_fabsf(v) < __builtin_huge_valf())) v = 0.0f;
+#pragma unroll
+              for (int n = 0; n < 3; ++n) {
+                f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+                c = __builtin_amdgcn_mfma_f32_16x16x4f32(kind[n], sees, c, 0, 0, 0);
+                const float add = n == 0 ? __builtin_nanf("")
+                                         : n == 1 ? __builtin_huge_valf() : kMinusInf;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (c[j] > 0.0f) acc[d][j] += add;
+              }
+            }
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[t][i], acc[d], 0, 0, 0);
+          }
+    }
+    const float inverse = 1.0f / sum_over_rows(sum);
+    if (row < length) {
+      float* const out = static_cast<float*>(p.out) +
+                         ((static_cast<int64_t>(begin) + row) * p.heads + w.head) * p.width;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int at = d * 16 + quarter * 4;
+        if (at < p.width) *reinterpret_cast<f32x4*>(out + at) = acc[d] * inverse;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launches
+
+int32_t launch_prompt_kernel(void (*kernel)(PromptParams), int bytes, const PromptParams& p,
+                             hipStream_t stream) {
+  const int64_t grid = static_cast<int64_t>(p.blocks) * p.heads * p.sequences;
+  if (grid > INT32_MAX) return fail(COWSDM_ELIMIT, "prompt_attention: too many workgroups");
+  if (bytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess)
+      return fail(static_cast<int32_t>(e), "prompt_attention: %s", hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(kPromptThreads), bytes,
+                     stream, p);
+  return launch_status("prompt_attention");
+}
+
+template <int DP>
+int32_t launch_prompt_float(PromptParams p, int64_t longest, hipStream_t stream) {
+  constexpr int kRows = kPromptWaves * 16;
+  constexpr int kBytes = 2 * kFloatKeys * (DP + 4) * 4;
+  p.blocks = static_cast<int32_t>((longest + kRows - 1) / kRows);
+  return launch_prompt_kernel(&prompt_float_kernel<DP>, kBytes, p, stream);
+}
+
+template <typename T, int DP, int RB>
+int32_t launch_prompt_half(PromptParams p, int64_t longest, hipStream_t stream) {
+  constexpr int kRows = kPromptWaves * RB * 32;
+  constexpr int kBytes = 2 * 2 * kTileKeys * DP * 2;
+  p.blocks = static_cast<int32_t>((longest + kRows - 1) / kRows);
+  return launch_prompt_kernel(&prompt_half_kernel<T, DP, RB>, kBytes, p, stream);
+}
+
+template <typename T>
+int32_t launch_prompt(const PromptParams& p, int64_t longest, hipStream_t stream) {
+  const int w = p.width;
+  if constexpr (sizeof(T) == 4) {
+    if (w <= 32) return launch_prompt_float<32>(p, longest, stream);
+    if (w <= 64) return launch_prompt_float<64>(p, longest, stream);
+    if (w <= 96) return launch_prompt_float<96>(p, longest, stream);
+    if (w <= 128) return launch_prompt_float<128>(p, longest, stream);
+    if (w <= 192) return launch_prompt_float<192>(p, longest, stream);
+    return launch_prompt_float<256>(p, longest, stream);
+  } else {
+    if (w <= 32) return launch_prompt_half<T, 32, 1>(p, longest, stream);
+    if (w <= 64) return launch_prompt_half<T, 64, 1>(p, longest, stream);
+    if (w <= 96) return launch_prompt_half<T, 96, 1>(p, longest, stream);
+    if (w <= 128) return launch_prompt_half<T, 128, 1>(p, longest, stream);
+    if (w <= 192) return launch_prompt_half<T, 192, 1>(p, longest, stream);
+    return launch_prompt_half<T, 256, 1>(p, longest, stream);
+  }
+}
+
+}  // namespace cowsdm_impl
+
+using namespace cowsdm_impl;
+
+extern "C" int32_t cowsdm_prompt_attention(const cowsdm_prompt_attention_t* attention,
+                                           void* stream) {
+  if (!attention) return fail(COWSDM_EARG, "prompt_attention: null argument");
+  const cowsdm_prompt_attention_t& a = *attention;
+  if (a.rows < 0 || a.sequences < 0 || a.longest < 0 || a.heads <= 0 || a.kv_heads <= 0)
+    return fail(COWSDM_EARG, "prompt_attention: bad size");
+  if (a.heads % a.kv_heads != 0)
+    return fail(COWSDM_EARG, "prompt_attention: query heads must be a multiple of key heads");
+  if (a.width <= 0 || a.width % 8 != 0)
+    return fail(COWSDM_EARG, "prompt_attention: head width must be a multiple of 8");
+  if (a.width > 256) return fail(COWSDM_ELIMIT, "prompt_attention: head width at most 256");
+  if (a.rows > (1 << 30) || a.sequences > (1 << 30) || a.heads > (1 << 20) ||
+      a.query_row >= (1 << 23) || a.key_row >= (1 << 23) || a.value_row >= (1 << 23))
+    return fail(COWSDM_ELIMIT, "prompt_attention: too large");
+  if (a.float_type != COWSDM_FLOAT32 && a.float_type != COWSDM_FLOAT16 &&
+      a.float_type != COWSDM_BFLOAT16)
+    return fail(COWSDM_EARG, "prompt_attention: bad float type");
+  if (!(a.scale > 0.0f) || a.scale > 3.0e38f)
+    return fail(COWSDM_EARG, "prompt_attention: the scale must be positive");
+  if (a.rows == 0) return 0;
+  if (a.sequences == 0) return fail(COWSDM_EARG, "prompt_attention: rows without a sequence");
+  if (!a.query || !a.key || !a.value || !a.offsets || !a.out)
+    return fail(COWSDM_EARG, "prompt_attention: null pointer argument");
+  const int64_t unit = a.float_type == COWSDM_FLOAT32 ? 4 : 8;
+  const int64_t strides[] = {a.query_row, a.query_head, a.key_row,
+                             a.key_head,  a.value_row,  a.value_head};
+  for (int64_t s : strides)
+    if (s < 0 || s % unit != 0)
+      return fail(COWSDM_EARG, "prompt_attention: strides must be multiples of 16 bytes");
+  const void* pointers[] = {a.query, a.key, a.value, a.out};
+  for (const void* x : pointers)
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0)
+      return fail(COWSDM_EARG, "prompt_attention: tensors must be 16-byte aligned");
+  PromptParams p{};
+  p.query = a.query;
+  p.key = a.key;
+  p.value = a.value;
+  p.query_row = a.query_row;
+  p.query_head = a.query_head;
+  p.key_row = a.key_row;
+  p.key_head = a.key_head;
+  p.value_row = a.value_row;
+  p.value_head = a.value_head;
+  p.offsets = a.offsets;
+  p.out = a.out;
+  p.rows = static_cast<int32_t>(a.rows);
+  p.sequences = static_cast<int32_t>(a.sequences);
+  p.heads = static_cast<int32_t>(a.heads);
+  p.kv_heads = static_cast<int32_t>(a.kv_heads);
+  p.width = static_cast<int32_t>(a.width);
+  p.scale = a.scale * kLog2E;
+  const int64_t longest = a.longest < 1 ? 1 : a.longest < a.rows ? a.longest : a.rows;
+  const auto s = static_cast<hipStream_t>(stream);
+  if (a.float_type == COWSDM_FLOAT32) return launch_prompt<float>(p, longest, s);
+  if (a.float_type == COWSDM_FLOAT16) return launch_prompt<_Float16>(p, longest, s);
+  return launch_prompt<__bf16>(p, longest, s);
+}

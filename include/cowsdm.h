@@ -780,6 +780,126 @@ int32_t cowsdm_dense_routes(const float* weights, const void* indices, int32_t i
                             int64_t rows, int64_t per_row, int64_t slots, float* dense,
                             int32_t* bad, void* stream);
 
+/* ------------------------------------------------------------ attention */
+
+/* The attention layers of a stack ("A" in its layout), which the reference
+ * runs in its model (CausalSelfAttention, model.py:47-189): a whole prompt,
+ * and single tokens over a cache.  The cache here is paged and held in 8
+ * bits.  Float types are COWSDM_FLOAT_* codes; rows of query, key and value
+ * are contiguous, 16-byte aligned and a multiple of 8 elements wide, with
+ * any strides of a multiple of 8 elements (4 for float32). */
+
+/* Causal attention over packed prompts with grouped heads.  Sequence s holds
+ * rows offsets[s] to offsets[s + 1] - 1 of query [rows, heads, width] and of
+ * key and value [rows, kv_heads, width]; query head h reads key head
+ * h / (heads / kv_heads):
+ *   out[i, h] = sum_{j <= i in s} softmax_j(scale * query[i, h] . key[j]) value[j]
+ * Rows of no sequence are 0.  `longest` is the longest sequence's length, or
+ * more; a smaller value costs time, not correctness. */
+typedef struct cowsdm_prompt_attention {
+  const void* query;
+  const void* key;
+  const void* value;
+  int64_t query_row, query_head;   /* strides, in elements                 */
+  int64_t key_row, key_head;
+  int64_t value_row, value_head;
+  const int32_t* offsets;          /* [sequences + 1], ascending           */
+  void* out;                       /* [rows, heads, width], contiguous     */
+  int64_t rows;
+  int64_t sequences;
+  int64_t longest;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t width;                   /* a multiple of 8, at most 256         */
+  int32_t float_type;
+  float scale;                     /* positive                             */
+} cowsdm_prompt_attention_t;
+
+/* Runs cowsdm_prompt_attention_t; COWSDM_ELIMIT for a width over 256. */
+int32_t cowsdm_prompt_attention(const cowsdm_prompt_attention_t* attention, void* stream);
+
+/* A step's page tables and token slots.  Request r holds lengths[r] tokens in
+ * the pages page_tables[r][0 .. ceil(lengths[r] / page_tokens) - 1] and gets
+ * added[r] more.  New pages come from the top of the free stack
+ * free_pages[0 .. *free_count - 1] in request order and are written to the
+ * tables in place.  lengths_out [requests] and *free_count_out get the sums
+ * (they are not lengths and free_count themselves), offsets [requests + 1]
+ * the new tokens before each request, and token t of the packed new tokens
+ * its position in its request and its slot page * page_tokens + position %
+ * page_tokens; tokens past the last are -1.  Where the pages, a table's
+ * columns or `tokens` do not suffice, or a count is negative, *overflow is 1,
+ * positions and slots are -1 and nothing else changes.  At most 4,096
+ * requests; page_tokens is 16, 32, 64, 128 or 256. */
+int32_t cowsdm_page_tables_extend(
+    const int32_t* lengths, const int32_t* added, int64_t requests, int32_t* page_tables,
+    int64_t columns, const int32_t* free_pages, int64_t pages, const int32_t* free_count,
+    int64_t page_tokens, int64_t tokens, int32_t* lengths_out, int32_t* free_count_out,
+    int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* overflow, void* stream);
+
+/* The pages of the n named requests (distinct) return to the top of the free
+ * stack in that order; their lengths become 0 and their table entries -1. */
+int32_t cowsdm_pages_release(int32_t* lengths, int32_t* page_tables, int64_t requests,
+                             int64_t columns, const int32_t* named, int64_t n,
+                             int32_t* free_pages, int64_t pages, int32_t* free_count,
+                             int64_t page_tokens, void* stream);
+
+/* One layer's cache: e4m3 codes, keys [pages, heads, page_tokens, width],
+ * values transposed [pages, heads, width, page_tokens], and a power of two
+ * for each page and head, [pages, heads], by which its codes count.  width is
+ * a head's width padded to 32, 64, 96, 128, 192 or 256; the padding holds
+ * zeros. */
+typedef struct cowsdm_kv_cache {
+  int64_t pages;
+  int64_t heads;
+  int64_t page_tokens;
+  int64_t width;
+  void* key_codes;
+  float* key_scales;
+  void* value_codes;
+  float* value_scales;
+} cowsdm_kv_cache_t;
+
+/* Writes keys and values [tokens, heads, width] into their slots (-1: not
+ * written).  A page's tokens of one call follow one another.  The scale of a
+ * page whose first token is written is the least power of two, from 2^-100 to
+ * 2^119, under which the call's largest finite magnitude is at most 448; a
+ * page that goes on keeps the larger of its own and that one, and its other
+ * codes are taken to it.  Codes round to nearest even; infinities and NaN
+ * become NaN. */
+int32_t cowsdm_kv_write(const cowsdm_kv_cache_t* cache, const void* key, int64_t key_row,
+                        int64_t key_head, const void* value, int64_t value_row,
+                        int64_t value_head, int32_t float_type, int64_t width,
+                        const int32_t* slots, int64_t tokens, void* stream);
+
+/* The newest `tokens` tokens of each request over the cache: query row i of
+ * request r sees positions 0 .. lengths[r] - tokens + i.  A row that sees
+ * nothing gives 0.  `longest` is the longest length, or more; a smaller value
+ * costs time, not correctness. */
+typedef struct cowsdm_cached_query {
+  const void* query;               /* [requests, tokens, heads, width]     */
+  int64_t query_request, query_token, query_head;   /* strides, in elements */
+  const int32_t* page_tables;      /* [requests, columns]                  */
+  const int32_t* lengths;          /* [requests]                           */
+  void* out;                       /* [requests, tokens, heads, width]     */
+  int64_t requests;
+  int64_t tokens;
+  int64_t heads;                   /* a multiple of the cache's            */
+  int64_t width;
+  int64_t columns;
+  int64_t longest;
+  int32_t float_type;
+  float scale;                     /* positive                             */
+} cowsdm_cached_query_t;
+
+/* Bytes of workspace that a call of cowsdm_cached_attention needs (0: none). */
+int64_t cowsdm_cached_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t heads,
+                                                int64_t kv_heads, int64_t cache_width,
+                                                int64_t longest);
+
+int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
+                                const cowsdm_cached_query_t* query, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,10 @@ Modules:
   and float32 exp: a second restatement for cross-checking, and the CPU
   dense-table baseline timed by bench.py.
 
+* ``oracle.attention`` -- float64 definitions of the attention operators:
+  causal attention over packed prompts, attention over the 8-bit cache, page
+  tables and the cache's codes, row by row.
+
 Every function of ``oracle.state`` is pinned by at least one check that does
 not restate its formula (see tests/test_oracle_pins.py): the reference's own
 known answers (tests/test_allocator.py:65-99), the independent serial
