@@ -139,14 +139,206 @@ __device__ __forceinline__ void load_rows(const void* first, int rows, int64_t s
     load_to_lds(first, bytes, from[i], to + i * kPromptThreads * 16);
 }
 
+// Four keys of this lane's column from a tile in LDS, each group of 16 lanes
+// reading four rows of 16 columns.
+__device__ __forceinline__ s16x4 read_turned(const lds_char* __restrict at) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+}
+
+// Of eight 16-bit numbers, whether one is not finite.
+template <typename T>
+__device__ __forceinline__ bool any_odd(typename Half<T>::vec v) {
+  constexpr uint32_t kHigh = Half<T>::kExponent & 0xffff0000u;
+  constexpr uint32_t kLow = Half<T>::kExponent & 0xffffu;
+  const u32x4 bits = __builtin_bit_cast(u32x4, v);
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    odd |= (bits[j] & kHigh) == kHigh | (bits[j] & kLow) == kLow;
+  return odd;
+}
+
+// One wave's RB * 32 query rows of one head: q the rows, acc their products
+// so far, transposed, most the maxima that the probabilities are relative to
+// and sum their sums (of this lane's keys).
+template <typename T, int DP, int RB>
+struct PromptRows {
+  using vec = typename Half<T>::vec;
+  static constexpr int KS = DP / 16;       // products along the width
+  static constexpr int DT = DP / 32;       // tiles of the output's width
+  vec q[RB][KS];
+  f32x16 acc[RB][DT];
+  float most[RB], sum[RB];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      most[r] = kMinusInf;
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[r][d][i] = 0.0f;
+    }
+  }
+
+  // The value operand of step h (16 keys) of column tile d.
+  __device__ __forceinline__ vec turned(const lds_char* values, const int (&at)[DT][2], int h,
+                                        int d) {
+    struct { s16x4 a, b; } both{read_turned(values + at[d][0] + h * 16 * DP * 2),
+                                read_turned(values + at[d][1] + h * 16 * DP * 2)};
+    return __builtin_bit_cast(vec, both);
+  }
+
+  // One tile of 64 keys from row k0 on.  Masked: some of the rows, from q0 on,
+  // do not see all of it.
+  template <bool kMasked>
+  __device__ __forceinline__ void tile(const lds_char* keys, const lds_char* values,
+                                       const int (&key_read)[KS],
+                                       const int (&value_read)[DT][2], float scale, int k0,
+                                       int q0) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int col = lane & 31, half = lane >> 5;
+    f32x16 s[RB][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[r][kb][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const vec a = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(
+            keys + key_read[k] + kb * 32 * DP * 2);
+#pragma unroll
+        for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(a, q[r][k], s[r][kb]);
+      }
+    }
+    bool poisoned = false;
+    if constexpr (kMasked) {
+#pragma unroll 1
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          poisoned |= any_odd<T>(turned(values, value_read, h, d));
+      poisoned = __any(poisoned);
+    }
+    vec prob[RB][4];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      if constexpr (kMasked) {
+        const int row = q0 + r * 32 + col;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 > row) s[r][kb][i] = kMinusInf;
+      }
+      float top = kMinusInf;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[r][kb][i]);
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
+                                                      false, false);
+      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * scale;
+      // The maximum that the probabilities are relative to moves only when a
+      // row's grows past 2^8 of it: sums of numbers up to 2^8 lose nothing in
+      // 32 bits, and a probability keeps its bits in 16.
+      if (__any(top > most[r] + 8.0f)) {
+        const float now = fmaxf(most[r], top);
+        const float keep = now == kMinusInf ? 1.0f : exp2_fast(most[r] - now);
+        most[r] = now;
+        sum[r] *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[r][d][i] *= keep;
+      }
+      const float shift = most[r] == kMinusInf ? 0.0f : most[r];
+      float part[4] = {};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = exp2_fast(__builtin_fmaf(s[r][kb][i], scale, -shift));
+          part[i % 4] += e;
+          prob[r][2 * kb + i / 8][i % 8] = static_cast<T>(e);
+        }
+      sum[r] += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        vec v = turned(values, value_read, h, d);
+        if (kMasked && poisoned) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(__builtin_fabsf(static_cast<float>(v[j])) < __builtin_huge_valf()))
+              v[j] = static_cast<T>(0.0f);
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) acc[r][d] = Half<T>::mfma(v, prob[r][h], acc[r][d]);
+      }
+    if constexpr (kMasked) {
+      if (poisoned) add_odd(values, value_read, k0, q0);
+    }
+  }
+
+  // Values that are not finite, for the rows that see them: a product with a
+  // probability of 0 would hand their NaN to the others.  Products of ones and
+  // zeros count them, and what is counted is added by itself.
+  __device__ __forceinline__ void add_odd(const lds_char* values, const int (&value_read)[DT][2],
+                                          int k0, int q0) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int col = lane & 31, half = lane >> 5;
+#pragma unroll 1
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const vec v = turned(values, value_read, h, d);
+        if (!__any(any_odd<T>(v))) continue;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          vec sees;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            sees[j] = static_cast<T>(
+                k0 + h * 16 + (j / 4) * 8 + half * 4 + j % 4 <= q0 + r * 32 + col ? 1.0f : 0.0f);
+#pragma unroll 1
+          for (int n = 0; n < 3; ++n) {
+            vec kind;
+            const float sign = n == 1 ? __builtin_huge_valf() : kMinusInf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float x = static_cast<float>(v[j]);
+              kind[j] = static_cast<T>((n == 0 ? x != x : x == sign) ? 1.0f : 0.0f);
+            }
+            f32x16 c;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+            c = Half<T>::mfma(kind, sees, c);
+            const float add = n == 0 ? __builtin_nanf("") : sign;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (c[i] > 0.0f) acc[r][d][i] += add;
+          }
+        }
+      }
+  }
+};
+
 // One workgroup: four waves of RB * 32 query rows each of one head.  Keys and
 // values come through LDS, 64 at a time, by loads that go to LDS without
 // passing registers; the next tile is on its way while this one is used.
 template <typename T, int DP, int RB>
-__global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParams p) {
+__global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half_kernel(
+    PromptParams p) {
+  using Rows = PromptRows<T, DP, RB>;
   using vec = typename Half<T>::vec;
-  constexpr int KS = DP / 16;          // products along the width
-  constexpr int DT = DP / 32;          // tiles of the output's width
+  constexpr int KS = Rows::KS, DT = Rows::DT;
   constexpr int kRows = kPromptWaves * RB * 32;
   constexpr int kTileBytes = kTileKeys * DP * 2;
   constexpr int kLoads = kTileBytes / (16 * kPromptThreads);
@@ -183,8 +375,8 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParam
     load_rows<kLoads>(value + first * p.value_row, rows, p.value_row, p.width, value_from,
                       to + kTileBytes);
   };
-  // this lane's reads of a tile: keys by row col, values transposed four keys
-  // of 16 columns at a time
+  // this lane's reads of a tile: keys by row col, values turned four keys of
+  // 16 columns at a time
   int key_read[KS], value_read[DT][2];
 #pragma unroll
   for (int s = 0; s < KS; ++s) key_read[s] = col * DP * 2 + place<DP>(col, 2 * s + half) * 16;
@@ -202,7 +394,8 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParam
 
   for (int block = w.block; block * kRows < length; block += p.blocks) {
     const int q0 = block * kRows + wave * RB * 32;      // this wave's first row
-    vec q[RB][KS];
+    Rows rows;
+    rows.clear();
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int row = q0 + r * 32 + col;
@@ -210,19 +403,8 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParam
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d = s * 16 + half * 8;
-        q[r][s] = d < p.width ? *reinterpret_cast<const vec*>(src + d) : vec{};
+        rows.q[r][s] = d < p.width ? *reinterpret_cast<const vec*>(src + d) : vec{};
       }
-    }
-    f32x16 acc[RB][DT];
-    float most[RB], sum[RB];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      most[r] = kMinusInf;
-      sum[r] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[r][d][i] = 0.0f;
     }
     const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
     const int count = (seen + kTileKeys - 1) / kTileKeys;
@@ -233,141 +415,16 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParam
       __syncthreads();                         // everyone's; the other buffer is used
       if (tile + 1 < count) load_tile(tile + 1, (tile + 1) & 1);
       const int k0 = tile * kTileKeys;
-      if (k0 > q0 + RB * 32 - 1 || q0 >= length) continue;
-      const bool masked = k0 + kTileKeys - 1 > q0;
-      const lds_char* const kt = tiles + (tile & 1) * 2 * kTileBytes;
-      const lds_char* const vt = kt + kTileBytes;
-      f32x16 s[RB][2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[r][kb][i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const vec a = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(
-              kt + key_read[k] + kb * 32 * DP * 2);
-#pragma unroll
-          for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(a, q[r][k], s[r][kb]);
-        }
-      }
-      vec prob[RB][2][2];
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        if (masked) {
-          const int row = q0 + r * 32 + col;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 > row) s[r][kb][i] = kMinusInf;
-        }
-        float top = kMinusInf;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[r][kb][i]);
-        {
-          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top),
-                                                          __float_as_uint(top), false, false);
-          top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * p.scale;
-        }
-        // the running maximum moves only when a row's grows by more than 2^8:
-        // until then its probabilities are at most 2^8, which costs no bits
-        if (__any(top > most[r] + 8.0f)) {
-          const float now = fmaxf(most[r], top);
-          const float keep = now == kMinusInf ? 1.0f : exp2_fast(most[r] - now);
-          most[r] = now;
-          sum[r] *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[r][d][i] *= keep;
-        }
-        const float shift = most[r] == kMinusInf ? 0.0f : most[r];
-        float part = 0.0f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = exp2_fast(__builtin_fmaf(s[r][kb][i], p.scale, -shift));
-            part += e;
-            prob[r][kb][i / 8][i % 8] = static_cast<T>(e);
-          }
-        sum[r] += part;
-      }
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s16x4*)(vt + value_read[d][0] + (kb * 32 + h * 16) * DP * 2));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s16x4*)(vt + value_read[d][1] + (kb * 32 + h * 16) * DP * 2));
-            struct { s16x4 a, b; } both{lo, hi};
-            vec v = __builtin_bit_cast(vec, both);
-            if (masked) {
-              // A value that is not finite reaches only the rows that see it:
-              // a product with 0 would hand its NaN to the others.  Counted
-              // by products of ones and zeros, it is added by itself.
-              u32x4 bits = __builtin_bit_cast(u32x4, v);
-              uint32_t odd = 0;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                constexpr uint32_t kHigh = Half<T>::kExponent & 0xffff0000u;
-                constexpr uint32_t kLow = Half<T>::kExponent & 0xffffu;
-                odd |= (bits[j] & kHigh) == kHigh || (bits[j] & kLow) == kLow ? 1u : 0u;
-              }
-              if (__any(odd != 0)) {
-                vec kind[3];            // NaN, +inf, -inf
-                vec rest = v;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float x = static_cast<float>(v[j]);
-                  kind[0][j] = static_cast<T>(x != x ? 1.0f : 0.0f);
-                  kind[1][j] = static_cast<T>(x == __builtin_huge_valf() ? 1.0f : 0.0f);
-                  kind[2][j] = static_cast<T>(x == kMinusInf ? 1.0f : 0.0f);
-                  if (!(__builtin_fabsf(x) < __builtin_huge_valf())) rest[j] = static_cast<T>(0.0f);
-                }
-                v = rest;
-#pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                  const int row = q0 + r * 32 + col;
-                  vec sees;
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) {
-                    const int i = h * 8 + j;
-                    sees[j] = static_cast<T>(
-                        k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 <= row ? 1.0f : 0.0f);
-                  }
-#pragma unroll
-                  for (int n = 0; n < 3; ++n) {
-                    f32x16 c;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) c[i] = 0.0f;
-                    c = Half<T>::mfma(kind[n], sees, c);
-                    const float add = n == 0 ? __builtin_nanf("")
-                                             : n == 1 ? __builtin_huge_valf() : kMinusInf;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                      if (c[i] > 0.0f) acc[r][d][i] += add;
-                  }
-                }
-              }
-            }
-#pragma unroll
-            for (int r = 0; r < RB; ++r)
-              acc[r][d] = Half<T>::mfma(v, prob[r][kb][h], acc[r][d]);
-          }
+      const lds_char* const keys = tiles + (tile & 1) * 2 * kTileBytes;
+      if (k0 + kTileKeys - 1 <= q0)
+        rows.template tile<false>(keys, keys + kTileBytes, key_read, value_read, p.scale, k0, q0);
+      else if (k0 <= q0 + RB * 32 - 1 && q0 < length)
+        rows.template tile<true>(keys, keys + kTileBytes, key_read, value_read, p.scale, k0, q0);
     }
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[r]),
-                                                      __float_as_uint(sum[r]), false, false);
+      const auto x = __builtin_amdgcn_permlane32_swap(
+          __float_as_uint(rows.sum[r]), __float_as_uint(rows.sum[r]), false, false);
       const float inverse = 1.0f / (__uint_as_float(x[0]) + __uint_as_float(x[1]));
       const int row = q0 + r * 32 + col;
       if (row >= length) continue;
@@ -378,9 +435,9 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_half_kernel(PromptParam
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = d * 32 + i * 8 + half * 4;
+          const f32x16& a = rows.acc[r][d];
           if (at < p.width)
-            store4(out + at, f32x4{acc[r][d][4 * i], acc[r][d][4 * i + 1], acc[r][d][4 * i + 2],
-                                   acc[r][d][4 * i + 3]} * inverse);
+            store4(out + at, f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]} * inverse);
         }
     }
   }
