@@ -408,17 +408,32 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
     }
     const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
     const int count = (seen + kTileKeys - 1) / kTileKeys;
+    // Tiles before the block's first row are seen by all of its rows; what
+    // follows, to the diagonal, has a loop of its own.  Both take a multiple
+    // of two tiles, so that a buffer's address is part of the instructions.
+    const int whole = block * (kRows / kTileKeys);
     __syncthreads();            // the tiles of the block before are used
     load_tile(0, 0);
-    for (int tile = 0; tile < count; ++tile) {
+    auto arrived = [&](int tile, int buffer) {
       __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this thread's part has arrived
       __syncthreads();                         // everyone's; the other buffer is used
-      if (tile + 1 < count) load_tile(tile + 1, (tile + 1) & 1);
+      if (tile + 1 < count) load_tile(tile + 1, buffer ^ 1);
+    };
+    for (int tile = 0; tile < whole; tile += 2) {
+#pragma unroll
+      for (int buffer = 0; buffer < 2; ++buffer) {
+        arrived(tile + buffer, buffer);
+        const lds_char* const keys = tiles + buffer * 2 * kTileBytes;
+        rows.template tile<false>(keys, keys + kTileBytes, key_read, value_read, p.scale,
+                                  (tile + buffer) * kTileKeys, q0);
+      }
+    }
+#pragma unroll 1
+    for (int tile = whole; tile < count; ++tile) {
+      arrived(tile, tile & 1);
       const int k0 = tile * kTileKeys;
       const lds_char* const keys = tiles + (tile & 1) * 2 * kTileBytes;
-      if (k0 + kTileKeys - 1 <= q0)
-        rows.template tile<false>(keys, keys + kTileBytes, key_read, value_read, p.scale, k0, q0);
-      else if (k0 <= q0 + RB * 32 - 1 && q0 < length)
+      if (k0 <= q0 + RB * 32 - 1 && q0 < length)
         rows.template tile<true>(keys, keys + kTileBytes, key_read, value_read, p.scale, k0, q0);
     }
 #pragma unroll
