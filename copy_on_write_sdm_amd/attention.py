@@ -34,6 +34,7 @@ import torch
 from . import _native as nat
 
 CODES = torch.float8_e4m3fn
+_INT32, _FLOAT32 = torch.int32, torch.float32
 MAX_REQUESTS = 4_096
 PAGE_TOKENS = (16, 32, 64, 128, 256)
 CACHE_WIDTHS = (32, 64, 96, 128, 192, 256)
@@ -84,12 +85,13 @@ def _rows(tensor: torch.Tensor) -> torch.Tensor:
     return tensor.clone() if tensor.data_ptr() % 16 else tensor
 
 
-def _int32(tensor: torch.Tensor, shape: tuple[int, ...], what: str) -> None:
-    if tensor.dtype != torch.int32 or tensor.shape != shape or not tensor.is_contiguous():
+def _int32(tensor: torch.Tensor, shape: tuple[int, ...], device: int, what: str) -> None:
+    if tensor.dtype is not _INT32 or tensor.shape != shape or not tensor.is_contiguous():
         raise ValueError(f"{what} must be contiguous int32 of shape {list(shape)}")
+    if tensor.get_device() != device:
+        raise ValueError(f"{what} must be on the other inputs' device")
 
 
-@torch.no_grad()
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                      offsets: torch.Tensor, *, longest: int | None = None,
                      scale: float | None = None) -> torch.Tensor:
@@ -115,13 +117,13 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     code = _float_type(query.dtype)
     if key.dtype != query.dtype or value.dtype != query.dtype:
         raise TypeError("attention query, key and value share one type")
-    device = query.device
     _need_device(query, "attention inputs")
-    if key.device != device or value.device != device or offsets.device != device:
+    device, index = query.device, query.get_device()
+    if key.get_device() != index or value.get_device() != index:
         raise ValueError("attention inputs must be on one device")
     if offsets.ndim != 1 or offsets.numel() == 0:
         raise ValueError("attention offsets must be a vector of sequences + 1")
-    _int32(offsets, offsets.shape, "attention offsets")
+    _int32(offsets, offsets.shape, index, "attention offsets")
     if longest is not None and longest < 0:
         raise ValueError("the longest sequence cannot be negative")
     factor = _scale(scale, width)
@@ -157,7 +159,6 @@ class PageTableStep(NamedTuple):
     overflow: torch.Tensor
 
 
-@torch.no_grad()
 def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: torch.Tensor,
                        free_pages: torch.Tensor, free_count: torch.Tensor, *, page_tokens: int,
                        tokens: int, out: Sequence[torch.Tensor] | None = None) -> PageTableStep:
@@ -172,43 +173,37 @@ def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: 
     stay as they were.  ``out``: the tensors to write, in the order of
     ``PageTableStep``, none of them an input."""
 
-    batch = lengths.numel()
     if lengths.ndim != 1 or page_tables.ndim != 2 or free_pages.ndim != 1:
         raise ValueError("page tables take lengths [B], page_tables [B,columns], free_pages [P]")
     _need_device(lengths, "page tables")
-    _int32(lengths, (batch,), "lengths")
-    _int32(added, (batch,), "added tokens")
-    _int32(page_tables, (batch, page_tables.shape[1]), "page tables")
-    _int32(free_pages, free_pages.shape, "free pages")
-    if free_count.dtype != torch.int32 or free_count.numel() != 1:
-        raise ValueError("the free count must be one int32")
+    batch, device, index = lengths.numel(), lengths.device, lengths.get_device()
+    columns, pages = page_tables.shape[1], free_pages.numel()
+    _int32(lengths, (batch,), index, "lengths")
+    _int32(added, (batch,), index, "added tokens")
+    _int32(page_tables, (batch, columns), index, "page tables")
+    _int32(free_pages, (pages,), index, "free pages")
+    _int32(free_count, (1,), index, "the free count")
     if page_tokens not in PAGE_TOKENS:
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
     if tokens < 0:
         raise ValueError("the token count cannot be negative")
     if batch > MAX_REQUESTS:
         raise ValueError(f"page tables take at most {MAX_REQUESTS} requests")
-    device = lengths.device
+    sizes = (batch, 1, batch + 1, tokens, tokens, 1)
     if out is None:
-        sizes = (batch, 1, batch + 1, tokens, tokens, 1)
-        step = PageTableStep(*torch.empty(sum(sizes), dtype=torch.int32, device=device)
-                             .split(sizes))
+        step = PageTableStep(*torch.empty(sum(sizes), dtype=_INT32, device=device).split(sizes))
     else:
         step = PageTableStep(*out)
-        for t, n in zip(step, (batch, 1, batch + 1, tokens, tokens, 1)):
-            _int32(t, (n,), "page table outputs")
-        if batch and (step.lengths.data_ptr() == lengths.data_ptr()):
+        for t, n in zip(step, sizes):
+            _int32(t, (n,), index, "page table outputs")
+        if batch and step.lengths.data_ptr() == lengths.data_ptr():
             raise ValueError("the new lengths cannot be written over the old")
         if step.free_count.data_ptr() == free_count.data_ptr():
             raise ValueError("the new free count cannot be written over the old")
-    for t in (added, page_tables, free_pages, free_count, *step):
-        if t.device != device:
-            raise ValueError("page table tensors must be on one device")
     rc = nat.lib().cowsdm_page_tables_extend(
-        lengths.data_ptr(), added.data_ptr(), batch, page_tables.data_ptr(),
-        page_tables.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-        page_tokens, tokens, step.lengths.data_ptr(), step.free_count.data_ptr(),
-        step.offsets.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(),
+        lengths.data_ptr(), added.data_ptr(), batch, page_tables.data_ptr(), columns,
+        free_pages.data_ptr(), pages, free_count.data_ptr(), page_tokens, tokens,
+        step.lengths.data_ptr(), step.free_count.data_ptr(), step.offsets.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(),
         step.overflow.data_ptr(), nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_page_tables_extend")
@@ -216,7 +211,7 @@ def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: 
 
 
 def _cache(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch.Tensor,
-           value_scales: torch.Tensor, width: int, device: torch.device) -> nat.KVCache:
+           value_scales: torch.Tensor, width: int, device: int) -> nat.KVCache:
     """The C view of one layer's cache, after checking its tensors."""
 
     if key_pages.ndim != 4:
@@ -225,8 +220,8 @@ def _cache(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch
     if (value_pages.shape != (pages, heads, padded, page_tokens)
             or key_scales.shape != (pages, heads) or value_scales.shape != (pages, heads)):
         raise ValueError("cache tensors do not align")
-    if (key_pages.dtype != CODES or value_pages.dtype != CODES
-            or key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32):
+    if (key_pages.dtype is not CODES or value_pages.dtype is not CODES
+            or key_scales.dtype is not _FLOAT32 or value_scales.dtype is not _FLOAT32):
         raise TypeError("cache codes are float8_e4m3fn and scales float32")
     if page_tokens not in PAGE_TOKENS:
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
@@ -235,13 +230,12 @@ def _cache(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch
     for t in (key_pages, key_scales, value_pages, value_scales):
         if not t.is_contiguous():
             raise ValueError("cache tensors must be contiguous")
-        if t.device != device:
+        if t.get_device() != device:
             raise ValueError("cache tensors must be on the inputs' device")
     return nat.KVCache(pages, heads, page_tokens, padded, key_pages.data_ptr(),
                        key_scales.data_ptr(), value_pages.data_ptr(), value_scales.data_ptr())
 
 
-@torch.no_grad()
 def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
                    key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch.Tensor,
                    value_scales: torch.Tensor) -> None:
@@ -261,13 +255,13 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
         raise ValueError("cache writes take key and value [T,heads,D]")
     tokens, heads, width = key.shape
     _need_device(key, "cache writes")
-    device = key.device
+    device = key.get_device()
     code = _float_type(key.dtype)
-    if value.dtype != key.dtype:
+    if value.dtype is not key.dtype:
         raise TypeError("cache keys and values share one type")
-    if value.device != device or slots.device != device:
+    if value.get_device() != device:
         raise ValueError("cache writes must be on one device")
-    _int32(slots, (tokens,), "cache slots")
+    _int32(slots, (tokens,), device, "cache slots")
     cache = _cache(key_pages, key_scales, value_pages, value_scales, width, device)
     if cache.heads != heads:
         raise ValueError("cache and keys differ in heads")
@@ -276,7 +270,7 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
     key, value = _rows(key), _rows(value)
     rc = nat.lib().cowsdm_kv_write(
         cache, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-        value.stride(1), code, width, slots.data_ptr(), tokens, nat.stream_handle(device))
+        value.stride(1), code, width, slots.data_ptr(), tokens, nat.stream_handle(key.device))
     if rc:
         nat.check(rc, "cowsdm_kv_write")
 
@@ -290,7 +284,6 @@ def cached_workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, w
                                                              cache_width(width), longest)
 
 
-@torch.no_grad()
 def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: torch.Tensor,
                      value_pages: torch.Tensor, value_scales: torch.Tensor,
                      page_tables: torch.Tensor, lengths: torch.Tensor, *,
@@ -307,18 +300,16 @@ def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: t
         raise ValueError("cached attention takes query [B,n,heads,D]")
     batch, tokens, heads, width = query.shape
     _need_device(query, "attention inputs")
-    device = query.device
+    device, index = query.device, query.get_device()
     code = _float_type(query.dtype)
-    cache = _cache(key_pages, key_scales, value_pages, value_scales, width, device)
+    cache = _cache(key_pages, key_scales, value_pages, value_scales, width, index)
     if heads == 0 or heads % cache.heads:
         raise ValueError("query heads must be a multiple of the cache's heads")
     if page_tables.ndim != 2:
         raise ValueError("page tables must be [B,columns]")
     columns = page_tables.shape[1]
-    _int32(page_tables, (batch, columns), "page tables")
-    _int32(lengths, (batch,), "lengths")
-    if page_tables.device != device or lengths.device != device:
-        raise ValueError("attention inputs must be on one device")
+    _int32(page_tables, (batch, columns), index, "page tables")
+    _int32(lengths, (batch,), index, "lengths")
     room = columns * cache.page_tokens
     if longest is None or longest > room:
         longest = room

@@ -377,8 +377,6 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_kernel(WriteParams p, 
 
 // ------------------------------------------------------- cached attention
 
-constexpr int kCachedWaves = 4;
-constexpr int kCachedThreads = kCachedWaves * kWave;
 constexpr int kCachedTokens = 64;         // tokens a wave takes at a time
 constexpr int kCachedRows = 16;           // query rows of a workgroup
 
@@ -412,26 +410,47 @@ struct CachedParams {
 template <int DP>
 constexpr int kPartFloats = 2 * kCachedRows + kCachedRows * DP;
 
+typedef const __attribute__((address_space(4))) int32_t* const_int32;
+
+// Number g of four, without a table in memory.
+__device__ __forceinline__ int pick4(int g, int a, int b, int c, int d) {
+  const int low = (g & 1) ? b : a, high = (g & 1) ? d : c;
+  return (g & 2) ? high : low;
+}
+
+// A block of 64 tokens as a lane holds it: its quarter of four key rows, 16
+// tokens of each of its value columns, and their scales.
+template <int DP>
+struct Fetched {
+  uint32_t kw[4][DP / 16];
+  u32x4 vw[DP / 16];
+  float ks, vs;
+  int base, v_page;
+};
+
 // A request's tokens, at most what its page table can hold.
 __device__ __forceinline__ int cached_length(const CachedParams& p, int request) {
-  const int n = p.lengths[request], most = p.columns << p.page_shift;
+  const int n = ((const_int32)p.lengths)[request], most = p.columns << p.page_shift;
   return n < 0 ? 0 : n < most ? n : most;
 }
 
 // One workgroup: 16 query rows (the tokens and grouped heads of one key head)
-// over one split of the cache.  Each wave takes every fourth block of 64
-// tokens.  Scores are computed transposed, S^T = K Q^T, so that a lane ends
+// over one split of the cache.  Its NW waves take blocks of 64 tokens in
+// turn, the next on its way while one is used.
+//
+// Scores are computed transposed, S^T = K Q^T, so that a lane ends
 // with 16 consecutive tokens of one query row: its probabilities are then the
 // right operand of O^T = V^T P^T as they stand, and no score leaves its
 // registers.  Key row m of tile t is token (m / 4) * 16 + 4 t + m % 4.
-template <int DP, typename T>
-__global__ __launch_bounds__(kCachedThreads) void cached_attention_kernel(CachedParams p) {
+template <int DP, typename T, int NW>
+__global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedParams p) {
   constexpr int N = AttentionType<T>::kParts;
   constexpr int KB = DP / 4;            // a lane's bytes of a key row
   constexpr int KS = DP / 32;           // products along the width
   constexpr int DT = DP / 16;           // tiles of the output's width
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const int wave = static_cast<int>(threadIdx.x) / kWave;
+  const int wave =
+      __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int col = lane & 15, row = lane >> 4;
   const int split = blockIdx.x % p.splits;
   const int tile = blockIdx.x / p.splits;
@@ -464,25 +483,22 @@ __global__ __launch_bounds__(kCachedThreads) void cached_attention_kernel(Cached
     }
   }
 
-  const int32_t* const table = p.page_tables + static_cast<int64_t>(request) * p.columns;
+  const const_int32 table =
+      (const_int32)(p.page_tables + static_cast<int64_t>(request) * p.columns);
   const int64_t page_bytes = static_cast<int64_t>(page) * DP;
-  // the page of the 16 tokens from `at`, -1 where there is none
-  auto page_at = [&](int at) -> int {
-    const int column = at >> p.page_shift;
-    if (at >= end || column >= p.columns) return -1;
-    const int id = table[column];
-    return id >= 0 && id < p.pages ? id : -1;
-  };
-
-  f32x4 acc[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float most = kMinusInf, sum = 0.0f;     // of logits times scale
-
-  for (int base = begin + wave * kCachedTokens; base < end;
-       base += kCachedWaves * kCachedTokens) {
+  // a lane's bytes of a block's keys and values, on their way
+  auto fetch = [&](int base, Fetched<DP>& f) {
+    // the page of the block's tokens 16 g on; columns of tokens before the
+    // length are below the table's
+    auto page_of = [&](int g) {
+      const int column = (base + 16 * g) >> p.page_shift;
+      const int id = table[column < p.columns ? column : p.columns - 1];
+      return base + 16 * g < end && id >= 0 && id < p.pages ? id : -1;
+    };
+    const int id0 = page_of(0), id1 = page_of(1), id2 = page_of(2), id3 = page_of(3);
+    const int k_page = pick4(col >> 2, id0, id1, id2, id3);
+    const int v_page = pick4(row, id0, id1, id2, id3);
     const int k_at = base + (col >> 2) * 16, v_at = base + row * 16;
-    const int k_page = page_at(k_at), v_page = page_at(v_at);
     const int64_t k_block = static_cast<int64_t>(k_page < 0 ? 0 : k_page) * p.kv_heads + kv;
     const int64_t v_block = static_cast<int64_t>(v_page < 0 ? 0 : v_page) * p.kv_heads + kv;
     const uint8_t* const kp = p.key_codes + k_block * page_bytes +
@@ -490,26 +506,39 @@ __global__ __launch_bounds__(kCachedThreads) void cached_attention_kernel(Cached
                               row * KB;
     const uint8_t* const vp = p.value_codes + v_block * page_bytes +
                               static_cast<int64_t>(col) * page + (v_at & (page - 1));
-    const float ks = p.key_scales[k_block], vs = p.value_scales[v_block];
-    uint32_t kw[4][KB / 4];
+    f.base = base;
+    f.v_page = v_page;
+    f.ks = p.key_scales[k_block];
+    f.vs = p.value_scales[v_block];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const uint8_t* const src = kp + t * 4 * DP;
       if constexpr (KB % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < KB / 16; ++i)
-          *reinterpret_cast<u32x4*>(&kw[t][4 * i]) = *reinterpret_cast<const u32x4*>(src + 16 * i);
+          *reinterpret_cast<u32x4*>(&f.kw[t][4 * i]) =
+              *reinterpret_cast<const u32x4*>(src + 16 * i);
       } else {
 #pragma unroll
         for (int i = 0; i < KB / 8; ++i)
-          *reinterpret_cast<u32x2*>(&kw[t][2 * i]) = *reinterpret_cast<const u32x2*>(src + 8 * i);
+          *reinterpret_cast<u32x2*>(&f.kw[t][2 * i]) =
+              *reinterpret_cast<const u32x2*>(src + 8 * i);
       }
     }
-    u32x4 vw[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      vw[d] = *reinterpret_cast<const u32x4*>(vp + static_cast<int64_t>(d) * 16 * page);
+      f.vw[d] = *reinterpret_cast<const u32x4*>(vp + static_cast<int64_t>(d) * 16 * page);
+  };
 
+  f32x4 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float most = kMinusInf, sum = 0.0f;     // of logits times scale
+  auto use = [&](Fetched<DP>& f) {
+    const int base = f.base, v_page = f.v_page, v_at = base + row * 16;
+    const float ks = f.ks, vs = f.vs;
+    auto& kw = f.kw;
+    auto& vw = f.vw;
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -621,13 +650,42 @@ __global__ __launch_bounds__(kCachedThreads) void cached_attention_kernel(Cached
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, prob[h][n], acc[d], 0, 0, 0);
       }
     }
+  };
+
+  int base = begin + wave * kCachedTokens;
+  constexpr int kStep = NW * kCachedTokens;
+  if constexpr (DP < 256) {
+    // Two blocks in turn.  Past its last block a wave fetches that one again
+    // (from cache) and does not use it: a branch there would make every use
+    // wait for all that is on its way.
+    if (base < end) {
+      Fetched<DP> one, two;
+      fetch(base, one);
+      for (;;) {
+        fetch(base + kStep < end ? base + kStep : base, two);
+        use(one);
+        base += kStep;
+        if (base >= end) break;
+        fetch(base + kStep < end ? base + kStep : base, one);
+        use(two);
+        base += kStep;
+        if (base >= end) break;
+      }
+    }
+  } else {
+    // two blocks of the widest rows do not fit the registers
+    for (; base < end; base += kStep) {
+      Fetched<DP> one;
+      fetch(base, one);
+      use(one);
+    }
   }
   sum = sum_over_rows(sum);
 
   // the waves' parts, joined pairwise in a fixed order
-  __shared__ __attribute__((aligned(16))) float s_part[kCachedWaves / 2][DT + 1][kWave * 4];
+  __shared__ __attribute__((aligned(16))) float s_part[NW / 2][DT + 1][kWave * 4];
 #pragma unroll
-  for (int half = kCachedWaves / 2; half > 0; half /= 2) {
+  for (int half = NW / 2; half > 0; half /= 2) {
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -675,10 +733,17 @@ __global__ __launch_bounds__(kCachedThreads) void cached_attention_kernel(Cached
   }
 }
 
-// Joins the splits of one query row, in their order: one wave a row.
+// Joins the splits of one query row: every group of DP / 4 lanes takes every
+// so many splits, and the groups' sums are added in their order.
+constexpr int kJoinThreads = 256;
+
 template <int DP, typename T>
-__global__ __launch_bounds__(kWave) void cached_join_kernel(CachedParams p) {
-  const int lane = static_cast<int>(threadIdx.x);
+__global__ __launch_bounds__(kJoinThreads) void cached_join_kernel(CachedParams p) {
+  constexpr int kLanes = DP / 4;
+  constexpr int kGroups = kJoinThreads / kLanes;
+  __shared__ __attribute__((aligned(16))) float s_sum[kGroups][DP + 4];
+  __shared__ float s_most[kJoinThreads / kWave];
+  const int tid = static_cast<int>(threadIdx.x);
   const int group = p.heads / p.kv_heads;
   const int head = blockIdx.x, token = blockIdx.y, request = blockIdx.z;
   const int kv = head / group;
@@ -694,28 +759,54 @@ __global__ __launch_bounds__(kWave) void cached_join_kernel(CachedParams p) {
       p.parts + ((static_cast<int64_t>(request) * p.kv_heads + kv) * p.row_tiles + tile) *
                     p.splits * kPartFloats<DP>;
   float most = kMinusInf;
-  for (int s = 0; s < used; ++s)
+  for (int s = tid; s < used; s += kJoinThreads)
     most = fmaxf(most, parts[static_cast<int64_t>(s) * kPartFloats<DP> + col]);
+  most = max_over_rows(most);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, kWave));
+  if ((tid & (kWave - 1)) == 0) s_most[tid / kWave] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / kWave; ++w) most = fmaxf(most, s_most[w]);
+  const int mine = tid / kLanes, at = (tid - mine * kLanes) * 4;
   float sum = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int at = lane * 4;
-  for (int s = 0; s < used; ++s) {
-    const float* const part = parts + static_cast<int64_t>(s) * kPartFloats<DP>;
-    const float w = most == kMinusInf ? 1.0f : exp2_fast(part[col] - most);
-    sum += part[kCachedRows + col] * w;
-    if (at < DP) acc += *reinterpret_cast<const f32x4*>(part + 2 * kCachedRows + col * DP + at) * w;
+  if (mine < kGroups) {
+#pragma unroll 4
+    for (int s = mine; s < used; s += kGroups) {
+      const float* const part = parts + static_cast<int64_t>(s) * kPartFloats<DP>;
+      const float w = most == kMinusInf ? 1.0f : exp2_fast(part[col] - most);
+      sum += part[kCachedRows + col] * w;
+      acc += *reinterpret_cast<const f32x4*>(part + 2 * kCachedRows + col * DP + at) * w;
+    }
+    *reinterpret_cast<f32x4*>(&s_sum[mine][at]) = acc;
+    if (at == 0) s_sum[mine][DP] = sum;
   }
-  if (at < p.width) store4(out + at, none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / sum));
+  __syncthreads();
+  if (tid >= kLanes || at >= p.width) return;
+  acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  sum = 0.0f;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    acc += *reinterpret_cast<const f32x4*>(&s_sum[g][at]);
+    sum += s_sum[g][DP];
+  }
+  store4(out + at, none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / sum));
 }
+
+// The waves of a workgroup: eight where the registers of the widths allow two
+// on a SIMD.
+constexpr int cached_waves(int64_t padded) { return padded <= 128 ? 8 : 4; }
 
 template <int DP, typename T>
 void launch_cached(const CachedParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL((cached_attention_kernel<DP, T>),
-                     dim3(p.splits * p.row_tiles, p.kv_heads, p.requests), dim3(kCachedThreads),
-                     0, stream, p);
+  constexpr int NW = cached_waves(DP);
+  hipLaunchKernelGGL((cached_attention_kernel<DP, T, NW>),
+                     dim3(p.splits * p.row_tiles, p.kv_heads, p.requests), dim3(NW * kWave), 0,
+                     stream, p);
   if (p.parts)
     hipLaunchKernelGGL((cached_join_kernel<DP, T>), dim3(p.heads, p.tokens, p.requests),
-                       dim3(kWave), 0, stream, p);
+                       dim3(kJoinThreads), 0, stream, p);
 }
 
 template <typename T>
@@ -731,14 +822,15 @@ void launch_cached_width(int64_t padded, const CachedParams& p, hipStream_t stre
 }
 
 // The splits of the cache that a call's launch makes: enough workgroups to
-// fill the chip, none with less than one block a wave.
-int64_t cached_splits(int64_t requests, int64_t kv_heads, int64_t row_tiles, int64_t longest) {
-  constexpr int64_t kWorkgroups = 1024;
-  constexpr int64_t kLeast = kCachedWaves * kCachedTokens;
+// fill the chip, none with less than two blocks a wave.
+int64_t cached_splits(int64_t requests, int64_t kv_heads, int64_t row_tiles, int64_t padded,
+                      int64_t longest) {
+  constexpr int64_t kWorkgroups = 256;
+  const int64_t least = 2 * cached_waves(padded) * kCachedTokens;
   const int64_t rows = requests * kv_heads * row_tiles;
-  const int64_t most = (longest + kLeast - 1) / kLeast;
-  int64_t splits = rows > 0 ? kWorkgroups / rows : 1;
-  splits = splits < 1 ? 1 : splits > most ? most : splits;
+  const int64_t most = (longest + least - 1) / least;
+  int64_t splits = rows > 0 ? (kWorkgroups + rows - 1) / rows : 1;
+  splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits;
 }
 
@@ -886,7 +978,7 @@ extern "C" int64_t cowsdm_cached_attention_workspace_bytes(int64_t requests, int
       !is_cache_width(padded_width) || longest < 0)
     return -1;
   const int64_t tiles = (tokens * (heads / kv_heads) + kCachedRows - 1) / kCachedRows;
-  const int64_t splits = cached_splits(requests, kv_heads, tiles, longest);
+  const int64_t splits = cached_splits(requests, kv_heads, tiles, padded_width, longest);
   if (splits == 1) return 0;
   return requests * kv_heads * tiles * splits * (2 * kCachedRows + kCachedRows * padded_width) *
          static_cast<int64_t>(sizeof(float));
@@ -942,8 +1034,9 @@ extern "C" int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
   const int64_t group = q.heads / cache->heads;
   const int64_t tiles = (q.tokens * group + kCachedRows - 1) / kCachedRows;
   p.row_tiles = static_cast<int32_t>(tiles);
-  p.splits = static_cast<int32_t>(cached_splits(q.requests, cache->heads, tiles, q.longest));
-  constexpr int64_t kBlock = kCachedWaves * kCachedTokens;
+  p.splits = static_cast<int32_t>(
+      cached_splits(q.requests, cache->heads, tiles, cache->width, q.longest));
+  const int64_t kBlock = cached_waves(cache->width) * kCachedTokens;
   const int64_t each = (q.longest + p.splits - 1) / p.splits;
   p.chunk = p.splits == 1 ? INT32_MAX / 2
                           : static_cast<int32_t>((each + kBlock - 1) / kBlock * kBlock);

@@ -73,7 +73,7 @@ def test_cached_refusals():
 
 
 def test_cache_checks():
-    device = torch.device("cpu")
+    device = -1              # what a CPU tensor gives
     view = attention._cache(*cache(), 64, device)
     assert (view.pages, view.heads, view.page_tokens, view.width) == (2, 2, 16, 64)
 
