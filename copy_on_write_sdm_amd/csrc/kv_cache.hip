@@ -10,6 +10,8 @@
 // values, each a power of two: codes keep their bits when a scale grows (but
 // for the smallest, which round), and code times scale is exact in bfloat16.
 
+#include <type_traits>
+
 #include "attention.h"
 
 namespace cowsdm_impl {
@@ -245,134 +247,281 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < __builtin_huge_valf() ? a : 0.0f;
 }
 
-// One run of tokens in one page and head, by the whole workgroup.
+// Eight elements as loaded: kept packed until they are used.
 template <typename T>
-__device__ void write_run(const WriteParams& p, int width, int head, int t0, int slot, int run,
+struct Eight {
+  u32x4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(raw[j / 4][j % 4]);
+    } else {
+      const uint32_t pair = raw[0][j / 2];
+      return widen_float(j % 2 ? pair >> 16 : pair & 0xffffu,
+                         std::is_same<T, __bf16>::value ? COWSDM_BFLOAT16 : COWSDM_FLOAT16);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p) {
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    e.raw[i] = reinterpret_cast<const u32x4*>(p)[i];
+  return e;
+}
+
+// Keeps the compiler from holding the elements widened from one use to the
+// next: the packed words are half the registers.
+template <typename T>
+__device__ __forceinline__ void stay_packed(Eight<T>& e) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t word = e.raw[i][j];
+      asm volatile("" : "+v"(word));
+      e.raw[i][j] = word;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float largest(const Eight<T>& e, float most) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = fmaxf(most, finite_abs(e[j]));
+  return most;
+}
+
+// What a workgroup writes: one run of tokens in one page and head.
+template <typename T>
+struct WriteRun {
+  const T* key;          // the run's first row
+  const T* value;
+  int64_t key_row, value_row;
+  uint8_t* kc;           // the page's codes
+  uint8_t* vc;
+  int columns, wide;     // eights of a row's elements, and of its codes
+  int page, first, run;  // tokens of the page, before the run, and of the run
+
+  // Eight elements of key row r; zeros in the padding.
+  __device__ __forceinline__ Eight<T> key_at(int r, int c) const {
+    return c < columns ? load_eight(key + r * key_row + c * 8) : Eight<T>{};
+  }
+  __device__ __forceinline__ void put_key(int r, int c, const Eight<T>& e, float inverse) const {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = code_value(e[j], inverse);
+    *reinterpret_cast<u32x2*>(kc + (static_cast<int64_t>(first + r) * wide + c) * 8) =
+        u32x2{encode4(x[0], x[1], x[2], x[3]), encode4(x[4], x[5], x[6], x[7])};
+  }
+  // Of the page's four tokens from 4 g on: eight columns of those of the run,
+  // and in the result their bytes.
+  __device__ __forceinline__ uint32_t values_at(int g, int c, Eight<T> (&e)[4]) const {
+    uint32_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = 4 * g + k - first;
+      const bool in = r >= 0 && r < run;
+      mine |= in ? 0xffu << (8 * k) : 0u;
+      e[k] = in && c < columns ? load_eight(value + r * value_row + c * 8) : Eight<T>{};
+    }
+    return mine;
+  }
+  __device__ __forceinline__ uint32_t* value_word(int g, int column) const {
+    return reinterpret_cast<uint32_t*>(vc + static_cast<int64_t>(column) * page) + g;
+  }
+  __device__ __forceinline__ uint32_t value_codes(const Eight<T> (&e)[4], int j,
+                                                  float inverse) const {
+    return encode4(code_value(e[0][j], inverse),
+                   code_value(e[1][j], inverse),
+                   code_value(e[2][j], inverse),
+                   code_value(e[3][j], inverse));
+  }
+};
+
+constexpr int kWriteKeys = 4;        // eights of keys that a thread holds
+
+// By the whole workgroup.  Held: a page has at most 8,192 elements (64 tokens
+// at width 128), and a run's stay in registers between the maximum and the
+// codes; else they are read twice, the second time from cache.
+template <typename T, bool kHeld>
+__device__ __forceinline__ void write_run(const WriteRun<T>& w, float* key_scale, float* value_scale,
                           float* s_most) {
   const int tid = static_cast<int>(threadIdx.x);
-  const int page = 1 << p.page_shift;
-  const int at = slot >> p.page_shift;          // the page
-  const int first = slot & (page - 1);          // the run's first token in it
-  const int64_t block = static_cast<int64_t>(at) * p.heads + head;
-  uint8_t* const kc = p.key_codes + block * page * width;
-  uint8_t* const vc = p.value_codes + block * page * width;
-  const T* const key = static_cast<const T*>(p.key) + t0 * p.key_row + head * p.key_head;
-  const T* const value = static_cast<const T*>(p.value) + t0 * p.value_row + head * p.value_head;
-  const int eighths = p.width / 8;
+  const int wave = tid / kWave;
+  const int g0 = w.first / 4, groups = (w.first + w.run + 3) / 4 - g0;
+  const int keys = w.run * w.wide, values = groups * w.wide;
+  const int vg = g0 + tid % groups, vcol = tid / groups;
+  Eight<T> k[kWriteKeys] = {}, v[4] = {};
+  uint32_t mine = 0, other[8] = {};
   float km = 0.0f, vm = 0.0f;
-  for (int i = tid; i < run * eighths; i += kWriteThreads) {
-    const int r = i / eighths, c = (i - r * eighths) * 8;
-    float x[8];
-    load8(key + r * p.key_row + c, x);
+  const float k_old = w.first ? *key_scale : 0.0f;
+  const float v_old = w.first ? *value_scale : 0.0f;
+  if constexpr (kHeld) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) km = fmaxf(km, finite_abs(x[j]));
-    load8(value + r * p.value_row + c, x);
+    for (int n = 0; n < kWriteKeys; ++n) {
+      const int i = tid + n * kWriteThreads;
+      if (i < keys) k[n] = w.key_at(i / w.wide, i % w.wide);
+    }
+    if (tid < values) {
+      mine = w.values_at(vg, vcol, v);
+      if (mine != 0xffffffffu) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vm = fmaxf(vm, finite_abs(x[j]));
+        for (int j = 0; j < 8; ++j) other[j] = *w.value_word(vg, vcol * 8 + j);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kWriteKeys; ++n)
+      if (tid + n * kWriteThreads < keys) km = largest(k[n], km);
+    if (tid < values) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) vm = largest(v[n], vm);
+    }
+  } else {
+    for (int i = tid; i < w.run * w.columns; i += kWriteThreads) {
+      const int r = i / w.columns, c = (i - r * w.columns) * 8;
+      km = largest(load_eight(w.key + r * w.key_row + c), km);
+      vm = largest(load_eight(w.value + r * w.value_row + c), vm);
+    }
   }
 #pragma unroll
   for (int o = kWave / 2; o > 0; o >>= 1) {
     km = fmaxf(km, __shfl_xor(km, o, kWave));
     vm = fmaxf(vm, __shfl_xor(vm, o, kWave));
   }
-  const int wave = tid / kWave;
-  const float k_old = first ? p.key_scales[block] : 0.0f;
-  const float v_old = first ? p.value_scales[block] : 0.0f;
   if ((tid & (kWave - 1)) == 0) {
     s_most[2 * wave] = km;
     s_most[2 * wave + 1] = vm;
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWriteThreads / kWave; ++w) {
-    km = fmaxf(km, s_most[2 * w]);
-    vm = fmaxf(vm, s_most[2 * w + 1]);
+  for (int n = 0; n < kWriteThreads / kWave; ++n) {
+    km = fmaxf(km, s_most[2 * n]);
+    vm = fmaxf(vm, s_most[2 * n + 1]);
   }
-  const float k_scale = fmaxf(power_scale(km), k_old);
-  const float v_scale = fmaxf(power_scale(vm), v_old);
+  if constexpr (kHeld && sizeof(T) == 2) {
+#pragma unroll
+    for (int n = 0; n < kWriteKeys; ++n) stay_packed(k[n]);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) stay_packed(v[n]);
+  }
+  const float k_scale = fmaxf(power_scale(km), k_old), ki = power_inverse(k_scale);
+  const float v_scale = fmaxf(power_scale(vm), v_old), vi = power_inverse(v_scale);
   if (tid == 0) {
-    p.key_scales[block] = k_scale;
-    p.value_scales[block] = v_scale;
+    *key_scale = k_scale;
+    *value_scale = v_scale;
   }
-  const float ki = power_inverse(k_scale), vi = power_inverse(v_scale);
-  // keys: a row of codes a token; the page's other rows where the scale grew
-  const int wide = width / 8;
-  for (int i = tid; i < run * wide; i += kWriteThreads) {
-    const int r = i / wide, c = (i - r * wide) * 8;
-    float x[8] = {};
-    if (c < p.width) load8(key + r * p.key_row + c, x);
+  const bool k_grew = w.first && k_scale > k_old, v_grew = w.first && v_scale > v_old;
+  const float k_ratio = k_old * ki, v_ratio = v_old * vi;
+  if constexpr (kHeld) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = code_value(x[j], ki);
-    u32x2 w = {encode4(x[0], x[1], x[2], x[3]), encode4(x[4], x[5], x[6], x[7])};
-    *reinterpret_cast<u32x2*>(kc + (first + r) * width + c) = w;
-  }
-  if (first && k_scale > k_old) {
-    const float ratio = k_old * ki;
-    for (int i = tid; i < (page - run) * width / 4; i += kWriteThreads) {
-      const int at = i < first * width / 4 ? i : i + run * width / 4;
-      uint32_t* const w = reinterpret_cast<uint32_t*>(kc) + at;
-      *w = rescale4(*w, ratio);
+    for (int n = 0; n < kWriteKeys; ++n) {
+      const int i = tid + n * kWriteThreads;
+      if (i < keys) w.put_key(i / w.wide, i % w.wide, k[n], ki);
     }
-  }
-  // values: four tokens of eight columns a thread, stored as four tokens of
-  // each column; a group of four that the run does not fill keeps its others
-  const bool grew = first && v_scale > v_old;
-  const float ratio = v_old * vi;
-  const int g0 = grew ? 0 : first / 4;
-  const int groups = (grew ? page / 4 : (first + run + 3) / 4) - g0;
-  for (int i = tid; i < groups * wide; i += kWriteThreads) {
-    const int c = (i / groups) * 8, g = g0 + i % groups;
-    float x[4][8] = {};
-    uint32_t mine = 0;                         // bytes of the run's tokens
+    if (tid < values) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = 4 * g + k - first;
-      if (r >= 0 && r < run) {
-        mine |= 0xffu << (8 * k);
-        if (c < p.width) load8(value + r * p.value_row + c, x[k]);
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t kept = v_grew ? rescale4(other[j], v_ratio) : other[j];
+        *w.value_word(vg, vcol * 8 + j) = (w.value_codes(v, j, vi) & mine) | (kept & ~mine);
       }
     }
+  } else {
+    for (int i = tid; i < keys; i += kWriteThreads)
+      w.put_key(i / w.wide, i % w.wide, w.key_at(i / w.wide, i % w.wide), ki);
+    for (int i = tid; i < values; i += kWriteThreads) {
+      const int g = g0 + i % groups, c = i / groups;
+      mine = w.values_at(g, c, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t* const w = reinterpret_cast<uint32_t*>(vc + (c + j) * page) + g;
-      uint32_t codes = encode4(code_value(x[0][j], vi), code_value(x[1][j], vi),
-                               code_value(x[2][j], vi), code_value(x[3][j], vi));
-      if (mine != 0xffffffffu) {
-        const uint32_t other = grew ? rescale4(*w, ratio) : *w;
-        codes = (codes & mine) | (other & ~mine);
+      for (int j = 0; j < 8; ++j) {
+        uint32_t* const word = w.value_word(g, c * 8 + j);
+        uint32_t codes = w.value_codes(v, j, vi);
+        if (mine != 0xffffffffu) {
+          const uint32_t kept = v_grew ? rescale4(*word, v_ratio) : *word;
+          codes = (codes & mine) | (kept & ~mine);
+        }
+        *word = codes;
       }
-      *w = codes;
+    }
+  }
+  // a grown scale takes the page's other codes along: the other rows of keys,
+  // and the groups of values outside the run
+  if (k_grew) {
+    const int row = w.wide * 2;
+    for (int i = tid; i < (w.page - w.run) * row; i += kWriteThreads) {
+      uint32_t* const word =
+          reinterpret_cast<uint32_t*>(w.kc) + (i < w.first * row ? i : i + w.run * row);
+      *word = rescale4(*word, k_ratio);
+    }
+  }
+  if (v_grew) {
+    const int rest = w.page / 4 - groups;
+    for (int i = tid; i < rest * w.wide * 8; i += kWriteThreads) {
+      const int g = i % rest;
+      uint32_t* const word = w.value_word(g < g0 ? g : g + groups, i / rest);
+      *word = rescale4(*word, v_ratio);
     }
   }
   __syncthreads();      // s_most is free for the next run
 }
 
 // A run is a stretch of the call's tokens whose slots follow one another in
-// one page; its first token's workgroup writes it, for one head.
-template <typename T>
+// one page; the workgroup of its first token's chunk (at most 64 tokens)
+// writes it, for one head.
+template <typename T, bool kHeld>
 __global__ __launch_bounds__(kWriteThreads) void kv_write_kernel(WriteParams p, int width) {
   __shared__ float s_most[2 * kWriteThreads / kWave];
   __shared__ int s_run;
   const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & (kWave - 1);
   const int head = blockIdx.y;
   const int page = 1 << p.page_shift;
   const int64_t limit = static_cast<int64_t>(p.pages) << p.page_shift;
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.chunk;
-  const int64_t end = begin + p.chunk < p.tokens ? begin + p.chunk : p.tokens;
-  for (int64_t t = begin; t < end; ++t) {
-    const int slot = p.slots[t];
-    if (slot < 0 || slot >= limit) continue;
-    if (t > 0 && (slot & (page - 1)) != 0 && p.slots[t - 1] == slot - 1) continue;
-    // the run's length: the first of the page's next slots that is not the next token's
-    if (tid == 0) s_run = page - (slot & (page - 1));
+  // every wave finds the chunk's first tokens of runs
+  const int64_t mine = begin + lane;
+  int slot = -1;
+  bool opens = false;
+  if (lane < p.chunk && mine < p.tokens) {
+    slot = p.slots[mine];
+    opens = slot >= 0 && slot < limit &&
+            ((slot & (page - 1)) == 0 || mine == 0 || p.slots[mine - 1] != slot - 1);
+  }
+  for (uint64_t runs = __ballot(opens); runs; runs &= runs - 1) {
+    const int from = __builtin_ctzll(runs);
+    const int t = static_cast<int>(begin) + from;
+    const int at = __builtin_amdgcn_readlane(slot, from);
+    const int first = at & (page - 1);
+    // the run ends before the first of the page's next slots that is not the
+    // next token's
+    if (tid == 0) s_run = page - first;
     __syncthreads();
     const int i = tid + 1;
-    if (i < page - (slot & (page - 1)) && (t + i >= p.tokens || p.slots[t + i] != slot + i))
+    if (i < page - first && (t + i >= p.tokens || p.slots[t + i] != at + i))
       atomicMin(&s_run, i);
     __syncthreads();
-    const int run = s_run;
-    write_run<T>(p, width, head, static_cast<int>(t), slot, run, s_most);
+    const int64_t block = static_cast<int64_t>(at >> p.page_shift) * p.heads + head;
+    WriteRun<T> w;
+    w.key = static_cast<const T*>(p.key) + t * p.key_row + head * p.key_head;
+    w.value = static_cast<const T*>(p.value) + t * p.value_row + head * p.value_head;
+    w.key_row = p.key_row;
+    w.value_row = p.value_row;
+    w.kc = p.key_codes + block * page * width;
+    w.vc = p.value_codes + block * page * width;
+    w.columns = p.width / 8;
+    w.wide = width / 8;
+    w.page = page;
+    w.first = first;
+    w.run = s_run;
+    write_run<T, kHeld>(w, p.key_scales + block, p.value_scales + block, s_most);
   }
+}
+
+template <typename T>
+void launch_write(const WriteParams& p, dim3 grid, int width, hipStream_t stream) {
+  const bool held = (width << p.page_shift) <= 8 * kWriteKeys * kWriteThreads;
+  hipLaunchKernelGGL((held ? &kv_write_kernel<T, true> : &kv_write_kernel<T, false>), grid,
+                     dim3(kWriteThreads), 0, stream, p, width);
 }
 
 // ------------------------------------------------------- cached attention
@@ -957,17 +1106,14 @@ extern "C" int32_t cowsdm_kv_write(const cowsdm_kv_cache_t* cache, const void* k
   p.width = static_cast<int32_t>(width);
   p.pages = static_cast<int32_t>(cache->pages);
   p.page_shift = shift;
-  p.chunk = tokens <= 1024 ? 1 : 16;
+  p.chunk = tokens <= 1024 ? 1 : kWave;
   const dim3 grid(static_cast<uint32_t>((tokens + p.chunk - 1) / p.chunk),
                   static_cast<uint32_t>(cache->heads));
   const int padded = static_cast<int>(cache->width);
   const auto s = static_cast<hipStream_t>(stream);
-  if (float_type == COWSDM_FLOAT32)
-    hipLaunchKernelGGL(kv_write_kernel<float>, grid, dim3(kWriteThreads), 0, s, p, padded);
-  else if (float_type == COWSDM_FLOAT16)
-    hipLaunchKernelGGL(kv_write_kernel<_Float16>, grid, dim3(kWriteThreads), 0, s, p, padded);
-  else
-    hipLaunchKernelGGL(kv_write_kernel<__bf16>, grid, dim3(kWriteThreads), 0, s, p, padded);
+  if (float_type == COWSDM_FLOAT32) launch_write<float>(p, grid, padded, s);
+  else if (float_type == COWSDM_FLOAT16) launch_write<_Float16>(p, grid, padded, s);
+  else launch_write<__bf16>(p, grid, padded, s);
   return launch_status("kv_write");
 }
 
