@@ -6,6 +6,8 @@
 // probabilities are the right operand of O^T = V^T P^T where they stand:
 // neither scores nor probabilities leave the registers.
 
+#include <type_traits>
+
 #include "attention.h"
 
 namespace cowsdm_impl {
@@ -159,6 +161,10 @@ __device__ __forceinline__ bool any_odd(typename Half<T>::vec v) {
   return odd;
 }
 
+// Whole: every row sees all of the tile.  Edge: some do not.  Careful: as
+// edge, and no value that is not finite reaches a row that does not see it.
+enum class PromptTile { kWhole, kEdge, kCareful };
+
 // One wave's RB * 32 query rows of one head: q the rows, acc their products
 // so far, transposed, most the maxima that the probabilities are relative to
 // and sum their sums (of this lane's keys).
@@ -191,9 +197,8 @@ struct PromptRows {
     return __builtin_bit_cast(vec, both);
   }
 
-  // One tile of 64 keys from row k0 on.  Masked: some of the rows, from q0 on,
-  // do not see all of it.
-  template <bool kMasked>
+  // One tile of 64 keys from row k0 on.
+  template <PromptTile kKind>
   __device__ __forceinline__ void tile(const lds_char* keys, const lds_char* values,
                                        const int (&key_read)[KS],
                                        const int (&value_read)[DT][2], float scale, int k0,
@@ -215,19 +220,10 @@ struct PromptRows {
         for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(a, q[r][k], s[r][kb]);
       }
     }
-    bool poisoned = false;
-    if constexpr (kMasked) {
-#pragma unroll 1
-      for (int h = 0; h < 4; ++h)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          poisoned |= any_odd<T>(turned(values, value_read, h, d));
-      poisoned = __any(poisoned);
-    }
     vec prob[RB][4];
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      if constexpr (kMasked) {
+      if constexpr (kKind != PromptTile::kWhole) {
         const int row = q0 + r * 32 + col;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -273,7 +269,7 @@ struct PromptRows {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         vec v = turned(values, value_read, h, d);
-        if (kMasked && poisoned) {
+        if constexpr (kKind == PromptTile::kCareful) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (!(__builtin_fabsf(static_cast<float>(v[j])) < __builtin_huge_valf()))
@@ -282,14 +278,23 @@ struct PromptRows {
 #pragma unroll
         for (int r = 0; r < RB; ++r) acc[r][d] = Half<T>::mfma(v, prob[r][h], acc[r][d]);
       }
-    if constexpr (kMasked) {
-      if (poisoned) add_odd(values, value_read, k0, q0);
-    }
+    if constexpr (kKind == PromptTile::kCareful) add_odd(values, value_read, k0, q0);
   }
 
-  // Values that are not finite, for the rows that see them: a product with a
-  // probability of 0 would hand their NaN to the others.  Products of ones and
-  // zeros count them, and what is counted is added by itself.
+  // Whether an output of this lane is NaN.
+  __device__ __forceinline__ bool any_nan() const {
+    bool nan = false;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) nan |= acc[r][d][i] != acc[r][d][i];
+    return nan;
+  }
+
+  // Values that are not finite, for the rows that see them.  Products of ones
+  // and zeros count them, and what is counted is added by itself.
   __device__ __forceinline__ void add_odd(const lds_char* values, const int (&value_read)[DT][2],
                                           int k0, int q0) {
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
@@ -394,8 +399,16 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
 
   for (int block = w.block; block * kRows < length; block += p.blocks) {
     const int q0 = block * kRows + wave * RB * 32;      // this wave's first row
+    const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
+    const int count = (seen + kTileKeys - 1) / kTileKeys;
+    __syncthreads();            // the tiles of the block before are used
+    load_tile(0, 0);
+    auto arrived = [&](int tile, int buffer) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this thread's part has arrived
+      __syncthreads();                         // everyone's; the other buffer is used
+      if (tile + 1 < count) load_tile(tile + 1, buffer ^ 1);
+    };
     Rows rows;
-    rows.clear();
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int row = q0 + r * 32 + col;
@@ -406,35 +419,39 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
         rows.q[r][s] = d < p.width ? *reinterpret_cast<const vec*>(src + d) : vec{};
       }
     }
-    const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
-    const int count = (seen + kTileKeys - 1) / kTileKeys;
+    rows.clear();
     // Tiles before the block's first row are seen by all of its rows; what
-    // follows, to the diagonal, has a loop of its own.  Both take a multiple
-    // of two tiles, so that a buffer's address is part of the instructions.
+    // follows, to the diagonal, has a loop of its own.  The first are a
+    // multiple of two, so that a buffer's address is part of the instructions.
     const int whole = block * (kRows / kTileKeys);
-    __syncthreads();            // the tiles of the block before are used
-    load_tile(0, 0);
-    auto arrived = [&](int tile, int buffer) {
-      __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this thread's part has arrived
-      __syncthreads();                         // everyone's; the other buffer is used
-      if (tile + 1 < count) load_tile(tile + 1, buffer ^ 1);
-    };
     for (int tile = 0; tile < whole; tile += 2) {
 #pragma unroll
       for (int buffer = 0; buffer < 2; ++buffer) {
         arrived(tile + buffer, buffer);
         const lds_char* const keys = tiles + buffer * 2 * kTileBytes;
-        rows.template tile<false>(keys, keys + kTileBytes, key_read, value_read, p.scale,
-                                  (tile + buffer) * kTileKeys, q0);
+        rows.template tile<PromptTile::kWhole>(keys, keys + kTileBytes, key_read, value_read,
+                                               p.scale, (tile + buffer) * kTileKeys, q0);
       }
     }
+    auto edges = [&](auto kind, int from) {
 #pragma unroll 1
-    for (int tile = whole; tile < count; ++tile) {
-      arrived(tile, tile & 1);
-      const int k0 = tile * kTileKeys;
-      const lds_char* const keys = tiles + (tile & 1) * 2 * kTileBytes;
-      if (k0 <= q0 + RB * 32 - 1 && q0 < length)
-        rows.template tile<true>(keys, keys + kTileBytes, key_read, value_read, p.scale, k0, q0);
+      for (int tile = from; tile < count; ++tile) {
+        arrived(tile, tile & 1);
+        const int k0 = tile * kTileKeys;
+        const lds_char* const keys = tiles + (tile & 1) * 2 * kTileBytes;
+        if (k0 <= q0 + RB * 32 - 1 && q0 < length)
+          rows.template tile<decltype(kind)::value>(keys, keys + kTileBytes, key_read,
+                                                    value_read, p.scale, k0, q0);
+      }
+    };
+    edges(std::integral_constant<PromptTile, PromptTile::kEdge>(), whole);
+    // A value that is not finite, times the probability 0 of a row that does
+    // not see it, is NaN.  Such values are rare and NaN stays in a sum: a
+    // block that has one at its end is done again with care.
+    if (__syncthreads_or(rows.any_nan())) {
+      rows.clear();
+      load_tile(0, 0);
+      edges(std::integral_constant<PromptTile, PromptTile::kCareful>(), 0);
     }
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
