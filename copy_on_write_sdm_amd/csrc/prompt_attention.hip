@@ -161,6 +161,8 @@ __device__ __forceinline__ bool any_odd(typename Half<T>::vec v) {
   return odd;
 }
 
+constexpr int kOthersMove = 0x406;       // a scheduling barrier that vector and scalar work passes
+
 // Whole: every row sees all of the tile.  Edge: some do not.  Careful: as
 // edge, and no value that is not finite reaches a row that does not see it.
 enum class PromptTile { kWhole, kEdge, kCareful };
@@ -173,6 +175,9 @@ struct PromptRows {
   using vec = typename Half<T>::vec;
   static constexpr int KS = DP / 16;       // products along the width
   static constexpr int DT = DP / 32;       // tiles of the output's width
+  // steps that operands are read ahead of their products, as registers allow
+  static constexpr int kKeysAhead = DP <= 192 ? 3 : 1;
+  static constexpr int kValuesAhead = DP <= 192 ? 1 : 0;
   vec q[RB][KS];
   f32x16 acc[RB][DT];
   float most[RB], sum[RB];
@@ -207,19 +212,40 @@ struct PromptRows {
     const int col = lane & 31, half = lane >> 5;
     f32x16 s[RB][2];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
-      for (int r = 0; r < RB; ++r)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[r][kb][i] = 0.0f;
+    // operands are read from LDS some steps before the products that take
+    // them, and are kept there: left to itself the compiler reads each at its
+    // product, whose wait is longer than the product
+    vec key[KS][2];
+    auto read_keys = [&](int k) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const vec a = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(
+      for (int kb = 0; kb < 2; ++kb)
+        key[k][kb] = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(
             keys + key_read[k] + kb * 32 * DP * 2);
+    };
 #pragma unroll
-        for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(a, q[r][k], s[r][kb]);
-      }
+    for (int k = 0; k < kKeysAhead && k < KS; ++k) read_keys(k);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      if (k + kKeysAhead < KS) read_keys(k + kKeysAhead);
+      __builtin_amdgcn_sched_barrier(kOthersMove);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(key[k][kb], q[r][k], s[r][kb]);
+      __builtin_amdgcn_sched_barrier(kOthersMove);
     }
+    vec value[4][DT];
+    auto read_values = [&](int h) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) value[h][d] = turned(values, value_read, h, d);
+    };
+    if constexpr (kValuesAhead > 0) read_values(0);
+    __builtin_amdgcn_sched_barrier(kOthersMove);
     vec prob[RB][4];
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
@@ -265,10 +291,12 @@ struct PromptRows {
       sum[r] += (part[0] + part[1]) + (part[2] + part[3]);
     }
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
+    for (int h = 0; h < 4; ++h) {
+      if (h + kValuesAhead < 4) read_values(h + kValuesAhead);
+      __builtin_amdgcn_sched_barrier(kOthersMove);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        vec v = turned(values, value_read, h, d);
+        vec v = value[h][d];
         if constexpr (kKind == PromptTile::kCareful) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -278,6 +306,8 @@ struct PromptRows {
 #pragma unroll
         for (int r = 0; r < RB; ++r) acc[r][d] = Half<T>::mfma(v, prob[r][h], acc[r][d]);
       }
+      __builtin_amdgcn_sched_barrier(kOthersMove);
+    }
     if constexpr (kKind == PromptTile::kCareful) add_odd(values, value_read, k0, q0);
   }
 
