@@ -507,22 +507,27 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
 
 // ----------------------------------------------------------------- float32
 
-constexpr int kFloatKeys = 32;
+constexpr int float_keys(int padded) { return padded <= 64 ? 64 : padded <= 128 ? 32 : 16; }
 
-// Float32 on the float32 matrix instructions: four waves of 16 query rows, 32
-// keys at a time through LDS.
+// Float32 on the float32 matrix instructions: four waves of 16 query rows,
+// 16 to 64 keys at a time through LDS.  A sixteenth of the 16-bit products'
+// rate leaves the rest of the work small beside them; the next tile's loads
+// pass registers while this one is used.
 template <int DP>
-__global__ __launch_bounds__(kPromptThreads) void prompt_float_kernel(PromptParams p) {
+__global__ __launch_bounds__(kPromptThreads, DP <= 64 ? 3 : 2) void prompt_float_kernel(PromptParams p) {
   constexpr int kRows = kPromptWaves * 16;
+  constexpr int kKeys = float_keys(DP);
+  constexpr int KT = kKeys / 16;
   constexpr int KS = DP / 16;
   constexpr int DT = DP / 16;
   constexpr int kStride = DP + 4;      // rows of four apart fall on other banks
+  constexpr int kLoads = kKeys * DP / 4 / kPromptThreads;
   extern __shared__ __attribute__((aligned(16))) char s_tiles[];
   float* const s_key = reinterpret_cast<float*>(s_tiles);
-  float* const s_value = s_key + kFloatKeys * kStride;
+  float* const s_value = s_key + kKeys * kStride;
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & (kWave - 1);
-  const int wave = tid / kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane & 15, quarter = lane >> 4;
   const PromptWork w = prompt_work(p);
   zero_rows<float>(p, w);
@@ -538,6 +543,23 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_float_kernel(PromptPara
   for (int block = w.block; block * kRows < length; block += p.blocks) {
     const int q0 = block * kRows + wave * 16;
     const int row = q0 + col;
+    const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
+    f32x4 next_key[kLoads], next_value[kLoads];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = i * kPromptThreads + tid;
+        const int r = k0 + at / (DP / 4), c = at % (DP / 4) * 4;
+        const bool inside = r < length && c < p.width;
+        const int64_t from = inside ? r : 0;
+        const int column = inside ? c : 0;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(key + from * p.key_row + column);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(value + from * p.value_row + column);
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        next_key[i] = inside ? a : zero;
+        next_value[i] = inside ? b : zero;
+      }
+    };
     f32x4 q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -548,92 +570,104 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_float_kernel(PromptPara
                          : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     f32x4 acc[DT];
+    float most, sum;
+    // careful: no value that is not finite reaches a row that does not see it
+    auto run = [&](auto careful) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float most = kMinusInf, sum = 0.0f;
-    const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
-    for (int k0 = 0; k0 < seen; k0 += kFloatKeys) {
-      __syncthreads();
-      for (int i = tid; i < kFloatKeys * (DP / 4); i += kPromptThreads) {
-        const int r = i / (DP / 4), c = (i % (DP / 4)) * 4;
-        f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
-        if (k0 + r < length && c < p.width) {
-          a = *reinterpret_cast<const f32x4*>(key + (k0 + r) * p.key_row + c);
-          b = *reinterpret_cast<const f32x4*>(value + (k0 + r) * p.value_row + c);
+      for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      most = kMinusInf;
+      sum = 0.0f;
+      fetch(0);
+      for (int k0 = 0; k0 < seen; k0 += kKeys) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int at = i * kPromptThreads + tid;
+          const int to = at / (DP / 4) * kStride + at % (DP / 4) * 4;
+          *reinterpret_cast<f32x4*>(s_key + to) = next_key[i];
+          *reinterpret_cast<f32x4*>(s_value + to) = next_value[i];
         }
-        *reinterpret_cast<f32x4*>(s_key + r * kStride + c) = a;
-        *reinterpret_cast<f32x4*>(s_value + r * kStride + c) = b;
-      }
-      __syncthreads();
-      if (k0 > q0 + 15 || q0 >= length) continue;
-      const bool masked = k0 + kFloatKeys - 1 > q0;
-      f32x4 s[2];
+        __syncthreads();
+        if (k0 + kKeys < seen) fetch(k0 + kKeys);
+        if (k0 > q0 + 15 || q0 >= length) continue;
+        f32x4 s[KT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < KT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(s_key + (t * 16 + col) * kStride +
-                                                          k * 16 + quarter * 4);
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], q[k][j], s[t], 0, 0, 0);
+          for (int t = 0; t < KT; ++t) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(s_key + (t * 16 + col) * kStride +
+                                                            k * 16 + quarter * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], q[k][j], s[t], 0, 0, 0);
+          }
+        if (k0 + kKeys - 1 > q0) {
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (k0 + t * 16 + quarter * 4 + i > row) s[t][i] = kMinusInf;
         }
-        if (masked)
+        float top = kMinusInf;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (k0 + t * 16 + quarter * 4 + i > row) s[t][i] = kMinusInf;
-      }
-      float top = kMinusInf;
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
+        top = max_over_rows(top) * p.scale;
+        if (__any(top > most)) {
+          const float now = fmaxf(most, top);
+          const float keep = now == kMinusInf ? 1.0f : exp2_fast(most - now);
+          most = now;
+          sum *= keep;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
-      top = max_over_rows(top) * p.scale;
-      if (__any(top > most)) {
-        const float now = fmaxf(most, top);
-        const float keep = now == kMinusInf ? 1.0f : exp2_fast(most - now);
-        most = now;
-        sum *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= keep;
-      }
-      const float shift = most == kMinusInf ? 0.0f : most;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], p.scale, -shift));
-          sum += s[t][i];
+          for (int d = 0; d < DT; ++d) acc[d] *= keep;
         }
+        const float shift = most == kMinusInf ? 0.0f : most;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = s_value[(t * 16 + quarter * 4 + i) * kStride + d * 16 + col];
-            if (masked && __any(!(__builtin_fabsf(v) < __builtin_huge_valf()))) {
-              // as in the 16-bit kernel
-              const float sees = k0 + t * 16 + quarter * 4 + i <= row ? 1.0f : 0.0f;
-              const float kind[3] = {v != v ? 1.0f : 0.0f,
-                                     v == __builtin_huge_valf() ? 1.0f : 0.0f,
-                                     v == kMinusInf ? 1.0f : 0.0f};
-              if (!(__builtin_fabsf(v) < __builtin_huge_valf())) v = 0.0f;
-#pragma unroll
-              for (int n = 0; n < 3; ++n) {
-                f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-                c = __builtin_amdgcn_mfma_f32_16x16x4f32(kind[n], sees, c, 0, 0, 0);
-                const float add = n == 0 ? __builtin_nanf("")
-                                         : n == 1 ? __builtin_huge_valf() : kMinusInf;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (c[j] > 0.0f) acc[d][j] += add;
-              }
-            }
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[t][i], acc[d], 0, 0, 0);
+            s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], p.scale, -shift));
+            sum += s[t][i];
           }
-    }
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              float v = s_value[(t * 16 + quarter * 4 + i) * kStride + d * 16 + col];
+              if constexpr (decltype(careful)::value) {
+                const float sees = k0 + t * 16 + quarter * 4 + i <= row ? 1.0f : 0.0f;
+                const float kind[3] = {v != v ? 1.0f : 0.0f,
+                                       v == __builtin_huge_valf() ? 1.0f : 0.0f,
+                                       v == kMinusInf ? 1.0f : 0.0f};
+                if (!(__builtin_fabsf(v) < __builtin_huge_valf())) v = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 3; ++n) {
+                  f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+                  c = __builtin_amdgcn_mfma_f32_16x16x4f32(kind[n], sees, c, 0, 0, 0);
+                  const float add = n == 0 ? __builtin_nanf("")
+                                           : n == 1 ? __builtin_huge_valf() : kMinusInf;
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    if (c[j] > 0.0f) acc[d][j] += add;
+                }
+              }
+              acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[t][i], acc[d], 0, 0, 0);
+            }
+      }
+    };
+    run(std::false_type());
+    // as in the 16-bit kernel
+    bool nan = false;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nan |= acc[d][i] != acc[d][i];
+    if (__syncthreads_or(nan)) run(std::true_type());
     const float inverse = 1.0f / sum_over_rows(sum);
     if (row < length) {
       float* const out = static_cast<float*>(p.out) +
@@ -667,7 +701,7 @@ int32_t launch_prompt_kernel(void (*kernel)(PromptParams), int bytes, const Prom
 template <int DP>
 int32_t launch_prompt_float(PromptParams p, int64_t longest, hipStream_t stream) {
   constexpr int kRows = kPromptWaves * 16;
-  constexpr int kBytes = 2 * kFloatKeys * (DP + 4) * 4;
+  constexpr int kBytes = 2 * float_keys(DP) * (DP + 4) * 4;
   p.blocks = static_cast<int32_t>((longest + kRows - 1) / kRows);
   return launch_prompt_kernel(&prompt_float_kernel<DP>, kBytes, p, stream);
 }
