@@ -42,6 +42,7 @@ from .attention import (
     prompt_attention,
     write_kv_cache,
 )
+from .kv_cache import PagedAttention, PagedKVCache
 from .controller import (
     ControllerDecodeGraph,
     ControllerStep,
@@ -61,6 +62,8 @@ __all__ = [
     "FaithfulSDMDecodeState",
     "PackedSDMCopyOnWriteState",
     "PageTableStep",
+    "PagedAttention",
+    "PagedKVCache",
     "PagedSlotMap",
     "SDMCopyOnWriteStep",
     "SDMStepInputs",
