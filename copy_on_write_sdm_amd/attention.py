@@ -68,26 +68,28 @@ def _scale(scale: float | None, width: int) -> float:
     return scale
 
 
-def _rows(tensor: torch.Tensor) -> torch.Tensor:
-    """``tensor`` itself where its rows can be loaded 16 bytes at a time (a
-    slice of a fused projection can), else a contiguous copy."""
+def _rows(tensor: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, ...]]:
+    """``tensor``, its address and its strides where its rows can be loaded 16
+    bytes at a time (a slice of a fused projection can), else those of a
+    contiguous copy."""
 
     step = 16 // tensor.element_size()
-    strides = tensor.stride()
-    if strides[-1] == 1 and not tensor.data_ptr() % 16:
+    strides, address = tensor.stride(), tensor.data_ptr()
+    if strides[-1] == 1 and not address % 16:
         for s in strides[:-1]:
             if s % step:
                 break
         else:
-            return tensor
-    tensor = tensor.contiguous()
-    # contiguous() is the tensor itself where only its address is odd
-    return tensor.clone() if tensor.data_ptr() % 16 else tensor
+            return tensor, address, strides
+    copy = tensor.contiguous()
+    if copy.data_ptr() % 16:        # contiguous as it was, only its address is odd
+        copy = copy.clone()
+    return copy, copy.data_ptr(), copy.stride()
 
 
-def _int32(tensor: torch.Tensor, shape: tuple[int, ...], device: int, what: str) -> None:
-    if tensor.dtype is not _INT32 or tensor.shape != shape or not tensor.is_contiguous():
-        raise ValueError(f"{what} must be contiguous int32 of shape {list(shape)}")
+def _int32(tensor: torch.Tensor, numbers: int, device: int, what: str) -> None:
+    if tensor.dtype is not _INT32 or tensor.numel() != numbers or not tensor.is_contiguous():
+        raise ValueError(f"{what} must be {numbers} contiguous int32 numbers")
     if tensor.get_device() != device:
         raise ValueError(f"{what} must be on the other inputs' device")
 
@@ -108,37 +110,40 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
         raise ValueError("attention takes query [T,heads,D] and key and value [T,kv_heads,D]")
     rows, heads, width = query.shape
-    kv_heads = key.shape[1]
-    if key.shape[0] != rows or key.shape[2] != width:
+    key_rows, kv_heads, key_width = key.shape
+    if key_rows != rows or key_width != width:
         raise ValueError("attention query, key and value do not align")
-    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+    if not kv_heads or not heads or heads % kv_heads:
         raise ValueError("query heads must be a multiple of the key heads")
     cache_width(width)
-    code = _float_type(query.dtype)
-    if key.dtype != query.dtype or value.dtype != query.dtype:
+    dtype = query.dtype
+    code = _float_type(dtype)
+    if key.dtype is not dtype or value.dtype is not dtype:
         raise TypeError("attention query, key and value share one type")
     _need_device(query, "attention inputs")
     device, index = query.device, query.get_device()
     if key.get_device() != index or value.get_device() != index:
         raise ValueError("attention inputs must be on one device")
-    if offsets.ndim != 1 or offsets.numel() == 0:
+    sequences = offsets.numel() - 1
+    if sequences < 0 or offsets.ndim != 1:
         raise ValueError("attention offsets must be a vector of sequences + 1")
-    _int32(offsets, offsets.shape, index, "attention offsets")
-    if longest is not None and longest < 0:
+    _int32(offsets, sequences + 1, index, "attention offsets")
+    if longest is None:
+        longest = rows
+    elif longest < 0:
         raise ValueError("the longest sequence cannot be negative")
     factor = _scale(scale, width)
-    sequences = offsets.numel() - 1
-    if sequences == 0:
-        return torch.zeros(rows, heads, width, device=device, dtype=query.dtype)
-    out = torch.empty(rows, heads, width, device=device, dtype=query.dtype)
-    if rows == 0:
+    if not sequences:
+        return torch.zeros(rows, heads, width, device=device, dtype=dtype)
+    out = torch.empty((rows, heads, width), device=device, dtype=dtype)
+    if not rows:
         return out
-    query, key, value = _rows(query), _rows(key), _rows(value)
-    a = nat.PromptAttention(
-        query.data_ptr(), key.data_ptr(), value.data_ptr(), query.stride(0), query.stride(1),
-        key.stride(0), key.stride(1), value.stride(0), value.stride(1), offsets.data_ptr(),
-        out.data_ptr(), rows, sequences, rows if longest is None else longest, heads, kv_heads,
-        width, code, factor)
+    query, q, (q_row, q_head, _) = _rows(query)
+    key, k, (k_row, k_head, _) = _rows(key)
+    value, v, (v_row, v_head, _) = _rows(value)
+    a = nat.PromptAttention(q, k, v, q_row, q_head, k_row, k_head, v_row, v_head,
+                            offsets.data_ptr(), out.data_ptr(), rows, sequences, longest, heads,
+                            kv_heads, width, code, factor)
     rc = nat.lib().cowsdm_prompt_attention(a, nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_prompt_attention")
@@ -178,24 +183,30 @@ def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: 
     _need_device(lengths, "page tables")
     batch, device, index = lengths.numel(), lengths.device, lengths.get_device()
     columns, pages = page_tables.shape[1], free_pages.numel()
-    _int32(lengths, (batch,), index, "lengths")
-    _int32(added, (batch,), index, "added tokens")
-    _int32(page_tables, (batch, columns), index, "page tables")
-    _int32(free_pages, (pages,), index, "free pages")
-    _int32(free_count, (1,), index, "the free count")
+    _int32(lengths, batch, index, "lengths")
+    _int32(added, batch, index, "added tokens")
+    _int32(page_tables, batch * columns, index, "page tables")
+    _int32(free_pages, pages, index, "free pages")
+    _int32(free_count, 1, index, "the free count")
+    if page_tables.shape[0] != batch:
+        raise ValueError("page tables must have a row for every request")
     if page_tokens not in PAGE_TOKENS:
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
     if tokens < 0:
         raise ValueError("the token count cannot be negative")
     if batch > MAX_REQUESTS:
         raise ValueError(f"page tables take at most {MAX_REQUESTS} requests")
-    sizes = (batch, 1, batch + 1, tokens, tokens, 1)
     if out is None:
+        sizes = (batch, 1, batch + 1, tokens, tokens, 1)
         step = PageTableStep(*torch.empty(sum(sizes), dtype=_INT32, device=device).split(sizes))
     else:
-        step = PageTableStep(*out)
-        for t, n in zip(step, sizes):
-            _int32(t, (n,), index, "page table outputs")
+        step = out if isinstance(out, PageTableStep) else PageTableStep(*out)
+        _int32(step.lengths, batch, index, "the new lengths")
+        _int32(step.free_count, 1, index, "the new free count")
+        _int32(step.offsets, batch + 1, index, "offsets")
+        _int32(step.positions, tokens, index, "positions")
+        _int32(step.slots, tokens, index, "slots")
+        _int32(step.overflow, 1, index, "the overflow flag")
         if batch and step.lengths.data_ptr() == lengths.data_ptr():
             raise ValueError("the new lengths cannot be written over the old")
         if step.free_count.data_ptr() == free_count.data_ptr():
@@ -227,11 +238,12 @@ def _cache(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
     if padded != cache_width(width):
         raise ValueError(f"a cache for heads of {width} is {cache_width(width)} wide")
-    for t in (key_pages, key_scales, value_pages, value_scales):
-        if not t.is_contiguous():
-            raise ValueError("cache tensors must be contiguous")
-        if t.get_device() != device:
-            raise ValueError("cache tensors must be on the inputs' device")
+    if not (key_pages.is_contiguous() and key_scales.is_contiguous()
+            and value_pages.is_contiguous() and value_scales.is_contiguous()):
+        raise ValueError("cache tensors must be contiguous")
+    if not (key_pages.get_device() == key_scales.get_device() == value_pages.get_device()
+            == value_scales.get_device() == device):
+        raise ValueError("cache tensors must be on the inputs' device")
     return nat.KVCache(pages, heads, page_tokens, padded, key_pages.data_ptr(),
                        key_scales.data_ptr(), value_pages.data_ptr(), value_scales.data_ptr())
 
@@ -261,16 +273,16 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
         raise TypeError("cache keys and values share one type")
     if value.get_device() != device:
         raise ValueError("cache writes must be on one device")
-    _int32(slots, (tokens,), device, "cache slots")
+    _int32(slots, tokens, device, "cache slots")
     cache = _cache(key_pages, key_scales, value_pages, value_scales, width, device)
     if cache.heads != heads:
         raise ValueError("cache and keys differ in heads")
     if tokens == 0:
         return
-    key, value = _rows(key), _rows(value)
-    rc = nat.lib().cowsdm_kv_write(
-        cache, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-        value.stride(1), code, width, slots.data_ptr(), tokens, nat.stream_handle(key.device))
+    key, k, (k_row, k_head, _) = _rows(key)
+    value, v, (v_row, v_head, _) = _rows(value)
+    rc = nat.lib().cowsdm_kv_write(cache, k, k_row, k_head, v, v_row, v_head, code, width,
+                                   slots.data_ptr(), tokens, nat.stream_handle(key.device))
     if rc:
         nat.check(rc, "cowsdm_kv_write")
 
@@ -308,24 +320,25 @@ def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: t
     if page_tables.ndim != 2:
         raise ValueError("page tables must be [B,columns]")
     columns = page_tables.shape[1]
-    _int32(page_tables, (batch, columns), index, "page tables")
-    _int32(lengths, (batch,), index, "lengths")
+    if page_tables.shape[0] != batch:
+        raise ValueError("page tables must have a row for every request")
+    _int32(page_tables, batch * columns, index, "page tables")
+    _int32(lengths, batch, index, "lengths")
     room = columns * cache.page_tokens
     if longest is None or longest > room:
         longest = room
     if longest < 0:
         raise ValueError("the longest length cannot be negative")
     factor = _scale(scale, width)
-    out = torch.empty(batch, tokens, heads, width, device=device, dtype=query.dtype)
-    if out.numel() == 0:
+    out = torch.empty((batch, tokens, heads, width), device=device, dtype=query.dtype)
+    if not batch or not tokens:
         return out
-    query = _rows(query)
+    query, q_at, (q_request, q_token, q_head, _) = _rows(query)
     need = cached_workspace_bytes(batch, tokens, heads, cache.heads, width, longest)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     q = nat.CachedQuery(
-        query.data_ptr(), query.stride(0), query.stride(1), query.stride(2),
-        page_tables.data_ptr(), lengths.data_ptr(), out.data_ptr(), batch, tokens, heads, width,
-        columns, longest, code, factor)
+        q_at, q_request, q_token, q_head, page_tables.data_ptr(), lengths.data_ptr(),
+        out.data_ptr(), batch, tokens, heads, width, columns, longest, code, factor)
     rc = nat.lib().cowsdm_cached_attention(cache, q, nat.ptr(workspace), need,
                                      nat.stream_handle(device))
     if rc:

@@ -98,10 +98,12 @@ def test_cache_checks():
 def test_rows_are_copied_only_where_they_cannot_be_loaded():
     x = torch.zeros(6, 8, 64, dtype=torch.bfloat16)
     for kept in (x, x[:, 2:4], x.transpose(0, 1), x[..., 8:24]):
-        assert attention._rows(kept).data_ptr() == kept.data_ptr()
+        tensor, address, strides = attention._rows(kept)
+        assert tensor is kept and address == kept.data_ptr() and strides == kept.stride()
     for copied in (x[..., 1:9], x[..., ::2], torch.zeros(6, 8, 65)[..., :64]):
-        assert attention._rows(copied).data_ptr() != copied.data_ptr()
-        assert attention._rows(copied).is_contiguous()
+        tensor, address, strides = attention._rows(copied)
+        assert address == tensor.data_ptr() != copied.data_ptr() and tensor.is_contiguous()
+        assert strides == tensor.stride() and torch.equal(tensor, copied)
 
 
 def test_c_entries_refuse_without_launching():
