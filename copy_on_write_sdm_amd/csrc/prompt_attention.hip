@@ -28,6 +28,7 @@ struct PromptParams {
   int32_t kv_heads;
   int32_t width;
   int32_t blocks;                  // query blocks of a sequence and head in the grid
+  int32_t pair_by_pair;            // the grid's order
   float scale;                     // times log2(e)
 };
 
@@ -37,27 +38,32 @@ struct PromptWork {
   int sequence, head, kv, block;
 };
 
-// The workgroups of one sequence and key head follow one another on one XCD
-// (workgroup n runs on XCD n % 8), so that its keys and values stay in that
-// XCD's L2; later query blocks, which see more keys, come first.
+// Workgroup n runs on XCD n % 8: a pair of a sequence and a key head keeps to
+// one XCD where the pairs divide by eight, so that its keys and values stay
+// in that XCD's L2.  Later query blocks, which see more keys, come first: of
+// all pairs in small grids, where what starts last decides (16 heads of 4,096
+// tokens: 92 us, pair by pair 118), and pair by pair in large ones, whose keys
+// and values would push each other out (2 x 8,192: 1,015 against 1,031).
 __device__ __forceinline__ PromptWork prompt_work(const PromptParams& p) {
   const int group = p.heads / p.kv_heads;
-  const int each = p.blocks * group;
   const int pairs = p.sequences * p.kv_heads;
-  int id = static_cast<int>(blockIdx.x), pair, rest;
-  if (pairs % 8 == 0) {
-    const int k = id >> 3;
-    pair = (k / each) * 8 + (id & 7);
-    rest = k % each;
+  const int sides = pairs % 8 == 0 ? 8 : 1;
+  const int id = static_cast<int>(blockIdx.x) / sides;
+  const int own = pairs / sides;              // pairs of this XCD
+  int pair, block;
+  if (p.pair_by_pair) {
+    pair = id / (p.blocks * group);
+    block = id / group % p.blocks;
   } else {
-    pair = id / each;
-    rest = id % each;
+    pair = id / group % own;
+    block = id / (group * own);
   }
+  pair = pair * sides + static_cast<int>(blockIdx.x) % sides;
   PromptWork w;
   w.sequence = pair / p.kv_heads;
   w.kv = pair - w.sequence * p.kv_heads;
-  w.block = p.blocks - 1 - rest / group;
-  w.head = w.kv * group + rest % group;
+  w.block = p.blocks - 1 - block;
+  w.head = w.kv * group + id % group;
   return w;
 }
 
@@ -132,13 +138,13 @@ __device__ __forceinline__ void load_to_lds(const void* first, int bytes, uint32
 
 // This thread's chunks of a tile into LDS, a wave's side by side.  Rows past
 // the sequence's end and columns past the width read as 0.
-template <int kLoads>
+template <int kLoads, int kThreads>
 __device__ __forceinline__ void load_rows(const void* first, int rows, int64_t stride, int width,
                                           const uint32_t (&from)[kLoads], lds_char* to) {
   const int bytes = static_cast<int>((rows - 1) * stride + width) * 2;
 #pragma unroll
   for (int i = 0; i < kLoads; ++i)
-    load_to_lds(first, bytes, from[i], to + i * kPromptThreads * 16);
+    load_to_lds(first, bytes, from[i], to + i * kThreads * 16);
 }
 
 // Four keys of this lane's column from a tile in LDS, each group of 16 lanes
@@ -167,10 +173,10 @@ constexpr int kOthersMove = 0x406;       // a scheduling barrier that vector and
 // edge, and no value that is not finite reaches a row that does not see it.
 enum class PromptTile { kWhole, kEdge, kCareful };
 
-// One wave's RB * 32 query rows of one head: q the rows, acc their products
-// so far, transposed, most the maxima that the probabilities are relative to
-// and sum their sums (of this lane's keys).
-template <typename T, int DP, int RB>
+// One wave's 32 query rows of one head: q the rows, acc their products so far,
+// transposed, most the maxima that the probabilities are relative to and sum
+// their sums (of this lane's keys).
+template <typename T, int DP>
 struct PromptRows {
   using vec = typename Half<T>::vec;
   static constexpr int KS = DP / 16;       // products along the width
@@ -178,20 +184,17 @@ struct PromptRows {
   // steps that operands are read ahead of their products, as registers allow
   static constexpr int kKeysAhead = DP <= 192 ? 3 : 1;
   static constexpr int kValuesAhead = DP <= 192 ? 1 : 0;
-  vec q[RB][KS];
-  f32x16 acc[RB][DT];
-  float most[RB], sum[RB];
+  vec q[KS];
+  f32x16 acc[DT];
+  float most, sum;
 
   __device__ __forceinline__ void clear() {
+    most = kMinusInf;
+    sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      most[r] = kMinusInf;
-      sum[r] = 0.0f;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[r][d][i] = 0.0f;
-    }
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
   }
 
   // The value operand of step h (16 keys) of column tile d.
@@ -202,6 +205,17 @@ struct PromptRows {
     return __builtin_bit_cast(vec, both);
   }
 
+  // The maxima grow to `now`.
+  __device__ __forceinline__ void rise(float now) {
+    const float keep = now == kMinusInf ? 1.0f : exp2_fast(most - now);
+    most = now;
+    sum *= keep;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] *= keep;
+  }
+
   // One tile of 64 keys from row k0 on.
   template <PromptTile kKind>
   __device__ __forceinline__ void tile(const lds_char* keys, const lds_char* values,
@@ -210,13 +224,11 @@ struct PromptRows {
                                        int q0) {
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int col = lane & 31, half = lane >> 5;
-    f32x16 s[RB][2];
+    f32x16 s[2];
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[r][kb][i] = 0.0f;
+      for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
     // operands are read from LDS some steps before the products that take
     // them, and are kept there: left to itself the compiler reads each at its
     // product, whose wait is longer than the product
@@ -234,9 +246,7 @@ struct PromptRows {
       if (k + kKeysAhead < KS) read_keys(k + kKeysAhead);
       __builtin_amdgcn_sched_barrier(kOthersMove);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < RB; ++r) s[r][kb] = Half<T>::mfma(key[k][kb], q[r][k], s[r][kb]);
+      for (int kb = 0; kb < 2; ++kb) s[kb] = Half<T>::mfma(key[k][kb], q[k], s[kb]);
       __builtin_amdgcn_sched_barrier(kOthersMove);
     }
     vec value[4][DT];
@@ -246,50 +256,38 @@ struct PromptRows {
     };
     if constexpr (kValuesAhead > 0) read_values(0);
     __builtin_amdgcn_sched_barrier(kOthersMove);
-    vec prob[RB][4];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      if constexpr (kKind != PromptTile::kWhole) {
-        const int row = q0 + r * 32 + col;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 > row) s[r][kb][i] = kMinusInf;
-      }
-      float top = kMinusInf;
+    if constexpr (kKind != PromptTile::kWhole) {
+      const int row = q0 + col;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[r][kb][i]);
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
-                                                      false, false);
-      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * scale;
-      // The maximum that the probabilities are relative to moves only when a
-      // row's grows past 2^8 of it: sums of numbers up to 2^8 lose nothing in
-      // 32 bits, and a probability keeps its bits in 16.
-      if (__any(top > most[r] + 8.0f)) {
-        const float now = fmaxf(most[r], top);
-        const float keep = now == kMinusInf ? 1.0f : exp2_fast(most[r] - now);
-        most[r] = now;
-        sum[r] *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[r][d][i] *= keep;
-      }
-      const float shift = most[r] == kMinusInf ? 0.0f : most[r];
-      float part[4] = {};
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = exp2_fast(__builtin_fmaf(s[r][kb][i], scale, -shift));
-          part[i % 4] += e;
-          prob[r][2 * kb + i / 8][i % 8] = static_cast<T>(e);
-        }
-      sum[r] += (part[0] + part[1]) + (part[2] + part[3]);
+        for (int i = 0; i < 16; ++i)
+          if (k0 + kb * 32 + (i / 4) * 8 + half * 4 + i % 4 > row) s[kb][i] = kMinusInf;
     }
+    float top = kMinusInf;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
+                                                    false, false);
+    top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * scale;
+    // The maximum that the probabilities are relative to moves only when a
+    // row's grows past 2^8 of it: sums of numbers up to 2^8 lose nothing in
+    // 32 bits, and a probability keeps its bits in 16.
+    if (__any(top > most + 8.0f)) rise(fmaxf(most, top));
+    const float shift = most == kMinusInf ? 0.0f : most;
+    vec prob[4];
+    float part[4] = {};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_fast(__builtin_fmaf(s[kb][i], scale, -shift));
+        part[i % 4] += e;
+        prob[2 * kb + i / 8][i % 8] = static_cast<T>(e);
+      }
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       if (h + kValuesAhead < 4) read_values(h + kValuesAhead);
@@ -303,8 +301,7 @@ struct PromptRows {
             if (!(__builtin_fabsf(static_cast<float>(v[j])) < __builtin_huge_valf()))
               v[j] = static_cast<T>(0.0f);
         }
-#pragma unroll
-        for (int r = 0; r < RB; ++r) acc[r][d] = Half<T>::mfma(v, prob[r][h], acc[r][d]);
+        acc[d] = Half<T>::mfma(v, prob[h], acc[d]);
       }
       __builtin_amdgcn_sched_barrier(kOthersMove);
     }
@@ -315,11 +312,9 @@ struct PromptRows {
   __device__ __forceinline__ bool any_nan() const {
     bool nan = false;
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) nan |= acc[r][d][i] != acc[r][d][i];
+      for (int i = 0; i < 16; ++i) nan |= acc[d][i] != acc[d][i];
     return nan;
   }
 
@@ -330,58 +325,87 @@ struct PromptRows {
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int col = lane & 31, half = lane >> 5;
 #pragma unroll 1
-    for (int h = 0; h < 4; ++h)
+    for (int h = 0; h < 4; ++h) {
+      vec sees;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        sees[j] = static_cast<T>(
+            k0 + h * 16 + (j / 4) * 8 + half * 4 + j % 4 <= q0 + col ? 1.0f : 0.0f);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const vec v = turned(values, value_read, h, d);
         if (!__any(any_odd<T>(v))) continue;
-#pragma unroll
-        for (int r = 0; r < RB; ++r) {
-          vec sees;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            sees[j] = static_cast<T>(
-                k0 + h * 16 + (j / 4) * 8 + half * 4 + j % 4 <= q0 + r * 32 + col ? 1.0f : 0.0f);
 #pragma unroll 1
-          for (int n = 0; n < 3; ++n) {
-            vec kind;
-            const float sign = n == 1 ? __builtin_huge_valf() : kMinusInf;
+        for (int n = 0; n < 3; ++n) {
+          vec kind;
+          const float sign = n == 1 ? __builtin_huge_valf() : kMinusInf;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float x = static_cast<float>(v[j]);
-              kind[j] = static_cast<T>((n == 0 ? x != x : x == sign) ? 1.0f : 0.0f);
-            }
-            f32x16 c;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) c[i] = 0.0f;
-            c = Half<T>::mfma(kind, sees, c);
-            const float add = n == 0 ? __builtin_nanf("") : sign;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c[i] > 0.0f) acc[r][d][i] += add;
+          for (int j = 0; j < 8; ++j) {
+            const float x = static_cast<float>(v[j]);
+            kind[j] = static_cast<T>((n == 0 ? x != x : x == sign) ? 1.0f : 0.0f);
           }
+          f32x16 c;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+          c = Half<T>::mfma(kind, sees, c);
+          const float add = n == 0 ? __builtin_nanf("") : sign;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c[i] > 0.0f) acc[d][i] += add;
         }
       }
+    }
+  }
+
+  // The rows' numbers to and from LDS, a register of the wave's lanes after
+  // the other.
+  static constexpr int kFloats = (DT * 16 + 2) * kWave;
+  typedef __attribute__((address_space(3))) float lds_float;
+  __device__ __forceinline__ void give(lds_float* to) const {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) to[(d * 16 + i) * kWave + lane] = acc[d][i];
+    to[DT * 16 * kWave + lane] = most;
+    to[(DT * 16 + 1) * kWave + lane] = sum;
+  }
+  __device__ __forceinline__ void join(const lds_float* from) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const float other = from[DT * 16 * kWave + lane];
+    rise(fmaxf(most, other));
+    const float keep = other == kMinusInf ? 0.0f : exp2_fast(other - most);
+    sum += from[(DT * 16 + 1) * kWave + lane] * keep;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] += from[(d * 16 + i) * kWave + lane] * keep;
   }
 };
 
-// One workgroup: four waves of RB * 32 query rows each of one head.  Keys and
-// values come through LDS, 64 at a time, by loads that go to LDS without
-// passing registers; the next tile is on its way while this one is used.
-template <typename T, int DP, int RB>
+// One workgroup: four waves and 128 query rows of one head, 32 to a wave.
+// Keys and values come through LDS, 64 at a time, by loads that go to LDS
+// without passing registers; the next tile is on its way while this one is
+// used.  KP = 2: 64 rows, of which two waves share 32; one takes the even and
+// one the odd tiles, and their sums are joined at the end.  That is for grids
+// that leave CUs empty, where the longest row's way through its keys counts.
+template <typename T, int DP, int KP>
 __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half_kernel(
     PromptParams p) {
-  using Rows = PromptRows<T, DP, RB>;
+  using Rows = PromptRows<T, DP>;
   using vec = typename Half<T>::vec;
   constexpr int KS = Rows::KS, DT = Rows::DT;
-  constexpr int kRows = kPromptWaves * RB * 32;
+  constexpr int kSide = kPromptThreads / KP;           // threads that share a tile
+  constexpr int kRows = kSide / 2;
   constexpr int kTileBytes = kTileKeys * DP * 2;
-  constexpr int kLoads = kTileBytes / (16 * kPromptThreads);
-  extern __shared__ __attribute__((aligned(16))) char s_tiles[];   // [2][keys, values]
-  lds_char* const tiles = (lds_char*)s_tiles;
-  const int tid = static_cast<int>(threadIdx.x);
-  const int lane = tid & (kWave - 1);
+  constexpr int kLoads = kTileBytes / (16 * kSide);
+  extern __shared__ __attribute__((aligned(16))) char s_tiles[];   // [KP][2][keys, values]
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int side = KP == 1 ? 0
+                           : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kSide);
+  const int tid = static_cast<int>(threadIdx.x) - side * kSide;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  lds_char* const tiles = (lds_char*)s_tiles + side * 4 * kTileBytes;
   const int col = lane & 31, half = lane >> 5;
   const PromptWork w = prompt_work(p);
   zero_rows<T>(p, w);
@@ -396,7 +420,7 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
   uint32_t key_from[kLoads], value_from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int at = i * kPromptThreads + tid;
+    const int at = i * kSide + tid;
     const int row = at / (DP / 8), c = place<DP>(row, at % (DP / 8));
     const bool inside = c * 8 < p.width;
     key_from[i] = inside ? row * static_cast<uint32_t>(p.key_row * 2) + c * 16 : 0x80000000u;
@@ -406,9 +430,9 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
     const int first = tile * kTileKeys;
     const int rows = length - first < kTileKeys ? length - first : kTileKeys;
     lds_char* const to = tiles + buffer * 2 * kTileBytes + wave * kWave * 16;
-    load_rows<kLoads>(key + first * p.key_row, rows, p.key_row, p.width, key_from, to);
-    load_rows<kLoads>(value + first * p.value_row, rows, p.value_row, p.width, value_from,
-                      to + kTileBytes);
+    load_rows<kLoads, kSide>(key + first * p.key_row, rows, p.key_row, p.width, key_from, to);
+    load_rows<kLoads, kSide>(value + first * p.value_row, rows, p.value_row, p.width,
+                             value_from, to + kTileBytes);
   };
   // this lane's reads of a tile: keys by row col, values turned four keys of
   // 16 columns at a time
@@ -428,48 +452,53 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
   }
 
   for (int block = w.block; block * kRows < length; block += p.blocks) {
-    const int q0 = block * kRows + wave * RB * 32;      // this wave's first row
+    const int q0 = block * kRows + wave * 32;           // this wave's first row
     const int seen = (block + 1) * kRows < length ? (block + 1) * kRows : length;
     const int count = (seen + kTileKeys - 1) / kTileKeys;
-    __syncthreads();            // the tiles of the block before are used
-    load_tile(0, 0);
-    auto arrived = [&](int tile, int buffer) {
+    // a turn takes KP tiles, one for each side
+    const int turns = (count + KP - 1) / KP;
+    auto load_turn = [&](int turn, int buffer) {
+      if (KP == 1 || turn * KP + side < count) load_tile(turn * KP + side, buffer);
+    };
+    auto arrived = [&](int turn, int buffer) {
       __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this thread's part has arrived
       __syncthreads();                         // everyone's; the other buffer is used
-      if (tile + 1 < count) load_tile(tile + 1, buffer ^ 1);
+      if (turn + 1 < turns) load_turn(turn + 1, buffer ^ 1);
     };
+    __syncthreads();            // the tiles of the block before are used
+    load_turn(0, 0);
     Rows rows;
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const int row = q0 + r * 32 + col;
+    {
+      const int row = q0 + col;
       const T* const src = query + static_cast<int64_t>(row < length ? row : 0) * p.query_row;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d = s * 16 + half * 8;
-        rows.q[r][s] = d < p.width ? *reinterpret_cast<const vec*>(src + d) : vec{};
+        rows.q[s] = d < p.width ? *reinterpret_cast<const vec*>(src + d) : vec{};
       }
     }
     rows.clear();
     // Tiles before the block's first row are seen by all of its rows; what
-    // follows, to the diagonal, has a loop of its own.  The first are a
-    // multiple of two, so that a buffer's address is part of the instructions.
-    const int whole = block * (kRows / kTileKeys);
-    for (int tile = 0; tile < whole; tile += 2) {
+    // follows, to the diagonal, has a loop of its own.  The first go two turns
+    // at a time, so that a buffer's address is part of the instructions.
+    const int whole = block * (kRows / kTileKeys) / KP / 2 * 2;
+    for (int turn = 0; turn < whole; turn += 2) {
 #pragma unroll
       for (int buffer = 0; buffer < 2; ++buffer) {
-        arrived(tile + buffer, buffer);
+        arrived(turn + buffer, buffer);
         const lds_char* const keys = tiles + buffer * 2 * kTileBytes;
         rows.template tile<PromptTile::kWhole>(keys, keys + kTileBytes, key_read, value_read,
-                                               p.scale, (tile + buffer) * kTileKeys, q0);
+                                               p.scale,
+                                               ((turn + buffer) * KP + side) * kTileKeys, q0);
       }
     }
     auto edges = [&](auto kind, int from) {
 #pragma unroll 1
-      for (int tile = from; tile < count; ++tile) {
-        arrived(tile, tile & 1);
-        const int k0 = tile * kTileKeys;
-        const lds_char* const keys = tiles + (tile & 1) * 2 * kTileBytes;
-        if (k0 <= q0 + RB * 32 - 1 && q0 < length)
+      for (int turn = from; turn < turns; ++turn) {
+        arrived(turn, turn & 1);
+        const int tile = turn * KP + side, k0 = tile * kTileKeys;
+        const lds_char* const keys = tiles + (turn & 1) * 2 * kTileBytes;
+        if (tile < count && k0 <= q0 + 31 && q0 < length)
           rows.template tile<decltype(kind)::value>(keys, keys + kTileBytes, key_read,
                                                     value_read, p.scale, k0, q0);
       }
@@ -480,28 +509,34 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
     // block that has one at its end is done again with care.
     if (__syncthreads_or(rows.any_nan())) {
       rows.clear();
-      load_tile(0, 0);
+      load_turn(0, 0);
       edges(std::integral_constant<PromptTile, PromptTile::kCareful>(), 0);
     }
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const auto x = __builtin_amdgcn_permlane32_swap(
-          __float_as_uint(rows.sum[r]), __float_as_uint(rows.sum[r]), false, false);
-      const float inverse = 1.0f / (__uint_as_float(x[0]) + __uint_as_float(x[1]));
-      const int row = q0 + r * 32 + col;
-      if (row >= length) continue;
-      T* const out = static_cast<T*>(p.out) +
-                     ((static_cast<int64_t>(begin) + row) * p.heads + w.head) * p.width;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = d * 32 + i * 8 + half * 4;
-          const f32x16& a = rows.acc[r][d];
-          if (at < p.width)
-            store4(out + at, f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]} * inverse);
-        }
+    if constexpr (KP == 2) {
+      using lds_float = typename Rows::lds_float;
+      lds_float* const given = (lds_float*)s_tiles + wave * Rows::kFloats;
+      __syncthreads();          // the last tiles are used
+      if (side == 1) rows.give(given);
+      __syncthreads();
+      if (side == 1) continue;
+      rows.join(given);
     }
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(rows.sum),
+                                                    __float_as_uint(rows.sum), false, false);
+    const float inverse = 1.0f / (__uint_as_float(x[0]) + __uint_as_float(x[1]));
+    const int row = q0 + col;
+    if (row >= length) continue;
+    T* const out = static_cast<T*>(p.out) +
+                   ((static_cast<int64_t>(begin) + row) * p.heads + w.head) * p.width;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = d * 32 + i * 8 + half * 4;
+        const f32x16& a = rows.acc[d];
+        if (at < p.width)
+          store4(out + at, f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]} * inverse);
+      }
   }
 }
 
@@ -683,10 +718,12 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 64 ? 3 : 2) void prompt_float
 
 // ---------------------------------------------------------------- launches
 
-int32_t launch_prompt_kernel(void (*kernel)(PromptParams), int bytes, const PromptParams& p,
-                             hipStream_t stream) {
+int32_t launch_prompt_kernel(void (*kernel)(PromptParams), int bytes, int rows, int64_t longest,
+                             PromptParams p, hipStream_t stream) {
+  p.blocks = static_cast<int32_t>((longest + rows - 1) / rows);
   const int64_t grid = static_cast<int64_t>(p.blocks) * p.heads * p.sequences;
   if (grid > INT32_MAX) return fail(COWSDM_ELIMIT, "prompt_attention: too many workgroups");
+  p.pair_by_pair = grid > 2048;        // four rounds of two workgroups a CU
   if (bytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -699,19 +736,28 @@ int32_t launch_prompt_kernel(void (*kernel)(PromptParams), int bytes, const Prom
 }
 
 template <int DP>
-int32_t launch_prompt_float(PromptParams p, int64_t longest, hipStream_t stream) {
-  constexpr int kRows = kPromptWaves * 16;
+int32_t launch_prompt_float(const PromptParams& p, int64_t longest, hipStream_t stream) {
   constexpr int kBytes = 2 * float_keys(DP) * (DP + 4) * 4;
-  p.blocks = static_cast<int32_t>((longest + kRows - 1) / kRows);
-  return launch_prompt_kernel(&prompt_float_kernel<DP>, kBytes, p, stream);
+  return launch_prompt_kernel(&prompt_float_kernel<DP>, kBytes, kPromptWaves * 16, longest, p,
+                              stream);
 }
 
-template <typename T, int DP, int RB>
-int32_t launch_prompt_half(PromptParams p, int64_t longest, hipStream_t stream) {
-  constexpr int kRows = kPromptWaves * RB * 32;
-  constexpr int kBytes = 2 * 2 * kTileKeys * DP * 2;
-  p.blocks = static_cast<int32_t>((longest + kRows - 1) / kRows);
-  return launch_prompt_kernel(&prompt_half_kernel<T, DP, RB>, kBytes, p, stream);
+template <typename T, int DP>
+int32_t launch_prompt_half(const PromptParams& p, int64_t longest, hipStream_t stream) {
+  constexpr int kTiles = 2 * 2 * kTileKeys * DP * 2;
+  if constexpr (DP <= 128) {
+    // Where 64 rows a workgroup leave the chip's 256 CUs no second one: 8 heads
+    // of 1,000 tokens at width 128 take 18 us so and 24 us by 128 rows.  Short
+    // rows lose by the join (4 prompts of 100: 11.6 against 10.4), and more
+    // workgroups by their tiles' traffic (16 heads of 4,096: 127 against 119).
+    const int64_t most = (static_cast<int64_t>(p.rows) / 64 + p.sequences) * p.heads;
+    constexpr int kJoin = 2 * PromptRows<T, DP>::kFloats * 4;
+    if (most <= 256 && longest >= 512)
+      return launch_prompt_kernel(&prompt_half_kernel<T, DP, 2>,
+                                  2 * kTiles > kJoin ? 2 * kTiles : kJoin, 64, longest, p,
+                                  stream);
+  }
+  return launch_prompt_kernel(&prompt_half_kernel<T, DP, 1>, kTiles, 128, longest, p, stream);
 }
 
 template <typename T>
@@ -725,12 +771,12 @@ int32_t launch_prompt(const PromptParams& p, int64_t longest, hipStream_t stream
     if (w <= 192) return launch_prompt_float<192>(p, longest, stream);
     return launch_prompt_float<256>(p, longest, stream);
   } else {
-    if (w <= 32) return launch_prompt_half<T, 32, 1>(p, longest, stream);
-    if (w <= 64) return launch_prompt_half<T, 64, 1>(p, longest, stream);
-    if (w <= 96) return launch_prompt_half<T, 96, 1>(p, longest, stream);
-    if (w <= 128) return launch_prompt_half<T, 128, 1>(p, longest, stream);
-    if (w <= 192) return launch_prompt_half<T, 192, 1>(p, longest, stream);
-    return launch_prompt_half<T, 256, 1>(p, longest, stream);
+    if (w <= 32) return launch_prompt_half<T, 32>(p, longest, stream);
+    if (w <= 64) return launch_prompt_half<T, 64>(p, longest, stream);
+    if (w <= 96) return launch_prompt_half<T, 96>(p, longest, stream);
+    if (w <= 128) return launch_prompt_half<T, 128>(p, longest, stream);
+    if (w <= 192) return launch_prompt_half<T, 192>(p, longest, stream);
+    return launch_prompt_half<T, 256>(p, longest, stream);
   }
 }
 
