@@ -46,6 +46,17 @@ __device__ __forceinline__ float sum_over_rows(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Of up to 64 numbers below 2^24, lane i's number n, the lane whose number has
+// `place` larger ones: the largest first, equal ones by lane.  Lanes from
+// `count` on hold none.
+__device__ __forceinline__ int lane_by_size(int n, int count, int place) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int key = lane < count ? n * kWave + (kWave - 1 - lane) : -1;
+  int rank = 0;
+  for (int j = 0; j < count; ++j) rank += __builtin_amdgcn_readlane(key, j) > key ? 1 : 0;
+  return __builtin_ctzll(__ballot(lane < count && rank == place));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // eight consecutive elements in float32

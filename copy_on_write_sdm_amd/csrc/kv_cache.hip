@@ -552,6 +552,7 @@ struct CachedParams {
   int32_t chunk;                   // tokens of a split
   int32_t splits;
   int32_t row_tiles;
+  int32_t by_length;               // the longest requests come first
 };
 
 // A split's block: the 16 rows' largest logits and sums, then their products
@@ -604,10 +605,20 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
   const int split = blockIdx.x % p.splits;
   const int tile = blockIdx.x / p.splits;
   const int kv = blockIdx.y;
-  const int request = blockIdx.z;
   const int page = 1 << p.page_shift;
   const int group = p.heads / p.kv_heads;
-  const int length = cached_length(p, request);
+  int request = blockIdx.z, length;
+  if (p.by_length) {
+    // More workgroups than the chip holds at once: the longest requests come
+    // first, so that short ones fill what they leave (64 requests of up to
+    // 2,560 tokens, 8 key heads: 43 us, in their own order 46.5).
+    const int n = lane < p.requests ? p.lengths[lane] : 0, most = p.columns << p.page_shift;
+    const int mine = n < 0 ? 0 : n < most ? n : most;
+    request = lane_by_size(mine, p.requests, blockIdx.z);
+    length = __builtin_amdgcn_readlane(mine, request);
+  } else {
+    length = cached_length(p, request);
+  }
   const int begin = split * p.chunk;
   if (begin >= length && split > 0) return;
   // the last split takes what a longest length given too short leaves
@@ -970,15 +981,16 @@ void launch_cached_width(int64_t padded, const CachedParams& p, hipStream_t stre
   }
 }
 
+constexpr int64_t kCachedWorkgroups = 256;      // one a CU
+
 // The splits of the cache that a call's launch makes: enough workgroups to
 // fill the chip, none with less than two blocks a wave.
 int64_t cached_splits(int64_t requests, int64_t kv_heads, int64_t row_tiles, int64_t padded,
                       int64_t longest) {
-  constexpr int64_t kWorkgroups = 256;
   const int64_t least = 2 * cached_waves(padded) * kCachedTokens;
   const int64_t rows = requests * kv_heads * row_tiles;
   const int64_t most = (longest + least - 1) / least;
-  int64_t splits = rows > 0 ? (kWorkgroups + rows - 1) / rows : 1;
+  int64_t splits = rows > 0 ? (kCachedWorkgroups + rows - 1) / rows : 1;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits;
 }
@@ -1186,6 +1198,9 @@ extern "C" int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
   const int64_t each = (q.longest + p.splits - 1) / p.splits;
   p.chunk = p.splits == 1 ? INT32_MAX / 2
                           : static_cast<int32_t>((each + kBlock - 1) / kBlock * kBlock);
+  p.by_length = q.requests > 1 && q.requests <= kWave && p.splits == 1 &&
+                q.requests * cache->heads * tiles > kCachedWorkgroups &&
+                q.columns * cache->page_tokens < (1 << 24);
   if (p.splits > 1) {
     const int64_t need = cowsdm_cached_attention_workspace_bytes(
         q.requests, q.tokens, q.heads, cache->heads, cache->width, q.longest);

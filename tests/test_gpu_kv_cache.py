@@ -412,3 +412,18 @@ def test_cached_offsets_past_32_bits(device):
     got = cow.cached_attention(q, *cache, ints(tables, device), ints([150], device))
     want = cow.cached_attention(q, *small, ints([[0, 1, 2]], device), ints([150], device))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("batch", [33, 64, 65])
+def test_cached_requests_longest_first(device, batch):
+    """More workgroups than run at once, where up to 64 requests are taken by
+    their length: every request is taken once, equal and empty ones too."""
+
+    rng = np.random.default_rng(batch)
+    lengths = [int(n) for n in rng.integers(0, 90, batch)]
+    lengths[3:9] = [17] * 6
+    lengths[10] = lengths[batch - 1] = 0
+    cache, numbers, tables = filled(lengths, 8, 32, 16, device, batch)
+    got = check_cached(queries(batch, 1, 8, 32, torch.float32, 1, device), cache, numbers, tables,
+                       lengths, device)
+    assert not got[10].any()
