@@ -214,8 +214,8 @@ def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: 
     rc = nat.lib().cowsdm_page_tables_extend(
         lengths.data_ptr(), added.data_ptr(), batch, page_tables.data_ptr(), columns,
         free_pages.data_ptr(), pages, free_count.data_ptr(), page_tokens, tokens,
-        step.lengths.data_ptr(), step.free_count.data_ptr(), step.offsets.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(),
-        step.overflow.data_ptr(), nat.stream_handle(device))
+        step.lengths.data_ptr(), step.free_count.data_ptr(), step.offsets.data_ptr(),
+        step.positions.data_ptr(), step.slots.data_ptr(), step.overflow.data_ptr(), nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_page_tables_extend")
     return step

@@ -19,12 +19,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kMostCode = 448.0f;         // the largest e4m3 number
-constexpr uint32_t kNanCode = 0x7f;
 
 // the row widths the cache is laid out for: a head's width is padded with
 // zeros to the next one
-constexpr int kCacheWidths[] = {32, 64, 96, 128, 192, 256};
-
 __host__ __device__ constexpr bool is_cache_width(int64_t w) {
   return w == 32 || w == 64 || w == 96 || w == 128 || w == 192 || w == 256;
 }
