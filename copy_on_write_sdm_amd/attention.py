@@ -40,12 +40,16 @@ PAGE_TOKENS = (16, 32, 64, 128, 256)
 CACHE_WIDTHS = (32, 64, 96, 128, 192, 256)
 
 
+_PADDED = {w: next(c for c in CACHE_WIDTHS if c >= w) for w in range(8, 257, 8)}
+
+
 def cache_width(head_width: int) -> int:
     """The row width of a cache for heads of ``head_width``."""
 
-    if head_width <= 0 or head_width % 8 or head_width > CACHE_WIDTHS[-1]:
+    padded = _PADDED.get(head_width)
+    if padded is None:
         raise ValueError("attention head width must be a multiple of 8, at most 256")
-    return next(w for w in CACHE_WIDTHS if w >= head_width)
+    return padded
 
 
 def _need_device(tensor: torch.Tensor, what: str) -> None:
@@ -68,19 +72,17 @@ def _scale(scale: float | None, width: int) -> float:
     return scale
 
 
-def _rows(tensor: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, ...]]:
+def _rows(tensor: torch.Tensor, step: int) -> tuple[torch.Tensor, int, tuple[int, ...]]:
     """``tensor``, its address and its strides where its rows can be loaded 16
-    bytes at a time (a slice of a fused projection can), else those of a
-    contiguous copy."""
+    bytes (``step`` elements) at a time, as a slice of a fused projection can,
+    else those of a contiguous copy."""
 
-    step = 16 // tensor.element_size()
     strides, address = tensor.stride(), tensor.data_ptr()
-    if strides[-1] == 1 and not address % 16:
-        for s in strides[:-1]:
-            if s % step:
-                break
-        else:
-            return tensor, address, strides
+    together = 0
+    for s in strides[:-1]:
+        together |= s
+    if strides[-1] == 1 and not together % step and not address % 16:
+        return tensor, address, strides
     copy = tensor.contiguous()
     if copy.data_ptr() % 16:        # contiguous as it was, only its address is odd
         copy = copy.clone()
@@ -135,12 +137,13 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     factor = _scale(scale, width)
     if not sequences:
         return torch.zeros(rows, heads, width, device=device, dtype=dtype)
-    out = torch.empty((rows, heads, width), device=device, dtype=dtype)
+    out = query.new_empty((rows, heads, width))
     if not rows:
         return out
-    query, q, (q_row, q_head, _) = _rows(query)
-    key, k, (k_row, k_head, _) = _rows(key)
-    value, v, (v_row, v_head, _) = _rows(value)
+    step = 8 if code else 4
+    query, q, (q_row, q_head, _) = _rows(query, step)
+    key, k, (k_row, k_head, _) = _rows(key, step)
+    value, v, (v_row, v_head, _) = _rows(value, step)
     a = nat.PromptAttention(q, k, v, q_row, q_head, k_row, k_head, v_row, v_head,
                             offsets.data_ptr(), out.data_ptr(), rows, sequences, longest, heads,
                             kv_heads, width, code, factor)
@@ -201,12 +204,17 @@ def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: 
         step = PageTableStep(*torch.empty(sum(sizes), dtype=_INT32, device=device).split(sizes))
     else:
         step = out if isinstance(out, PageTableStep) else PageTableStep(*out)
-        _int32(step.lengths, batch, index, "the new lengths")
-        _int32(step.free_count, 1, index, "the new free count")
-        _int32(step.offsets, batch + 1, index, "offsets")
-        _int32(step.positions, tokens, index, "positions")
-        _int32(step.slots, tokens, index, "slots")
-        _int32(step.overflow, 1, index, "the overflow flag")
+        a, b, c, d, e, f = step
+        if not (a.dtype is b.dtype is c.dtype is d.dtype is e.dtype is f.dtype is _INT32
+                and a.numel() == batch and b.numel() == 1 and c.numel() == batch + 1
+                and d.numel() == e.numel() == tokens and f.numel() == 1
+                and a.is_contiguous() and b.is_contiguous() and c.is_contiguous()
+                and d.is_contiguous() and e.is_contiguous() and f.is_contiguous()
+                and a.get_device() == b.get_device() == c.get_device() == d.get_device()
+                == e.get_device() == f.get_device() == index):
+            raise ValueError(f"page table outputs must be contiguous int32 of {batch}, 1, "
+                             f"{batch + 1}, {tokens}, {tokens} and 1 numbers on the inputs' "
+                             "device")
         if batch and step.lengths.data_ptr() == lengths.data_ptr():
             raise ValueError("the new lengths cannot be written over the old")
         if step.free_count.data_ptr() == free_count.data_ptr():
@@ -236,7 +244,7 @@ def _cache(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: torch
         raise TypeError("cache codes are float8_e4m3fn and scales float32")
     if page_tokens not in PAGE_TOKENS:
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
-    if padded != cache_width(width):
+    if padded != _PADDED.get(width):
         raise ValueError(f"a cache for heads of {width} is {cache_width(width)} wide")
     if not (key_pages.is_contiguous() and key_scales.is_contiguous()
             and value_pages.is_contiguous() and value_scales.is_contiguous()):
@@ -279,8 +287,9 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
         raise ValueError("cache and keys differ in heads")
     if tokens == 0:
         return
-    key, k, (k_row, k_head, _) = _rows(key)
-    value, v, (v_row, v_head, _) = _rows(value)
+    step = 8 if code else 4
+    key, k, (k_row, k_head, _) = _rows(key, step)
+    value, v, (v_row, v_head, _) = _rows(value, step)
     rc = nat.lib().cowsdm_kv_write(cache, k, k_row, k_head, v, v_row, v_head, code, width,
                                    slots.data_ptr(), tokens, nat.stream_handle(key.device))
     if rc:
@@ -330,11 +339,12 @@ def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: t
     if longest < 0:
         raise ValueError("the longest length cannot be negative")
     factor = _scale(scale, width)
-    out = torch.empty((batch, tokens, heads, width), device=device, dtype=query.dtype)
+    out = query.new_empty((batch, tokens, heads, width))
     if not batch or not tokens:
         return out
-    query, q_at, (q_request, q_token, q_head, _) = _rows(query)
-    need = cached_workspace_bytes(batch, tokens, heads, cache.heads, width, longest)
+    query, q_at, (q_request, q_token, q_head, _) = _rows(query, 8 if code else 4)
+    need = nat.lib().cowsdm_cached_attention_workspace_bytes(batch, tokens, heads, cache.heads,
+                                                             cache.width, longest)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     q = nat.CachedQuery(
         q_at, q_request, q_token, q_head, page_tables.data_ptr(), lengths.data_ptr(),

@@ -98,10 +98,10 @@ def test_cache_checks():
 def test_rows_are_copied_only_where_they_cannot_be_loaded():
     x = torch.zeros(6, 8, 64, dtype=torch.bfloat16)
     for kept in (x, x[:, 2:4], x.transpose(0, 1), x[..., 8:24]):
-        tensor, address, strides = attention._rows(kept)
+        tensor, address, strides = attention._rows(kept, 8)
         assert tensor is kept and address == kept.data_ptr() and strides == kept.stride()
     for copied in (x[..., 1:9], x[..., ::2], torch.zeros(6, 8, 65)[..., :64]):
-        tensor, address, strides = attention._rows(copied)
+        tensor, address, strides = attention._rows(copied, 8)
         assert address == tensor.data_ptr() != copied.data_ptr() and tensor.is_contiguous()
         assert strides == tensor.stride() and torch.equal(tensor, copied)
 
