@@ -559,23 +559,29 @@ constexpr int float_keys(int padded) { return padded <= 64 ? 64 : padded <= 128 
 // pass registers while this one is used.  4 prompts of 2,048 tokens, 8 heads
 // over 2, width 128: 365 us, 94 TFLOP/s of the 140 that a library's float32
 // product reaches; 4 of 128, 4 heads of 32: 8 us, two tiles' round trips.
-template <int DP>
-__global__ __launch_bounds__(kPromptThreads, DP <= 64 ? 3 : 2) void prompt_float_kernel(
+//
+// KP = 2: 32 rows, of which two waves share 16; one takes the even and one the
+// odd tiles, as in the 16-bit kernel.
+template <int DP, int KP>
+__global__ __launch_bounds__(kPromptThreads, DP <= 64 && KP == 1 ? 3 : 2) void prompt_float_kernel(
     PromptParams p) {
-  constexpr int kRows = kPromptWaves * 16;
+  constexpr int kSide = kPromptThreads / KP;           // threads that share a tile
+  constexpr int kRows = kSide / 4;
   constexpr int kKeys = float_keys(DP);
   constexpr int KT = kKeys / 16;
   constexpr int KS = DP / 16;
   constexpr int DT = DP / 16;
   constexpr int kStride = DP + 4;      // rows of four apart fall on other banks
-  constexpr int kLoads = kKeys * DP / 4 / kPromptThreads;
+  constexpr int kLoads = kKeys * DP / 4 / kSide;
   extern __shared__ __attribute__((aligned(16))) char s_tiles[];
-  float* const s_key = reinterpret_cast<float*>(s_tiles);
-  float* const s_value = s_key + kKeys * kStride;
-  const int tid = static_cast<int>(threadIdx.x);
-  const int lane = tid & (kWave - 1);
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int side = KP == 1 ? 0
+                           : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kSide);
+  const int tid = static_cast<int>(threadIdx.x) - side * kSide;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane & 15, quarter = lane >> 4;
+  float* const s_key = reinterpret_cast<float*>(s_tiles) + side * 2 * kKeys * kStride;
+  float* const s_value = s_key + kKeys * kStride;
   const PromptWork w = prompt_work(p);
   zero_rows<float>(p, w);
   int begin, length;
@@ -595,7 +601,7 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 64 ? 3 : 2) void prompt_float
     auto fetch = [&](int k0) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int at = i * kPromptThreads + tid;
+        const int at = i * kSide + tid;
         const int r = k0 + at / (DP / 4), c = at % (DP / 4) * 4;
         const bool inside = r < length && c < p.width;
         const int64_t from = inside ? r : 0;
@@ -624,19 +630,21 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 64 ? 3 : 2) void prompt_float
       for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       most = kMinusInf;
       sum = 0.0f;
-      fetch(0);
-      for (int k0 = 0; k0 < seen; k0 += kKeys) {
+      fetch(side * kKeys);
+      // a turn takes KP tiles, one for each side
+      for (int first = 0; first < seen; first += KP * kKeys) {
+        const int k0 = first + side * kKeys;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int at = i * kPromptThreads + tid;
+          const int at = i * kSide + tid;
           const int to = at / (DP / 4) * kStride + at % (DP / 4) * 4;
           *reinterpret_cast<f32x4*>(s_key + to) = next_key[i];
           *reinterpret_cast<f32x4*>(s_value + to) = next_value[i];
         }
         __syncthreads();
-        if (k0 + kKeys < seen) fetch(k0 + kKeys);
-        if (k0 > q0 + 15 || q0 >= length) continue;
+        if (k0 + KP * kKeys < seen) fetch(k0 + KP * kKeys);
+        if (k0 >= seen || k0 > q0 + 15 || q0 >= length) continue;
         f32x4 s[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -715,7 +723,32 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 64 ? 3 : 2) void prompt_float
 #pragma unroll
       for (int i = 0; i < 4; ++i) nan |= acc[d][i] != acc[d][i];
     if (__syncthreads_or(nan)) run(std::true_type());
-    const float inverse = 1.0f / sum_over_rows(sum);
+    sum = sum_over_rows(sum);
+    if constexpr (KP == 2) {
+      float* const given = reinterpret_cast<float*>(s_tiles) + wave * (DT * 4 + 2) * kWave + lane;
+      __syncthreads();          // the last tiles are used
+      if (side == 1) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) given[(d * 4 + i) * kWave] = acc[d][i];
+        given[DT * 4 * kWave] = most;
+        given[(DT * 4 + 1) * kWave] = sum;
+      }
+      __syncthreads();
+      if (side == 1) continue;
+      const float other = given[DT * 4 * kWave], now = fmaxf(most, other);
+      const float mine = most == kMinusInf ? 0.0f : exp2_fast(most - now);
+      const float theirs = other == kMinusInf ? 0.0f : exp2_fast(other - now);
+      // a row whose logits are all -inf stays 0 / 0
+      sum = sum * mine + given[(DT * 4 + 1) * kWave] * theirs;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[d][i] = acc[d][i] * mine + given[(d * 4 + i) * kWave] * theirs;
+    }
+    const float inverse = 1.0f / sum;
     if (row < length) {
       float* const out = static_cast<float*>(p.out) +
                          ((static_cast<int64_t>(begin) + row) * p.heads + w.head) * p.width;
@@ -750,8 +783,18 @@ int32_t launch_prompt_kernel(void (*kernel)(PromptParams), int bytes, int rows, 
 template <int DP>
 int32_t launch_prompt_float(const PromptParams& p, int64_t longest, hipStream_t stream) {
   constexpr int kBytes = 2 * float_keys(DP) * (DP + 4) * 4;
-  return launch_prompt_kernel(&prompt_float_kernel<DP>, kBytes, kPromptWaves * 16, longest, p,
-                              stream);
+  if constexpr (DP < 256) {      // whose registers would not hold another tile
+    // Where 64 rows a workgroup leave a CU about one: 4 heads of 4,096 tokens
+    // at width 32 take 81 us by 32 rows and 123 by 64, 8 heads of 1,000 at
+    // width 64 40 and 56; with more workgroups the halves are in each other's
+    // way (8 heads of 12 prompts of up to 465: 68 and 64), and short rows lose
+    // by the join (4 prompts of 128: 11.0 and 10.1).
+    const int64_t most = (static_cast<int64_t>(p.rows) / 64 + p.sequences) * p.heads;
+    if (most <= 288 && longest >= 4 * float_keys(DP))
+      return launch_prompt_kernel(&prompt_float_kernel<DP, 2>, 2 * kBytes, 32, longest, p,
+                                  stream);
+  }
+  return launch_prompt_kernel(&prompt_float_kernel<DP, 1>, kBytes, 64, longest, p, stream);
 }
 
 template <typename T, int DP>

@@ -168,3 +168,39 @@ def test_repeats_are_the_same_bits(device):
     q, k, v, offsets = packed([257, 600, 64], 8, 8, 64, torch.float16, 14, device)
     first = cow.prompt_attention(q, k, v, offsets)
     assert all(torch.equal(cow.prompt_attention(q, k, v, offsets), first) for _ in range(3))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [32, 96, 128])
+def test_few_rows_of_many_keys(device, dtype, width):
+    """Grids that leave the chip empty, where two waves share a row's keys:
+    lengths whose last turn is one tile, two, or ends inside either, values
+    that are not finite, and the same rows of a larger grid."""
+
+    for length in (512, 577, 640, 705):
+        print(f"few rows {length} width {width} {dtype}", flush=True)
+        q, k, v, offsets = packed([length, 3], 1, 1, width, dtype, length, device)
+        check(q, k, v, offsets, cow.prompt_attention(q, k, v, offsets, longest=length))
+    v[300, 0, 1], v[650, 0, 2], v[651, 0, 2] = float("nan"), float("inf"), float("-inf")
+    check(q, k, v, offsets, cow.prompt_attention(q, k, v, offsets, longest=705))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_workgroups(device, dtype):
+    """More than four rounds of workgroups, whose order is another, and heads
+    over eight, five and one key heads."""
+
+    for heads, kv_heads in ((16, 8), (20, 5), (16, 1)):
+        print(f"many workgroups {heads} over {kv_heads} {dtype}", flush=True)
+        q, k, v, offsets = packed([130, 1, 0] * 60, heads, kv_heads, 8, dtype, heads, device)
+        got = cow.prompt_attention(q, k, v, offsets, longest=130)
+        some = slice(0, 131 * 2)
+        out, weight, logit = ref.prompt(wide(q[some]), wide(k[some]), wide(v[some]),
+                                        offsets[:7].tolist())
+        assert_within(got[some], out, weight, logit, longest=130, values=wide(v))
+        # the other sequences of 130 rows alone
+        for at in (5, 59):
+            rows = slice(131 * at, 131 * at + 130)
+            alone = torch.tensor([0, 130], dtype=torch.int32, device=device)
+            one = cow.prompt_attention(q[rows], k[rows], v[rows], alone)
+            assert torch.equal(got[rows], one)
