@@ -994,16 +994,24 @@ void launch_cached_width(int64_t padded, const CachedParams& p, hipStream_t stre
   }
 }
 
-constexpr int64_t kCachedWorkgroups = 256;      // one a CU
+// Workgroups that fill the chip: one a CU, two of the narrowest rows, whose
+// registers allow it (10 requests of 65,485 tokens, 7 query tokens, width 32:
+// 19 us with two and 25 with one; at width 128 12 of 16,167 take 38 and 29).
+constexpr int64_t cached_workgroups(int64_t padded) { return padded <= 32 ? 512 : 256; }
 
 // The splits of the cache that a call's launch makes: enough workgroups to
-// fill the chip, none with less than two blocks a wave.
+// fill the chip, none with less than two blocks a wave; and none at all up to
+// 2,048 tokens of 131,072 elements of a key head's rows together, for which
+// the second launch of a join costs more than the splits give (8 requests of
+// 2,048 tokens at width 64: 11 us, 16 in two splits; 4 of 1,500 at width 128,
+// past that bound, measure 16 either way).
 int64_t cached_splits(int64_t requests, int64_t kv_heads, int64_t row_tiles, int64_t padded,
                       int64_t longest) {
+  if (longest <= 2048 && longest * padded <= 131072) return 1;
   const int64_t least = 2 * cached_waves(padded) * kCachedTokens;
   const int64_t rows = requests * kv_heads * row_tiles;
   const int64_t most = (longest + least - 1) / least;
-  int64_t splits = rows > 0 ? (kCachedWorkgroups + rows - 1) / rows : 1;
+  int64_t splits = rows > 0 ? (cached_workgroups(padded) + rows - 1) / rows : 1;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits;
 }
@@ -1212,7 +1220,7 @@ extern "C" int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
   p.chunk = p.splits == 1 ? INT32_MAX / 2
                           : static_cast<int32_t>((each + kBlock - 1) / kBlock * kBlock);
   p.by_length = q.requests > 1 && q.requests <= kWave && p.splits == 1 &&
-                q.requests * cache->heads * tiles > kCachedWorkgroups &&
+                q.requests * cache->heads * tiles > cached_workgroups(cache->width) &&
                 q.columns * cache->page_tokens < (1 << 24);
   if (p.splits > 1) {
     const int64_t need = cowsdm_cached_attention_workspace_bytes(
