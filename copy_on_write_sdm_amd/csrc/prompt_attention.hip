@@ -403,6 +403,7 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
     PromptParams p) {
   using Rows = PromptRows<T, DP>;
   using vec = typename Half<T>::vec;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
   constexpr int KS = Rows::KS, DT = Rows::DT;
   constexpr int kSide = kPromptThreads / KP;           // threads that share a tile
   constexpr int kRows = kSide / 2;
@@ -520,6 +521,7 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
       rows.clear();
       load_turn(0, 0);
       edges(std::integral_constant<PromptTile, PromptTile::kCareful>(), 0);
+      if constexpr (KP == 1) __syncthreads();        // the last tiles are used
     }
     if constexpr (KP == 2) {
       using lds_float = typename Rows::lds_float;
@@ -533,19 +535,34 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(rows.sum),
                                                     __float_as_uint(rows.sum), false, false);
     const float inverse = 1.0f / (__uint_as_float(x[0]) + __uint_as_float(x[1]));
-    const int row = q0 + col;
-    if (row >= length) continue;
-    T* const out = static_cast<T*>(p.out) +
-                   ((static_cast<int64_t>(begin) + row) * p.heads + w.head) * p.width;
+    // The rows go out through LDS: as they are, a store would write 16 bytes
+    // of each of 32 rows; so, it writes whole rows.
+    // Its addresses are kept from being worked out before the loop, whose
+    // registers they would take.
+    int own = lane;
+    asm volatile("" : "+v"(own));
+    lds_char* const turned =
+        (lds_char*)s_tiles + wave * (KP == 1 ? 32 * DP * 2 : Rows::kFloats * 4);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int at = d * 32 + i * 8 + half * 4;
         const f32x16& a = rows.acc[d];
-        if (at < p.width)
-          store4(out + at, f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]} * inverse);
+        const f32x4 x = f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]} * inverse;
+        *reinterpret_cast<__attribute__((address_space(3))) vec4*>(
+            turned + own % 32 * DP * 2 + place<DP>(own % 32, d * 4 + i) * 16 + own / 32 * 8) =
+            __builtin_convertvector(x, vec4);
       }
+    T* const out = static_cast<T*>(p.out) +
+                   ((static_cast<int64_t>(begin) + q0) * p.heads + w.head) * p.width;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const int at = i * kWave + own, row = at / (DP / 8), c = at % (DP / 8);
+      const vec x = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(
+          turned + row * DP * 2 + place<DP>(row, c) * 16);
+      if (q0 + row < length && c * 8 < p.width)
+        *reinterpret_cast<vec*>(out + static_cast<int64_t>(row) * p.heads * p.width + c * 8) = x;
+    }
   }
 }
 
