@@ -390,14 +390,15 @@ struct PromptRows {
 // one the odd tiles, and their sums are joined at the end.  That is for grids
 // that leave CUs empty, where the longest row's way through its keys counts.
 //
-// Two prompts of 8,192 tokens, 32 heads over 8, width 128, bfloat16: 1,020 us,
-// 1,078 TFLOP/s of what causality leaves (a library's product of two 8,192
+// Two prompts of 8,192 tokens, 32 heads over 8, width 128, bfloat16: 975 us,
+// 1,128 TFLOP/s of what causality leaves (a library's product of two 8,192
 // square matrices reaches 1,238 on the same card).  The matrix cores are busy
-// 54 % of the cycles and the vector units, whose exponentials, maxima, sums
-// and roundings are as long a chain, about 60 %, at the 1.9 GHz that such a
-// load runs at; waits are 16 %, LDS a quarter busy without conflicts, L2 hits
-// 95 %.  24 packed prompts of up to 2,048 take 324 us, 690 TFLOP/s: a fifth of
-// their tiles lie on the diagonal.
+// 60 % of the cycles and the vector units, whose exponentials, maxima, sums
+// and roundings are as long a chain, about as much, at the 1.9 GHz that such a
+// load runs at; waits are 16 %, LDS a quarter busy, L2 hits 95 %.  24 packed
+// prompts of up to 2,048 take 308 us, 723 TFLOP/s: a fifth of their tiles lie
+// on the diagonal, and a workgroup starts and ends, with 64 KB from and to
+// memory, around nine tiles (2 us each beside another workgroup, and 6 us).
 template <typename T, int DP, int KP>
 __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half_kernel(
     PromptParams p) {
@@ -536,7 +537,8 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
                                                     __float_as_uint(rows.sum), false, false);
     const float inverse = 1.0f / (__uint_as_float(x[0]) + __uint_as_float(x[1]));
     // The rows go out through LDS: as they are, a store would write 16 bytes
-    // of each of 32 rows; so, it writes whole rows.
+    // of each of 32 rows; so, it writes whole rows (24 packed prompts 308 us,
+    // 325 without).
     // Its addresses are kept from being worked out before the loop, whose
     // registers they would take.
     int own = lane;
