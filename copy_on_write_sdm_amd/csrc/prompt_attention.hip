@@ -820,16 +820,20 @@ template <typename T, int DP>
 int32_t launch_prompt_half(const PromptParams& p, int64_t longest, hipStream_t stream) {
   constexpr int kTiles = 2 * 2 * kTileKeys * DP * 2;
   if constexpr (DP <= 128) {
-    // Where 64 rows a workgroup leave the chip's 256 CUs no second one: 8 heads
-    // of 1,000 tokens at width 128 take 18 us so and 24 us by 128 rows.  Short
-    // rows lose by the join (4 prompts of 100: 11.6 against 10.4), and more
-    // workgroups by their tiles' traffic (16 heads of 4,096: 127 against 119).
+    // Where the chip holds all workgroups of 64 rows at once, by the LDS they
+    // take: 8 heads of 1,000 tokens at width 128 take 18 us so and 24 us by 128
+    // rows, 8 of 4,096 at width 64 34 and 50, 8 of 8,192 at width 32 69 and 89.
+    // Short rows lose by the join, the more so as the chip is full (4 prompts
+    // of 100: 11.6 against 10.4; 2 of 550, 32 heads of 64: 14.6 against 11.9;
+    // 8 of 600, 8 heads: 10.8 against 12.3), and more workgroups by their
+    // tiles' traffic (4 of 1,024, 12 heads of 64: 21 against 18; 16 heads of
+    // 4,096 at width 128: 127 against 119).
     const int64_t most = (static_cast<int64_t>(p.rows) / 64 + p.sequences) * p.heads;
     constexpr int kJoin = 2 * PromptRows<T, DP>::kFloats * 4;
-    if (most <= 256 && longest >= 512)
-      return launch_prompt_kernel(&prompt_half_kernel<T, DP, 2>,
-                                  2 * kTiles > kJoin ? 2 * kTiles : kJoin, 64, longest, p,
-                                  stream);
+    constexpr int kBytes = 2 * kTiles > kJoin ? 2 * kTiles : kJoin;
+    constexpr int kHeld = 160 * 1024 / kBytes < 4 ? 160 * 1024 / kBytes : 4;   // by a CU
+    if (most <= (longest >= 1000 ? 288 : 192) * kHeld && longest >= 512)
+      return launch_prompt_kernel(&prompt_half_kernel<T, DP, 2>, kBytes, 64, longest, p, stream);
   }
   return launch_prompt_kernel(&prompt_half_kernel<T, DP, 1>, kTiles, 128, longest, p, stream);
 }
