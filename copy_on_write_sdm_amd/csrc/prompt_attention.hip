@@ -805,11 +805,14 @@ int32_t launch_prompt_float(const PromptParams& p, int64_t longest, hipStream_t 
   if constexpr (DP < 256) {      // whose registers would not hold another tile
     // Where 64 rows a workgroup leave a CU about one: 4 heads of 4,096 tokens
     // at width 32 take 81 us by 32 rows and 123 by 64, 8 heads of 1,000 at
-    // width 64 40 and 56; with more workgroups the halves are in each other's
-    // way (8 heads of 12 prompts of up to 465: 68 and 64), and short rows lose
-    // by the join (4 prompts of 128: 11.0 and 10.1).
+    // width 64 40 and 56; or two of the narrowest, whose registers allow twice
+    // as many (4 heads of 8,192: 211 and 288).  With more workgroups the
+    // halves are in each other's way (8 heads of 12 prompts of up to 465: 68
+    // and 64), and short rows lose by the join (4 prompts of 128: 11.0 and
+    // 10.1; 8 of 256, 14 heads of 32: 17 and 14).
     const int64_t most = (static_cast<int64_t>(p.rows) / 64 + p.sequences) * p.heads;
-    if (most <= 288 && longest >= 4 * float_keys(DP))
+    if ((most <= 288 && longest >= 4 * float_keys(DP)) ||
+        (DP <= 32 && most <= 576 && longest >= 512))
       return launch_prompt_kernel(&prompt_float_kernel<DP, 2>, 2 * kBytes, 32, longest, p,
                                   stream);
   }
