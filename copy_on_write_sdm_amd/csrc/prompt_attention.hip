@@ -388,7 +388,8 @@ struct PromptRows {
 // without passing registers; the next tile is on its way while this one is
 // used.  KP = 2: 64 rows, of which two waves share 32; one takes the even and
 // one the odd tiles, and their sums are joined at the end.  That is for grids
-// that leave CUs empty, where the longest row's way through its keys counts.
+// that the chip holds at once, where the longest row's way through its keys
+// counts.
 //
 // Two prompts of 8,192 tokens, 32 heads over 8, width 128, bfloat16: 975 to
 // 990 us, 1,110 to 1,128 TFLOP/s of what causality leaves (a library's
@@ -396,9 +397,10 @@ struct PromptRows {
 // matrix cores are busy 60 % of the cycles and the vector units, whose
 // exponentials, maxima, sums and roundings are as long a chain, about as much,
 // at the 1.9 GHz that such a load runs at; waits are 16 %, LDS a quarter busy,
-// L2 hits 95 %.  24 packed prompts of up to 2,048 take 308 us, 723 TFLOP/s: a fifth of their tiles lie
-// on the diagonal, and a workgroup starts and ends, with 64 KB from and to
-// memory, around nine tiles (2 us each beside another workgroup, and 6 us).
+// L2 hits 95 %.  24 packed prompts of up to 2,048 take 308 us, 723 TFLOP/s: a
+// fifth of their tiles lie on the diagonal, and a workgroup starts and ends,
+// with 64 KB from and to memory, around nine tiles (2 us each beside another
+// workgroup, and 6 us).
 template <typename T, int DP, int KP>
 __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half_kernel(
     PromptParams p) {
