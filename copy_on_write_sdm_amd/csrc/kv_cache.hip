@@ -606,6 +606,7 @@ __device__ __forceinline__ int cached_length(const CachedParams& p, int request)
 template <int DP, typename T, int NW>
 __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedParams p) {
   constexpr int N = AttentionType<T>::kParts;
+  constexpr int NP = AttentionType<T>::kProbParts;
   constexpr int KB = DP / 4;            // a lane's bytes of a key row
   constexpr int KS = DP / 32;           // products along the width
   constexpr int DT = DP / 16;           // tiles of the output's width
@@ -766,13 +767,13 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
         pr[4 * t + i] = e;
         sum += e;
       }
-    bf16x8 prob[2][N];
+    bf16x8 prob[2][NP];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = pr[8 * h + j];
-      split_bf16<N>(x, prob[h]);
+      split_bf16<NP>(x, prob[h]);
     }
     uint32_t poisoned = 0;
     if (masked && p.tokens > 1) {
@@ -817,7 +818,7 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
       for (int h = 0; h < 2; ++h) {
         const bf16x8 a = widen_codes(vw[d][2 * h], vw[d][2 * h + 1], vs);
 #pragma unroll
-        for (int n = N - 1; n >= 0; --n)
+        for (int n = NP - 1; n >= 0; --n)
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, prob[h][n], acc[d], 0, 0, 0);
       }
     }
