@@ -708,7 +708,8 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
   float most = kMinusInf, sum = 0.0f;     // of logits times scale
   auto use = [&](Fetched<DP>& f) {
     const int base = f.base, v_page = f.v_page, v_at = base + row * 16;
-    const float ks = f.ks, vs = f.vs;
+    const float ks = f.ks;
+    float vs = f.vs;
     auto& kw = f.kw;
     auto& vw = f.vw;
     f32x4 s[4];
@@ -733,8 +734,10 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (v_page < 0 || v_at + 4 * t + i > last) s[t][i] = kMinusInf;
-      // codes of tokens past the length are whatever the page held before
+      // codes of tokens past the length are whatever the page held before;
+      // where there is no page, the scale is one that nobody may have written
       const int keep = v_page < 0 ? 0 : length - v_at;
+      if (v_page < 0) vs = 1.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = keep - 4 * i;
