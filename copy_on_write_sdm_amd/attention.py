@@ -312,8 +312,9 @@ def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: t
     """Attention of each request's newest tokens over one layer's cache: query
     [B, n, heads, D] holds the last n of its ``lengths`` [B] tokens (written
     before), and row i sees positions 0 to length - n + i.  Grouped heads as
-    in ``prompt_attention``.  Returns [B, n, heads, D] in the query's type; a
-    row that sees nothing is zero.  ``longest`` bounds the lengths (the
+    in ``prompt_attention``.  Returns [B, n, heads, D] in the query's type.
+    Tokens whose table entry is no page of the pool are left out, and a row
+    that sees nothing is zero.  ``longest`` bounds the lengths (the
     tables' columns when not given): a bound that is too small costs time, not
     correctness."""
 

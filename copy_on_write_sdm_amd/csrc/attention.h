@@ -17,6 +17,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kMinusInf = -__builtin_huge_valf();
+constexpr float kLeastFloat = -3.402823466e38f;   // the lowest finite number
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kMostCode = 448.0f;         // the largest e4m3 number
 

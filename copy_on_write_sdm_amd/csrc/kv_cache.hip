@@ -728,7 +728,11 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
     // where a page is missing
     const bool tail = base + kCachedTokens > length - p.tokens + 1;
     const bool masked = tail || __any(v_page < 0);
+    // a row that sees a token has a finite maximum, were its logits all -inf;
+    // one that has seen none keeps -inf, and gives 0
+    float least = kLeastFloat;
     if (masked) {
+      least = v_page < 0 || v_at > last ? kMinusInf : kLeastFloat;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -751,7 +755,7 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
-    top = max_over_rows(top) * p.scale;
+    top = max_over_rows(fmaxf(top * p.scale, least));
     if (__any(top > most)) {
       const float now = fmaxf(most, top);
       const float keep = now == kMinusInf ? 1.0f : exp2_fast(most - now);
@@ -904,7 +908,7 @@ __global__ __launch_bounds__(NW * kWave) void cached_attention_kernel(CachedPara
   for (int d = 0; d < DT; ++d) {
     const int at = d * 16 + row * 4;
     if (at < p.width)
-      store4(out + at, last < 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[d] * inverse);
+      store4(out + at, most == kMinusInf ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[d] * inverse);
   }
 }
 
@@ -929,9 +933,8 @@ __global__ __launch_bounds__(kJoinThreads) void cached_join_kernel(CachedParams 
   const int length = cached_length(p, request);
   T* const out = static_cast<T*>(p.out) +
                  ((static_cast<int64_t>(request) * p.tokens + token) * p.heads + head) * p.width;
-  const bool none = length - p.tokens + token < 0;
   const int chunks = (length + p.chunk - 1) / p.chunk;
-  const int used = none ? 0 : chunks < p.splits ? chunks : p.splits;
+  const int used = length - p.tokens + token < 0 ? 0 : chunks < p.splits ? chunks : p.splits;
   const float* const parts =
       p.parts + ((static_cast<int64_t>(request) * p.kv_heads + kv) * p.row_tiles + tile) *
                     p.splits * kPartFloats<DP>;
@@ -968,7 +971,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_join_kernel(CachedParams 
     acc += *reinterpret_cast<const f32x4*>(&s_sum[g][at]);
     sum += s_sum[g][DP];
   }
-  store4(out + at, none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / sum));
+  store4(out + at, most == kMinusInf ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / sum));
 }
 
 // The waves of a workgroup: eight where the registers of the widths allow two

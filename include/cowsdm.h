@@ -872,8 +872,9 @@ int32_t cowsdm_kv_write(const cowsdm_kv_cache_t* cache, const void* key, int64_t
                         const int32_t* slots, int64_t tokens, void* stream);
 
 /* The newest `tokens` tokens of each request over the cache: query row i of
- * request r sees positions 0 .. lengths[r] - tokens + i.  A row that sees
- * nothing gives 0.  `longest` is the longest length, or more; a smaller value
+ * request r sees positions 0 .. lengths[r] - tokens + i, but for those whose
+ * table entry is no page of the pool.  A row that sees nothing gives 0.
+ * `longest` is the longest length, or more; a smaller value
  * costs time, not correctness. */
 typedef struct cowsdm_cached_query {
   const void* query;               /* [requests, tokens, heads, width]     */
