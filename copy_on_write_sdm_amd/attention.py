@@ -106,8 +106,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     rows offsets[s] to offsets[s + 1] - 1.  Returns [T, heads, D] in the
     query's type; rows of no sequence are zero.  ``longest`` bounds the
     sequences' lengths (T when not given) and sizes the launch: a bound that
-    is too small costs time, not correctness.  ``scale`` defaults to
-    D ** -0.5."""
+    is too small or too large costs time, not correctness.  ``scale`` defaults
+    to D ** -0.5."""
 
     if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
         raise ValueError("attention takes query [T,heads,D] and key and value [T,kv_heads,D]")

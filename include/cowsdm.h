@@ -815,7 +815,8 @@ typedef struct cowsdm_prompt_attention {
   float scale;                     /* positive                             */
 } cowsdm_prompt_attention_t;
 
-/* Runs cowsdm_prompt_attention_t; COWSDM_ELIMIT for a width over 256. */
+/* Runs cowsdm_prompt_attention_t; COWSDM_ELIMIT for a width over 256, or for
+ * 2^24 pairs of a head and a sequence or more. */
 int32_t cowsdm_prompt_attention(const cowsdm_prompt_attention_t* attention, void* stream);
 
 /* A step's page tables and token slots.  Request r holds lengths[r] tokens in

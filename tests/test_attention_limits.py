@@ -1,0 +1,18 @@
+"""Limits of the attention entries, refused before any launch: no GPU needed."""
+
+from __future__ import annotations
+
+from copy_on_write_sdm_amd import _native as nat
+
+
+def test_prompts_of_more_pairs_than_a_launch_holds():
+    """A launch counts its threads in 32 bits: 2^24 workgroups of 256 are too
+    many, however short the sequences."""
+
+    lib = nat.lib()
+    fake = 0x1000           # never dereferenced: the call fails first
+    for heads, sequences in ((1 << 12, 1 << 12), (1 << 20, 1 << 30), (1, 1 << 24)):
+        a = nat.PromptAttention(fake, fake, fake, 64, 64, 64, 64, 64, 64, fake, fake, 4,
+                                sequences, 1, heads, 1, 64, 0, 0.1)
+        assert lib.cowsdm_prompt_attention(a, None) == -2
+        assert b"pairs" in lib.cowsdm_last_error_string()
