@@ -36,6 +36,7 @@ from . import _native as nat
 CODES = torch.float8_e4m3fn
 _INT32, _FLOAT32 = torch.int32, torch.float32
 MAX_REQUESTS = 4_096
+_FAR = 1 << 23        # elements between rows from which prompts are copied
 PAGE_TOKENS = (16, 32, 64, 128, 256)
 CACHE_WIDTHS = (32, 64, 96, 128, 192, 256)
 
@@ -72,16 +73,17 @@ def _scale(scale: float | None, width: int) -> float:
     return scale
 
 
-def _rows(tensor: torch.Tensor, step: int) -> tuple[torch.Tensor, int, tuple[int, ...]]:
+def _rows(tensor: torch.Tensor, step: int, far: float = math.inf
+          ) -> tuple[torch.Tensor, int, tuple[int, ...]]:
     """``tensor``, its address and its strides where its rows can be loaded 16
     bytes (``step`` elements) at a time, as a slice of a fused projection can,
-    else those of a contiguous copy."""
+    and lie less than ``far`` elements apart; else those of a contiguous copy."""
 
     strides, address = tensor.stride(), tensor.data_ptr()
     together = 0
     for s in strides[:-1]:
         together |= s
-    if strides[-1] == 1 and not together % step and not address % 16:
+    if strides[-1] == 1 and not together % step and not address % 16 and strides[0] < far:
         return tensor, address, strides
     copy = tensor.contiguous()
     if copy.data_ptr() % 16:        # contiguous as it was, only its address is odd
@@ -141,9 +143,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if not rows:
         return out
     step = 8 if code else 4
-    query, q, (q_row, q_head, _) = _rows(query, step)
-    key, k, (k_row, k_head, _) = _rows(key, step)
-    value, v, (v_row, v_head, _) = _rows(value, step)
+    query, q, (q_row, q_head, _) = _rows(query, step, _FAR)
+    key, k, (k_row, k_head, _) = _rows(key, step, _FAR)
+    value, v, (v_row, v_head, _) = _rows(value, step, _FAR)
     a = nat.PromptAttention(q, k, v, q_row, q_head, k_row, k_head, v_row, v_head,
                             offsets.data_ptr(), out.data_ptr(), rows, sequences, longest, heads,
                             kv_heads, width, code, factor)
