@@ -88,7 +88,12 @@ def _rows(tensor: torch.Tensor, step: int, far: float = math.inf
     copy = tensor.contiguous()
     if copy.data_ptr() % 16:        # contiguous as it was, only its address is odd
         copy = copy.clone()
-    return copy, copy.data_ptr(), copy.stride()
+    # of its sizes, not its own: a tensor is contiguous whatever the strides of
+    # its axes of one element
+    strides = [1]
+    for size in reversed(copy.shape[1:]):
+        strides.append(strides[-1] * size)
+    return copy, copy.data_ptr(), tuple(reversed(strides))
 
 
 def _int32(tensor: torch.Tensor, numbers: int, device: int, what: str) -> None:

@@ -2,7 +2,10 @@
 
 from __future__ import annotations
 
+import torch
+
 from copy_on_write_sdm_amd import _native as nat
+from copy_on_write_sdm_amd import attention
 
 
 def test_prompts_of_more_pairs_than_a_launch_holds():
@@ -16,3 +19,12 @@ def test_prompts_of_more_pairs_than_a_launch_holds():
                                 sequences, 1, heads, 1, 64, 0, 0.1)
         assert lib.cowsdm_prompt_attention(a, None) == -2
         assert b"pairs" in lib.cowsdm_last_error_string()
+
+
+def test_strides_of_axes_of_one_element_say_nothing():
+    """torch calls a tensor contiguous whatever they are."""
+
+    for t in (torch.zeros(1, 1, 65)[..., :64], torch.zeros(1, 3, 1, 64)[..., ::2],
+              torch.zeros(70).as_strided((1, 1, 64), (1, 3, 1))):
+        _, _, strides = attention._rows(t, 4)
+        assert strides == torch.empty(t.shape).stride()

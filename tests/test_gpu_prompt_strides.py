@@ -27,3 +27,32 @@ def test_rows_far_apart(device, dtype):
         some[i] = far[i]
         assert torch.equal(cow.prompt_attention(*some, offsets), want)
     assert torch.equal(cow.prompt_attention(*far, offsets), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_row_with_any_stride(device, dtype):
+    """The strides of an axis of one element say nothing."""
+
+    q, k, v, offsets = packed([1], 1, 1, 40, dtype, 44, device)
+    want = cow.prompt_attention(q, k, v, offsets)
+    for stride in (41, 1, (1 << 23) + 8):
+        room = torch.zeros(1 << 24, dtype=dtype, device=device)
+        odd = [room[64 * i:].as_strided((1, 1, 40), (stride, stride, 1)).copy_(t)
+               for i, t in enumerate((q, k, v))]
+        assert torch.equal(cow.prompt_attention(*odd, offsets), want)
+        caches = []
+        for pair in ((k, v), odd[1:]):
+            cache = [torch.zeros(2, 1, 16, 64, dtype=torch.uint8, device=device),
+                     torch.ones(2, 1, device=device),
+                     torch.zeros(2, 1, 64, 16, dtype=torch.uint8, device=device),
+                     torch.ones(2, 1, device=device)]
+            caches.append([t.view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t
+                           for t in cache])
+            cow.write_kv_cache(*pair, torch.zeros(1, dtype=torch.int32, device=device),
+                               *caches[-1])
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+                   for a, b in zip(*caches))
+        table, one = torch.zeros(1, 1, dtype=torch.int32, device=device), torch.ones(
+            1, dtype=torch.int32, device=device)
+        assert torch.equal(cow.cached_attention(odd[0][None], *caches[0], table, one),
+                           cow.cached_attention(q[None], *caches[0], table, one))
