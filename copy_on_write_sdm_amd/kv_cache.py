@@ -11,6 +11,7 @@ are shared by the layers, whose requests are equally long.
 
 from __future__ import annotations
 
+from contextlib import contextmanager
 from typing import Callable, Sequence
 
 import torch
@@ -58,6 +59,7 @@ class PagedKVCache:
         self._lengths: list[int] = []
         self._released: set[int] = set()
         self._free = pages
+        self._before: tuple | None = None       # what the last extend may be taken back to
         self._added: dict[tuple[int, ...], torch.Tensor] = {}
 
     @property
@@ -94,19 +96,34 @@ class PagedKVCache:
         first = self.requests
         rows = torch.full((requests, self.page_tables.shape[1]), -1, dtype=torch.int32,
                           device=self.device)
-        self.page_tables = torch.cat((self.page_tables, rows))
-        self.lengths = torch.cat((self.lengths, self.lengths.new_zeros(requests)))
-        self._lengths += [0] * requests
+        tables = torch.cat((self.page_tables, rows))
+        lengths = torch.cat((self.lengths, self.lengths.new_zeros(requests)))
+        self.page_tables, self.lengths = tables, lengths
+        self._lengths = self._lengths + [0] * requests
+        self._before = None
         self._added.clear()
         return list(range(first, first + requests))
 
-    def _drop(self, requests: int) -> None:
-        """The rows after the first ``requests``, which hold nothing, go."""
+    def _now(self) -> tuple:
+        """What ``extend`` and ``admit`` replace, none of it in place: a table's
+        entries past the pages that its request holds are not read."""
 
-        self.page_tables = self.page_tables[:requests].clone()
-        self.lengths = self.lengths[:requests].clone()
-        del self._lengths[requests:]
+        return self.page_tables, self.lengths, self.free_count, self._lengths, self._free
+
+    def _back_to(self, before: tuple) -> None:
+        self.page_tables, self.lengths, self.free_count, self._lengths, self._free = before
+        self._before = None
         self._added.clear()
+
+    def take_back(self) -> None:
+        """Takes the last ``extend`` back, as long as no other change has
+        followed it: its pages are free again, and what ``write`` has put into
+        its slots lies past the lengths, where nothing reads.  (A page that it
+        went on in keeps a scale that those tokens raised.)"""
+
+        if self._before is None:
+            raise ValueError("there is no KV cache step to take back")
+        self._back_to(self._before)
 
     def extend(self, added: int | Sequence[int]) -> PageTableStep:
         """Pages for ``added`` more tokens of every request (one number for
@@ -133,6 +150,7 @@ class PagedKVCache:
         step = extend_page_tables(self.lengths, tensor, self.page_tables, self.free_pages,
                                   self.free_count, page_tokens=self.page_tokens,
                                   tokens=sum(counts))
+        self._before = self._now()
         self.lengths, self.free_count = step.lengths, step.free_count
         self._lengths, self._free = lengths, self._free - need
         return step
@@ -170,6 +188,7 @@ class PagedKVCache:
             self.free_pages.numel(), self.free_count.data_ptr(), self.page_tokens,
             nat.stream_handle(self.device)), "cowsdm_pages_release")
         freed = sum(self._pages(self._lengths[r]) for r in named)
+        self._before = None
         for r in named:
             self._lengths[r] = 0
         self._released |= set(named)
@@ -183,8 +202,9 @@ class PagedKVCache:
         kept = [r for r in range(self.requests) if r not in self._released]
         if self._released:
             index = torch.tensor(kept, dtype=torch.int64, device=self.device)
-            self.page_tables = self.page_tables.index_select(0, index)
-            self.lengths = self.lengths.index_select(0, index)
+            tables, lengths = (t.index_select(0, index) for t in (self.page_tables, self.lengths))
+            self.page_tables, self.lengths = tables, lengths
+            self._before = None
             self._lengths = [self._lengths[r] for r in kept]
             self._released = set()
             self._added.clear()
@@ -223,11 +243,20 @@ class PagedAttention:
     * ``finish(layer, tokens [T, width], mixed [T, heads, D])`` -> the block's
       residual stream [T, width] (output projection, residual add, MLP).
 
-    ``layers`` are the positions of the "A" layers in the layout.  A prefill
-    admits its requests after those that the cache holds, as
+    ``layers`` are the positions of the "A" layers in the layout, in the order
+    in which they run.  A prefill admits its requests after those that the cache holds, as
     ``FaithfulSDMDecodeState.admit`` appends them to the batch; ``release`` and
     ``compact`` of the cache go with the state's.  The state's own dense caches
-    of these layers hold no heads."""
+    of these layers hold no heads.
+
+    A step is a token, or a prompt, through all of these layers.  The stack's
+    prefill and decode open it before their first layer runs, so that one that
+    the cache has no room for changes nothing, and take it back when any layer
+    raises: the cache then stands where the decode state does, and the step can
+    be run again.  Called by itself, the first layer's call opens the step, a
+    layer that raises takes it back, and ``abort`` does so for what fails
+    between the layers.  What SDM layers have written before a failure is
+    theirs and stays."""
 
     def __init__(self, cache: PagedKVCache, layers: Sequence[int], project: Project,
                  finish: Finish, *, scale: float | None = None):
@@ -236,49 +265,135 @@ class PagedAttention:
             raise ValueError("the cache needs a layer for every attention layer")
         self.project, self.finish, self.scale = project, finish, scale
         self._step: PageTableStep | None = None
+        self._next = 0              # the layer of the step that runs next
+        self._prompt = False
+        self._before: tuple | None = None       # where the cache stood before the step
 
-    def _layer(self, layer: int) -> int:
+    # ------------------------------------------------------------- the steps
+
+    def _open(self, step: PageTableStep, prompt: bool) -> None:
+        self._step, self._next, self._prompt = step, 0, prompt
+        self._before = self.cache._before
+
+    def _unfinished(self) -> bool:
+        return self._step is not None and self._next < len(self.layers)
+
+    def _none_unfinished(self) -> None:
+        if self._unfinished():
+            raise ValueError(f"the last step has not run attention layer "
+                             f"{self.layers[self._next]}: abort() takes it back")
+
+    def _begin_prefill(self, batch: int, time: int) -> None:
+        self._none_unfinished()
+        cache, before = self.cache, self.cache._now()
+        try:
+            cache.admit(batch)
+            step = cache.extend([0] * len(before[3]) + [time] * batch)
+        except BaseException:
+            # no room: the cache is as it was
+            cache._back_to(before)
+            raise
+        cache._before = before
+        self._open(step, True)
+
+    def _begin_decode(self, batch: int, position: "int | Sequence[int] | torch.Tensor") -> None:
+        self._none_unfinished()
+        held = self.cache._lengths
+        if isinstance(position, int):
+            at = [position] * batch
+        else:
+            at = position.tolist() if isinstance(position, torch.Tensor) else list(position)
+        if at != held:
+            raise ValueError("decode positions do not match the KV cache")
+        self._open(self.cache.extend(1), False)
+
+    def abort(self) -> None:
+        """Takes the last step back, whichever of its layers have run; nothing
+        where there is none, or the cache has changed since."""
+
+        before, self._before, self._step = self._before, None, None
+        if before is not None and self.cache._before is before:
+            self.cache.take_back()
+
+    @contextmanager
+    def _whole_step(self, begin: Callable[..., None], *args):
+        begin(*args)
+        try:
+            yield
+            if self._unfinished():
+                raise ValueError(f"attention layer {self.layers[self._next]} is not in the layout")
+        except BaseException:
+            self.abort()
+            raise
+
+    def prefill_step(self, batch: int, time: int):
+        """A context that opens the step of a prompt and takes it back when its
+        body raises or leaves an attention layer out."""
+
+        return self._whole_step(self._begin_prefill, batch, time)
+
+    def decode_step(self, batch: int, position: "int | Sequence[int] | torch.Tensor"):
+        """The same of one token of every request, which stand at ``position``
+        (one for all, or one each)."""
+
+        return self._whole_step(self._begin_decode, batch, position)
+
+    def _enter(self, layer: int, prompt: bool, begin: Callable[..., None], *args
+               ) -> tuple[int, PageTableStep]:
+        """The layer's index and step, opened by its first layer if need be."""
+
         if layer not in self.layers:
             raise ValueError(f"layer {layer} is not one of the attention layers {self.layers}")
-        return self.layers.index(layer)
+        index = self.layers.index(layer)
+        if not self._unfinished() and index == 0:
+            begin(*args)
+        if not self._unfinished() or index != self._next or prompt is not self._prompt:
+            raise ValueError(f"attention layer {layer} is not the next of its step")
+        return index, self._step
+
+    # ------------------------------------------------------------ the layers
 
     def prefill(self, layer: int, tokens: torch.Tensor):
         """``attention_block``: tokens [B, T, width] of B new requests."""
 
-        index = self._layer(layer)
         batch, time, width = tokens.shape
-        if index == 0:
-            before = self.cache.requests
-            self.cache.admit(batch)
-            try:
-                self._step = self.cache.extend([0] * before + [time] * batch)
-            except ValueError:
-                # no room: the cache is as it was
-                self.cache._drop(before)
-                raise
-        step, rows = self._step, tokens.reshape(batch * time, width)
-        query, key, value = self.project(layer, rows, step.positions)
-        self.cache.write(index, key, value, step.slots)
-        mixed = prompt_attention(query, key, value, step.offsets, longest=time,
-                                 scale=self.scale)
-        out = self.finish(layer, rows, mixed).reshape(batch, time, width)
-        none = tokens.new_empty(batch, 0, time, self.cache.head_width)
+        index, step = self._enter(layer, True, self._begin_prefill, batch, time)
+        try:
+            rows = tokens.reshape(batch * time, width)
+            query, key, value = self.project(layer, rows, step.positions)
+            self.cache.write(index, key, value, step.slots)
+            mixed = prompt_attention(query, key, value, step.offsets, longest=time,
+                                     scale=self.scale)
+            out = self.finish(layer, rows, mixed).reshape(batch, time, width)
+            none = tokens.new_empty(batch, 0, time, self.cache.head_width)
+        except BaseException:
+            self.abort()
+            raise
+        self._next = index + 1
         return out, none, none
 
     def decode(self, layer: int, tokens: torch.Tensor, key_cache: torch.Tensor,
                value_cache: torch.Tensor, position: "int | torch.Tensor") -> torch.Tensor:
         """``attention_decode``: one more token [B, 1, width] of every request."""
 
-        index = self._layer(layer)
         batch, _, width = tokens.shape
-        if index == 0:
-            held = self.cache.request_lengths()
-            if len(held) != batch or (isinstance(position, int)
-                                      and any(n != position for n in held)):
-                raise ValueError("decode positions do not match the KV cache")
-            self._step = self.cache.extend(1)
-        step, rows = self._step, tokens.reshape(batch, width)
-        query, key, value = self.project(layer, rows, step.positions)
-        self.cache.write(index, key, value, step.slots)
-        mixed = self.cache.attend(index, query.unsqueeze(1), scale=self.scale)
-        return self.finish(layer, rows, mixed.squeeze(1)).reshape(batch, 1, width)
+        index, step = self._enter(layer, False, self._begin_decode, batch, position)
+        try:
+            rows = tokens.reshape(batch, width)
+            query, key, value = self.project(layer, rows, step.positions)
+            self.cache.write(index, key, value, step.slots)
+            mixed = self.cache.attend(index, query.unsqueeze(1), scale=self.scale)
+            out = self.finish(layer, rows, mixed.squeeze(1)).reshape(batch, 1, width)
+        except BaseException:
+            self.abort()
+            raise
+        self._next = index + 1
+        return out
+
+
+def paged_owner(attention) -> PagedAttention | None:
+    """The ``PagedAttention`` whose bound method ``attention`` is, for the
+    stack's prefill and decode."""
+
+    owner = getattr(attention, "__self__", None)
+    return owner if isinstance(owner, PagedAttention) else None

@@ -16,6 +16,7 @@ gate, output projection).  Float32; there is no CPU path.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Callable, Sequence
 
@@ -23,6 +24,7 @@ import torch
 
 from .controller import SDMController, finish_sdm_step, prepare_sdm_step
 from .inference import FaithfulSDMDecodeState, pack_prefill_layers
+from .kv_cache import paged_owner
 from .recurrence import route_recurrence
 
 
@@ -160,34 +162,39 @@ def prefill_faithful_sdm_stack(
     if "A" in layout and attention_block is None:
         raise ValueError("an attention layer needs attention_block")
 
-    keys: list[torch.Tensor] = []
-    values: list[torch.Tensor] = []
-    handoffs = []   # (initial memory, final memory, write routes) per SDM layer
-    sdm_index = 0
-    for layer, kind in enumerate(layout):
-        if kind == "A":
-            tokens, key, value = attention_block(layer, tokens)
-            key_cache, value_cache = allocate_dense_cache(key, value, selected_capacity)
-            keys.append(key_cache)
-            values.append(value_cache)
-            continue
-        controller, initial_memory = sdm_layers[sdm_index]
-        pre = prefill_sdm_layer(controller, initial_memory, tokens)
-        tokens = tokens + pre.output
-        if sdm_tail is not None:
-            tokens = sdm_tail(layer, tokens)
-        handoffs.append((initial_memory, pre.final_memory, pre.write_indices))
-        del pre
-        sdm_index += 1
-    # every SDM layer's handoff (_pack_prefill_layer, inference.py:314-366)
-    # at once: the handoff's host reads are made once for all layers
-    states = pack_prefill_layers(
-        [h[0] for h in handoffs], [h[1] for h in handoffs], [h[2] for h in handoffs],
-        capacity_rows=list(per_layer), decode_capacity=selected_capacity,
-        growth_quantum_rows=sdm_growth_quantum_rows)
-    del handoffs
-    return tokens, FaithfulSDMDecodeState(
-        layout=layout, position=time, capacity=selected_capacity, activation_dtype=tokens.dtype,
-        active_sequences=torch.ones(batch, device=tokens.device, dtype=torch.bool),
-        sdm_layer_positions=layer_positions, sdm_states=tuple(states),
-        dense_keys=tuple(keys), dense_values=tuple(values))
+    # a paged cache admits the requests before any layer has run, and lets them
+    # go again where one raises
+    paged = paged_owner(attention_block) if "A" in layout else None
+    with nullcontext() if paged is None else paged.prefill_step(batch, time):
+        keys: list[torch.Tensor] = []
+        values: list[torch.Tensor] = []
+        handoffs = []   # (initial memory, final memory, write routes) per SDM layer
+        sdm_index = 0
+        for layer, kind in enumerate(layout):
+            if kind == "A":
+                tokens, key, value = attention_block(layer, tokens)
+                key_cache, value_cache = allocate_dense_cache(key, value, selected_capacity)
+                keys.append(key_cache)
+                values.append(value_cache)
+                continue
+            controller, initial_memory = sdm_layers[sdm_index]
+            pre = prefill_sdm_layer(controller, initial_memory, tokens)
+            tokens = tokens + pre.output
+            if sdm_tail is not None:
+                tokens = sdm_tail(layer, tokens)
+            handoffs.append((initial_memory, pre.final_memory, pre.write_indices))
+            del pre
+            sdm_index += 1
+        # every SDM layer's handoff (_pack_prefill_layer, inference.py:314-366)
+        # at once: the handoff's host reads are made once for all layers
+        states = pack_prefill_layers(
+            [h[0] for h in handoffs], [h[1] for h in handoffs], [h[2] for h in handoffs],
+            capacity_rows=list(per_layer), decode_capacity=selected_capacity,
+            growth_quantum_rows=sdm_growth_quantum_rows)
+        del handoffs
+        return tokens, FaithfulSDMDecodeState(
+            layout=layout, position=time, capacity=selected_capacity,
+            activation_dtype=tokens.dtype,
+            active_sequences=torch.ones(batch, device=tokens.device, dtype=torch.bool),
+            sdm_layer_positions=layer_positions, sdm_states=tuple(states),
+            dense_keys=tuple(keys), dense_values=tuple(values))

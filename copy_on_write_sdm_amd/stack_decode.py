@@ -26,6 +26,7 @@ token, one per request (``positions``) after admissions at other lengths.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Callable, Sequence
 
 import torch
@@ -33,6 +34,7 @@ import torch
 from .controller import (SDMController, can_decode_layers, decode_sdm_layer_controller,
                          decode_sdm_layers_controller)
 from .inference import FaithfulSDMDecodeState
+from .kv_cache import paged_owner
 
 AttentionDecode = Callable[[int, torch.Tensor, torch.Tensor, torch.Tensor, "int | torch.Tensor"],
                            torch.Tensor]
@@ -95,14 +97,19 @@ def decode_faithful_sdm_stack(
         raise ValueError("decode state layout does not match the stack")
     if tokens.device != state.device or tokens.dtype != state.dtype:
         raise ValueError("decode tokens do not match state device and dtype")
+    paged = paged_owner(attention_decode) if "A" in layout else None
     if state.positions is None:
         if state.position >= state.capacity:
             raise ValueError("decode state has reached its fixed capacity")
         attention_position: int | torch.Tensor = int(state.position)
-        furthest = int(state.position)
+        furthest = at = int(state.position)
     else:
         positions = state.positions
-        furthest = int(positions.max().item()) if positions.numel() else -1
+        if paged is None:
+            furthest = int(positions.max().item()) if positions.numel() else -1
+        else:        # which compares them with its own
+            at = positions.tolist()
+            furthest = max(at, default=-1)
         if furthest >= state.capacity:
             raise ValueError("decode state has reached its fixed capacity")
         attention_position = positions
@@ -119,39 +126,42 @@ def decode_faithful_sdm_stack(
     if expected_dense and attention_decode is None:
         raise ValueError("an attention layer needs attention_decode")
 
-    dense_index = 0
-    sdm_index = 0
-    done = 0   # layers below this one have run
-    for layer, kind in enumerate(layout):
-        if layer < done:
-            continue
-        if kind == "A":
-            tokens = attention_decode(layer, tokens, state.dense_keys[dense_index],
-                                      state.dense_values[dense_index], attention_position)
-            dense_index += 1
-            continue
-        if state.sdm_layer_positions[sdm_index] != layer:
-            raise ValueError("SDM decode layer ordering is inconsistent")
-        # SDM layers in a row with nothing of the caller's between them run
-        # as one chain of launches
-        run = 0
-        while (sdm_tail is None and layer + run < len(layout) and layout[layer + run] == "B"
-               and state.sdm_layer_positions[sdm_index + run] == layer + run
-               and can_decode_layers(state.sdm_states[sdm_index + run], backend)):
-            run += 1
-        if run:
-            tokens = decode_sdm_layers_controller(
-                controllers[sdm_index:sdm_index + run],
-                state.sdm_states[sdm_index:sdm_index + run], tokens)
-            sdm_index += run
-            done = layer + run
-            continue
-        mixed = decode_sdm_layer_controller(controllers[sdm_index], tokens,
-                                            state.sdm_states[sdm_index], backend=backend)
-        tokens = tokens + mixed
-        if sdm_tail is not None:
-            tokens = sdm_tail(layer, tokens)
-        sdm_index += 1
+    # a paged cache opens the token's step before any layer has run: one that
+    # it refuses changes nothing, and one that fails is taken back
+    with nullcontext() if paged is None else paged.decode_step(state.batch, at):
+        dense_index = 0
+        sdm_index = 0
+        done = 0   # layers below this one have run
+        for layer, kind in enumerate(layout):
+            if layer < done:
+                continue
+            if kind == "A":
+                tokens = attention_decode(layer, tokens, state.dense_keys[dense_index],
+                                          state.dense_values[dense_index], attention_position)
+                dense_index += 1
+                continue
+            if state.sdm_layer_positions[sdm_index] != layer:
+                raise ValueError("SDM decode layer ordering is inconsistent")
+            # SDM layers in a row with nothing of the caller's between them run
+            # as one chain of launches
+            run = 0
+            while (sdm_tail is None and layer + run < len(layout) and layout[layer + run] == "B"
+                   and state.sdm_layer_positions[sdm_index + run] == layer + run
+                   and can_decode_layers(state.sdm_states[sdm_index + run], backend)):
+                run += 1
+            if run:
+                tokens = decode_sdm_layers_controller(
+                    controllers[sdm_index:sdm_index + run],
+                    state.sdm_states[sdm_index:sdm_index + run], tokens)
+                sdm_index += run
+                done = layer + run
+                continue
+            mixed = decode_sdm_layer_controller(controllers[sdm_index], tokens,
+                                                state.sdm_states[sdm_index], backend=backend)
+            tokens = tokens + mixed
+            if sdm_tail is not None:
+                tokens = sdm_tail(layer, tokens)
+            sdm_index += 1
     if state.positions is None:
         state.position += 1
     else:
