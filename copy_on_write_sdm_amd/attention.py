@@ -21,7 +21,8 @@ by which the codes count, [pages, heads].  The width is a head's, padded with
 zeros to 32, 64, 96, 128, 192 or 256 (``cache_width``).
 
 Kernels: csrc/prompt_attention.hip and csrc/kv_cache.hip.  Float32, float16
-and bfloat16; there is no backward pass and no CPU path.
+and bfloat16; there is no backward pass (inputs that require a gradient are
+refused, where gradients are recorded) and no CPU path.
 """
 
 from __future__ import annotations
@@ -56,6 +57,12 @@ def cache_width(head_width: int) -> int:
 def _need_device(tensor: torch.Tensor, what: str) -> None:
     if not tensor.is_cuda:
         raise RuntimeError(f"{what} must be on the GPU: the attention kernels have no CPU path")
+
+
+def _need_no_gradient(*tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+        raise RuntimeError("the attention operators have no backward pass: call them under "
+                           "torch.no_grad(), or with detached inputs")
 
 
 def _float_type(dtype: torch.dtype) -> int:
@@ -125,6 +132,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if not kv_heads or not heads or heads % kv_heads:
         raise ValueError("query heads must be a multiple of the key heads")
     cache_width(width)
+    _need_no_gradient(query, key, value)
     dtype = query.dtype
     code = _float_type(dtype)
     if key.dtype is not dtype or value.dtype is not dtype:
@@ -281,6 +289,7 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
     if key.ndim != 3 or value.shape != key.shape:
         raise ValueError("cache writes take key and value [T,heads,D]")
     tokens, heads, width = key.shape
+    _need_no_gradient(key, value)
     _need_device(key, "cache writes")
     device = key.get_device()
     code = _float_type(key.dtype)
@@ -328,6 +337,7 @@ def cached_attention(query: torch.Tensor, key_pages: torch.Tensor, key_scales: t
     if query.ndim != 4:
         raise ValueError("cached attention takes query [B,n,heads,D]")
     batch, tokens, heads, width = query.shape
+    _need_no_gradient(query)
     _need_device(query, "attention inputs")
     device, index = query.device, query.get_device()
     code = _float_type(query.dtype)

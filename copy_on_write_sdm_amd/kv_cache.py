@@ -353,6 +353,7 @@ class PagedAttention:
 
     # ------------------------------------------------------------ the layers
 
+    @torch.no_grad()
     def prefill(self, layer: int, tokens: torch.Tensor):
         """``attention_block``: tokens [B, T, width] of B new requests."""
 
@@ -372,6 +373,7 @@ class PagedAttention:
         self._next = index + 1
         return out, none, none
 
+    @torch.no_grad()
     def decode(self, layer: int, tokens: torch.Tensor, key_cache: torch.Tensor,
                value_cache: torch.Tensor, position: "int | torch.Tensor") -> torch.Tensor:
         """``attention_decode``: one more token [B, 1, width] of every request."""

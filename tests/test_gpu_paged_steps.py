@@ -261,3 +261,13 @@ def test_take_back(device):
     cache.extend([0, 5])
     cache.take_back()
     assert cache.request_lengths() == [17, 0] and cache.free == 6
+
+
+def test_layers_whose_weights_require_a_gradient(device):
+    """As in the stack, no gradient is recorded."""
+
+    run = Run("A", device)
+    run.wqkv[0].requires_grad_(), run.wo[0].requires_grad_()
+    out = run.block.prefill(0, run.tokens(2, 5))[0]
+    assert not out.requires_grad
+    assert not run.block.decode(0, out[:, -1:], None, None, 5).requires_grad
