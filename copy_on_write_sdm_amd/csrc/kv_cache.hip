@@ -1037,6 +1037,10 @@ int32_t check_cache(const cowsdm_kv_cache_t* c, const char* where, int& shift) {
   if (c->heads > 65535) return fail(COWSDM_ELIMIT, "%s: at most 65,535 heads", where);
   if (c->pages > 0 && (!c->key_codes || !c->key_scales || !c->value_codes || !c->value_scales))
     return fail(COWSDM_EARG, "%s: null cache tensor", where);
+  // codes are loaded 16 bytes at a time
+  if ((reinterpret_cast<uintptr_t>(c->key_codes) | reinterpret_cast<uintptr_t>(c->value_codes)) %
+      16)
+    return fail(COWSDM_EARG, "%s: cache codes must be 16-byte aligned", where);
   return 0;
 }
 

@@ -844,11 +844,11 @@ int32_t cowsdm_pages_release(int32_t* lengths, int32_t* page_tables, int64_t req
                              int32_t* free_pages, int64_t pages, int32_t* free_count,
                              int64_t page_tokens, void* stream);
 
-/* One layer's cache: e4m3 codes, keys [pages, heads, page_tokens, width],
- * values transposed [pages, heads, width, page_tokens], and a power of two
- * for each page and head, [pages, heads], by which its codes count.  width is
- * a head's width padded to 32, 64, 96, 128, 192 or 256; the padding holds
- * zeros. */
+/* One layer's cache: e4m3 codes, 16-byte aligned, keys [pages, heads,
+ * page_tokens, width] and values transposed, [pages, heads, width,
+ * page_tokens], and a power of two for each page and head, [pages, heads], by
+ * which its codes count.  width is a head's width padded to 32, 64, 96, 128,
+ * 192 or 256; the padding holds zeros. */
 typedef struct cowsdm_kv_cache {
   int64_t pages;
   int64_t heads;
@@ -875,8 +875,8 @@ int32_t cowsdm_kv_write(const cowsdm_kv_cache_t* cache, const void* key, int64_t
 /* The newest `tokens` tokens of each request over the cache: query row i of
  * request r sees positions 0 .. lengths[r] - tokens + i, but for those whose
  * table entry is no page of the pool.  A row that sees nothing gives 0.
- * `longest` is the longest length, or more; a smaller value
- * costs time, not correctness. */
+ * `longest` is the longest length, or more; a smaller value costs time, not
+ * correctness. */
 typedef struct cowsdm_cached_query {
   const void* query;               /* [requests, tokens, heads, width]     */
   int64_t query_request, query_token, query_head;   /* strides, in elements */

@@ -28,3 +28,20 @@ def test_strides_of_axes_of_one_element_say_nothing():
               torch.zeros(70).as_strided((1, 1, 64), (1, 3, 1))):
         _, _, strides = attention._rows(t, 4)
         assert strides == torch.empty(t.shape).stride()
+
+
+def test_cache_codes_that_cannot_be_loaded():
+    """Codes are loaded 16 bytes at a time, from the cache's own address on."""
+
+    lib = nat.lib()
+    fake = 0x1000
+    q = nat.CachedQuery(fake, 64, 64, 64, fake, fake, fake, 2, 1, 1, 64, 3, 48, 0, 0.1)
+    for field in ("key_codes", "value_codes"):
+        for off in (1, 8, 15):
+            c = nat.KVCache(4, 1, 16, 64, fake, fake, fake, fake)
+            setattr(c, field, fake + off)
+            q.requests = 0              # nothing to run, were it not refused
+            assert lib.cowsdm_cached_attention(c, q, None, 0, None) == -1
+            assert b"codes must be 16-byte aligned" in lib.cowsdm_last_error_string()
+            assert lib.cowsdm_kv_write(c, fake, 64, 64, fake, 64, 64, 0, 64, fake, 0, None) == -1
+            assert b"codes must be 16-byte aligned" in lib.cowsdm_last_error_string()
