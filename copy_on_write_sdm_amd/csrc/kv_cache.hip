@@ -1124,7 +1124,10 @@ extern "C" int32_t cowsdm_kv_write(const cowsdm_kv_cache_t* cache, const void* k
   int shift = 0;
   if (int32_t e = check_cache(cache, "kv_write", shift)) return e;
   if (int32_t e = check_row_width(width, cache->width, "kv_write")) return e;
-  if (tokens < 0 || tokens > INT32_MAX) return fail(COWSDM_EARG, "kv_write: bad token count");
+  if (tokens < 0) return fail(COWSDM_EARG, "kv_write: bad token count");
+  // a launch counts its threads in 32 bits
+  if (tokens >= (int64_t{1} << 30))
+    return fail(COWSDM_ELIMIT, "kv_write: 2^30 tokens or more a call");
   if (float_type != COWSDM_FLOAT32 && float_type != COWSDM_FLOAT16 &&
       float_type != COWSDM_BFLOAT16)
     return fail(COWSDM_EARG, "kv_write: bad float type");
@@ -1226,6 +1229,9 @@ extern "C" int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
   p.row_tiles = static_cast<int32_t>(tiles);
   p.splits = static_cast<int32_t>(
       cached_splits(q.requests, cache->heads, tiles, cache->width, q.longest));
+  // a launch counts its threads in 32 bits
+  if (tiles * p.splits * cached_waves(cache->width) * kWave > UINT32_MAX)
+    return fail(COWSDM_ELIMIT, "cached_attention: too many query rows a request");
   const int64_t kBlock = cached_waves(cache->width) * kCachedTokens;
   const int64_t each = (q.longest + p.splits - 1) / p.splits;
   p.chunk = p.splits == 1 ? INT32_MAX / 2

@@ -45,3 +45,16 @@ def test_cache_codes_that_cannot_be_loaded():
             assert b"codes must be 16-byte aligned" in lib.cowsdm_last_error_string()
             assert lib.cowsdm_kv_write(c, fake, 64, 64, fake, 64, 64, 0, 64, fake, 0, None) == -1
             assert b"codes must be 16-byte aligned" in lib.cowsdm_last_error_string()
+
+
+def test_writes_and_queries_of_more_than_a_launch_holds():
+    lib = nat.lib()
+    fake = 0x1000
+    c = nat.KVCache(4, 1, 16, 64, fake, fake, fake, fake)
+    for tokens in (1 << 30, (1 << 31) - 1):
+        assert lib.cowsdm_kv_write(c, fake, 64, 64, fake, 64, 64, 0, 64, fake, tokens, None) == -2
+        assert b"2^30" in lib.cowsdm_last_error_string()
+    # 65,535 query tokens of 65,535 heads over one key head: 2^28 tiles of rows
+    q = nat.CachedQuery(fake, 64, 64, 64, fake, fake, fake, 1, 65535, 65535, 64, 3, 48, 0, 0.1)
+    assert lib.cowsdm_cached_attention(c, q, None, 0, None) == -2
+    assert b"query rows" in lib.cowsdm_last_error_string()
