@@ -186,10 +186,11 @@ def extend_page_tables(lengths: torch.Tensor, added: torch.Tensor, page_tables: 
                        free_pages: torch.Tensor, free_count: torch.Tensor, *, page_tokens: int,
                        tokens: int, out: Sequence[torch.Tensor] | None = None) -> PageTableStep:
     """Room for ``added`` [B] new tokens of requests that hold ``lengths``
-    [B]: pages popped from the top of the free stack (``free_pages`` [P],
-    ``free_count`` [1]) in request order go into ``page_tables`` [B, columns]
-    in place, and every new token gets its position and slot (page *
-    page_tokens + position % page_tokens).  ``tokens`` is the size of the
+    [B]: pages popped from the top of the free stack (``free_pages``, of which
+    the first ``free_count`` [1] are free) in request order go into
+    ``page_tables`` [B, columns] in place, and every new token gets its
+    position and slot (page * page_tokens + position % page_tokens; -1 where
+    the table holds no page).  ``tokens`` is the size of the
     packed token outputs, at least the sum of ``added``; entries past it are
     -1.  Where the pages, the columns or ``tokens`` do not suffice, or a count
     is negative, ``overflow`` is 1, positions and slots are -1 and the tables

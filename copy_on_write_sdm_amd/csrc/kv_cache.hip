@@ -153,7 +153,9 @@ __global__ __launch_bounds__(kTableThreads) void extend_tables_kernel(ExtendPara
         id = p.free_pages[count - 1 - (s_pages[lo] + column)];
         if ((position & (page - 1)) == 0) *entry = id;
       }
-      if (id >= 0 && id < p.pages) slot = id * page + (position & (page - 1));
+      // an entry that is no page of the pool gives a slot that is none either
+      if (id >= 0 && id <= (INT32_MAX >> p.page_shift))
+        slot = (id << p.page_shift) + (position & (page - 1));
     }
     p.positions[t] = position;
     p.slots[t] = slot;

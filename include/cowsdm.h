@@ -822,8 +822,8 @@ int32_t cowsdm_prompt_attention(const cowsdm_prompt_attention_t* attention, void
 /* A step's page tables and token slots.  Request r holds lengths[r] tokens in
  * the pages page_tables[r][0 .. ceil(lengths[r] / page_tokens) - 1] and gets
  * added[r] more.  New pages come from the top of the free stack
- * free_pages[0 .. *free_count - 1] in request order and are written to the
- * tables in place.  lengths_out [requests] and *free_count_out get the sums
+ * free_pages[0 .. *free_count - 1], which has room for `pages`, in request
+ * order and are written to the tables in place.  lengths_out [requests] and *free_count_out get the sums
  * (they are not lengths and free_count themselves), offsets [requests + 1]
  * the new tokens before each request, and token t of the packed new tokens
  * its position in its request and its slot page * page_tokens + position %
