@@ -1155,6 +1155,13 @@ extern "C" int32_t cowsdm_kv_write(const cowsdm_kv_cache_t* cache, const void* k
   p.width = static_cast<int32_t>(width);
   p.pages = static_cast<int32_t>(cache->pages);
   p.page_shift = shift;
+  // Single tokens are a run each and want a workgroup each; of a prompt's, whose
+  // runs are pages, most workgroups would find nothing to open.  The call does
+  // not say which it is, so that the token count has to: 8 heads of 128, us by
+  // one token and by 64 a workgroup: 512 single tokens 24 and 188, 1,024 41 and
+  // 186, 2,048 75 and 185, 4,096 188 and 223; 16 prompts of 64 32 and 10, 4 of
+  // 500 21 and 10, 8 of 2,000 341 and 25.  So more than 1,024 single tokens, and
+  // prompts of fewer in all, take the slower side.
   p.chunk = tokens <= 1024 ? 1 : kWave;
   const dim3 grid(static_cast<uint32_t>((tokens + p.chunk - 1) / p.chunk),
                   static_cast<uint32_t>(cache->heads));

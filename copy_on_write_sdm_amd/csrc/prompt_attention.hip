@@ -42,8 +42,11 @@ struct PromptWork {
 // one XCD where the pairs divide by eight, so that its keys and values stay
 // in that XCD's L2.  Later query blocks, which see more keys, come first: of
 // all pairs in small grids, where what starts last decides (16 heads of 4,096
-// tokens: 92 us, pair by pair 118), and pair by pair in large ones, whose keys
-// and values would push each other out (2 x 8,192: 1,015 against 1,031).
+// tokens: 91 us, pair by pair 112), and pair by pair in large ones, whose keys
+// and values would push each other out (24 prompts of 2,048, 32 heads over 8:
+// 909 against 936; 2 x 8,192: 987 against 991).  The grid's size counts
+// workgroups that end at once, too: a prompt of 8,192 among 30 of 64 has a
+// large grid and little work, and takes 589 pair by pair, 545 the other way.
 __device__ __forceinline__ PromptWork prompt_work(const PromptParams& p) {
   const int group = p.heads / p.kv_heads;
   const int pairs = p.sequences * p.kv_heads;
@@ -842,14 +845,19 @@ template <typename T, int DP>
 int32_t launch_prompt_half(const PromptParams& p, int64_t longest, hipStream_t stream) {
   constexpr int kTiles = 2 * 2 * kTileKeys * DP * 2;
   if constexpr (DP <= 128) {
-    // Where the chip holds all workgroups of 64 rows at once, by the LDS they
-    // take: 8 heads of 1,000 tokens at width 128 take 18 us so and 24 us by 128
-    // rows, 8 of 4,096 at width 64 34 and 50, 8 of 8,192 at width 32 69 and 89.
-    // Short rows lose by the join, the more so as the chip is full (4 prompts
-    // of 100: 11.6 against 10.4; 2 of 550, 32 heads of 64: 14.6 against 11.9;
-    // 8 of 600, 8 heads: 10.8 against 12.3), and more workgroups by their
-    // tiles' traffic (4 of 1,024, 12 heads of 64: 21 against 18; 16 heads of
-    // 4,096 at width 128: 127 against 119).
+    // For grids that are small beside what the chip holds, by the LDS that
+    // workgroups of 64 rows take.  The bounds are fitted, on the safe side: a
+    // split that is not taken costs less than one too many.  At width 128,
+    // where a CU holds one: 8 heads of 1,000 tokens take 19 us so and 22.5 by
+    // 128 rows, 18 heads (the bound) 20 and 23, 24 heads 23.7 and 23.0; 16 heads
+    // of 600 14.6 and 16.3, and past the bound 24 still 14.9 and 16.8; 4 heads
+    // of 4,096 50 and 68, past it 8 heads 59 and 69, 16 heads 114 and 85.
+    // Narrower: 8 of 4,096 at width 64 36 and 51, 8 of 8,192 at width 32 69 and
+    // 89, 8 prompts of 600 with 8 heads of 32 11 and 12.5.  More workgroups
+    // lose by their tiles' traffic (4 of 1,024, 12 heads of 64: 20 and 18; 8 of
+    // 600, 8 heads of 64: 16 and 13.5; 2 of 550, 32 heads of 64: 15 and 12.5),
+    // and shorter rows gain no more than the join takes (450 tokens, 8 heads of
+    // 64: 10.4 and 11.2; 300: 10.4 and 10.5; 4 of 100: 10.9 and 10.8).
     const int64_t most = (static_cast<int64_t>(p.rows) / 64 + p.sequences) * p.heads;
     constexpr int kJoin = 2 * PromptRows<T, DP>::kFloats * 4;
     constexpr int kBytes = 2 * kTiles > kJoin ? 2 * kTiles : kJoin;
