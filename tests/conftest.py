@@ -22,3 +22,30 @@ def device():
     if not torch.cuda.is_available():
         pytest.fail("GPU test requested but no HIP device is visible")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def cleared_memory():
+    """GPU tests of a module start on memory without the NaN that other modules
+    leave: some compare whole buffers, places that nothing has written too, and
+    a NaN there differs from its own copy."""
+
+    import torch
+
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
+        taken = []
+        # what the allocator holds free in segments that are in use
+        for size in [1 << n for n in range(24, 20, -1)] + [(1 << 20) + 512] + [
+                1 << n for n in range(20, 8, -1)]:
+            while True:
+                held = torch.cuda.memory_reserved()
+                part = torch.zeros(size, dtype=torch.uint8, device="cuda")
+                if torch.cuda.memory_reserved() > held:
+                    break
+                taken.append(part)
+            del part
+            torch.cuda.empty_cache()
+        taken.clear()
+        torch.cuda.empty_cache()
+    yield
