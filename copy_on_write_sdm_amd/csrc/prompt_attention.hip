@@ -1,7 +1,8 @@
 // Causal attention over packed prompts with grouped heads.
 //
 // out[i] = sum_{j <= i} softmax_j(scale q_i . k_j) v_j, in one pass over the
-// keys with the running maximum and sum of each row.  Scores are computed
+// keys with the running maximum and sum of each row (the online softmax of
+// Milakov and Gimelshein, 2018).  Scores are computed
 // transposed, S^T = K Q^T, so that a lane holds keys of one query row and its
 // probabilities are the right operand of O^T = V^T P^T where they stand:
 // neither scores nor probabilities leave the registers.

@@ -15,7 +15,8 @@ residual stream; consecutive ones without a tail between them share launches
   reference's ``attention.decode_with_cache`` at the request positions, its
   residual add and its MLP, model.py:127-185).  It writes the token's key and
   value into that layer's cache; ``write_dense_cache`` does that write as the
-  reference does;
+  reference does, and ``PagedAttention.decode`` writes a paged cache, whose step
+  is opened before the first layer runs and taken back where one raises;
 * ``sdm_tail(layer, tokens) -> tokens`` after an SDM layer's residual add
   (the reference's SDM MLP; identity when omitted).
 
