@@ -281,6 +281,10 @@ struct PromptRows {
     // 32 bits, and a probability keeps its bits in 16.
     if (__any(top > most + 8.0f)) rise(fmaxf(most, top));
     const float shift = most == kMinusInf ? 0.0f : most;
+    // A 16-bit product takes its probabilities in 16 bits (the error against 64
+    // bits is 0.0020 of the output's size in bfloat16, 0.0016 with
+    // probabilities of 32 bits; 0.00025 and 0.00020 in float16); their sum
+    // stays in 32.
     vec prob[4];
     float part[4] = {};
 #pragma unroll
