@@ -109,8 +109,9 @@ def draw(rng):
         most = 16383 * 40 * 128 * 2 // ((heads + kv_heads) * width * FLOATS[floats].itemsize)
         return dict(kind=kind, rows=_log_int(rng, 1, min(65536, most)), heads=heads,
                     kv_heads=kv_heads, width=width,
-                    rotated=rng.choice([width, width, width // 16 * 8]), interleaved=rng.random() < 0.3,
-                    norm=rng.random() < 0.7, furthest=_log_int(rng, 16, 1 << 22), floats=floats)
+                    rotated=rng.choice([width, width, width // 16 * 8]),
+                    interleaved=rng.random() < 0.3, norm=rng.random() < 0.7,
+                    furthest=_log_int(rng, 16, 1 << 22), floats=floats)
     if kind == "release":
         family = rng.choice([1, 1, 2, 4, 8])
         batch = family * _log_int(rng, 1, 1024 // family)
