@@ -42,6 +42,17 @@ from .attention import (
     prompt_attention,
     write_kv_cache,
 )
+from .linear import linear
+from .head_rotation import HeadRotation, rotate_heads
+from .pages import (
+    PageFork,
+    PageMoves,
+    PageRelease,
+    compact_page_tables,
+    copy_pages,
+    fork_page_tables,
+    release_page_tables,
+)
 from .kv_cache import PagedAttention, PagedKVCache
 from .controller import (
     ControllerDecodeGraph,
@@ -60,7 +71,11 @@ __all__ = [
     "SDMController",
     "SDMPrefill",
     "FaithfulSDMDecodeState",
+    "HeadRotation",
     "PackedSDMCopyOnWriteState",
+    "PageFork",
+    "PageMoves",
+    "PageRelease",
     "PageTableStep",
     "PagedAttention",
     "PagedKVCache",
@@ -70,6 +85,8 @@ __all__ = [
     "allocate_dense_cache",
     "cache_width",
     "cached_attention",
+    "compact_page_tables",
+    "copy_pages",
     "decode_faithful_sdm_stack",
     "decode_sdm_layer",
     "decode_sdm_layer_controller",
@@ -80,7 +97,9 @@ __all__ = [
     "dense_sparse_routes",
     "extend_page_tables",
     "finish_sdm_step",
+    "fork_page_tables",
     "gated_delta_recurrence",
+    "linear",
     "mark_written",
     "pack_prefill_layer",
     "pack_prefill_layers",
@@ -91,6 +110,8 @@ __all__ = [
     "prepare_sdm_step",
     "product_key_routes",
     "prompt_attention",
+    "release_page_tables",
+    "rotate_heads",
     "sdm_recurrence",
     "write_dense_cache",
     "write_kv_cache",

@@ -25,7 +25,8 @@ SOURCE_DIR = PACKAGE_DIR / "csrc"
 # one translation unit per step-kernel family so hipcc can run in parallel
 SOURCES = ("cowsdm.hip", "step_i32_packed.hip", "step_i32_dense.hip", "step_i64_packed.hip",
            "step_i64_dense.hip", "trace_plan.hip", "routes.hip", "controller.hip",
-           "recurrence.hip", "route_recurrence.hip", "prompt_attention.hip", "kv_cache.hip")
+           "recurrence.hip", "route_recurrence.hip", "prompt_attention.hip", "kv_cache.hip",
+           "pages.hip", "head_rotation.hip", "linear.hip")
 INCLUDE_DIR = REPO_DIR / "include"
 LIBRARY = PACKAGE_DIR / "lib" / "libcowsdm.so"
 BUILD_DIR = PACKAGE_DIR / "_build"
@@ -361,6 +362,53 @@ class CachedQuery(ctypes.Structure):
     ]
 
 
+class Linear(ctypes.Structure):
+    """cowsdm_linear_t."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("x_row", ctypes.c_int64),
+        ("weight_row", ctypes.c_int64),
+        ("residual_row", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("inner", ctypes.c_int64),
+        ("outer", ctypes.c_int64),
+        ("float_type", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+    ]
+
+
+class RotateHeads(ctypes.Structure):
+    """cowsdm_rotate_heads_t."""
+
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("key", ctypes.c_void_p),
+        ("query_row", ctypes.c_int64),
+        ("query_head", ctypes.c_int64),
+        ("key_row", ctypes.c_int64),
+        ("key_head", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("turns", ctypes.c_void_p),
+        ("query_weight", ctypes.c_void_p),
+        ("key_weight", ctypes.c_void_p),
+        ("query_out", ctypes.c_void_p),
+        ("key_out", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("rotated", ctypes.c_int64),
+        ("interleaved", ctypes.c_int32),
+        ("float_type", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -457,6 +505,18 @@ SIGNATURES: dict[str, tuple] = {
         _I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "cowsdm_cached_attention": (
         _I32, [ctypes.POINTER(KVCache), ctypes.POINTER(CachedQuery), _P, _I64, _P]),
+    "cowsdm_page_tables_fork": (
+        _I32, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P,
+               _P, _P]),
+    "cowsdm_page_tables_release_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "cowsdm_page_tables_release": (
+        _I32, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
+    "cowsdm_page_tables_compact_workspace_bytes": (_I64, [_I64]),
+    "cowsdm_page_tables_compact": (
+        _I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "cowsdm_pages_copy": (_I32, [ctypes.POINTER(KVCache), _I64, _P, _P, _I64, _P]),
+    "cowsdm_linear": (_I32, [ctypes.POINTER(Linear), _P]),
+    "cowsdm_rotate_heads": (_I32, [ctypes.POINTER(RotateHeads), _P]),
     "cowsdm_product_key_routes": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P]),
 }
 

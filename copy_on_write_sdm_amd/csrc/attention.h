@@ -1,6 +1,6 @@
-// What the attention kernels share: vector types, conversions between the
-// float types and the 8-bit codes of the K/V cache, and the softmax's moves
-// across the lanes of a wave.
+// What the kernels of the attention layers share: vector types, conversions
+// between the float types and the 8-bit codes of the K/V cache, the softmax's
+// moves across the lanes of a wave, and loads from memory into LDS.
 #pragma once
 
 #include "common.h"
@@ -115,6 +115,19 @@ template <>
 struct AttentionType<_Float16> { static constexpr int kParts = 2, kProbParts = 2; };
 template <>
 struct AttentionType<__bf16> { static constexpr int kParts = 1, kProbParts = 2; };
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+// 16 bytes a lane from `from` bytes past `first` to 16 times the lane past
+// `to` (the wave's), 0 where they lie past the first `bytes`.
+__device__ __forceinline__ void load_to_lds(const void* first, int bytes, uint32_t from,
+                                            lds_char* to) {
+#if defined(__HIP_DEVICE_COMPILE__)   // the host's pass does not know the load's width
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, bytes, 0x00020000),
+      (__attribute__((address_space(3))) void*)to, 16, from, 0, 0, 0);
+#endif
+}
 
 // four consecutive elements from float32
 template <typename T>

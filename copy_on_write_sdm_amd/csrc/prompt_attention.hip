@@ -127,19 +127,6 @@ __device__ __forceinline__ int place(int row, int c) {
   else return c ^ ((row >> 2) & 3);
 }
 
-typedef __attribute__((address_space(3))) char lds_char;
-
-// 16 bytes a lane from `from` bytes past `first` to 16 times the lane past
-// `to` (the wave's), 0 where they lie past the first `bytes`.
-__device__ __forceinline__ void load_to_lds(const void* first, int bytes, uint32_t from,
-                                            lds_char* to) {
-#if defined(__HIP_DEVICE_COMPILE__)   // the host's pass does not know the load's width
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, bytes, 0x00020000),
-      (__attribute__((address_space(3))) void*)to, 16, from, 0, 0, 0);
-#endif
-}
-
 // This thread's chunks of a tile into LDS, a wave's side by side.  Rows past
 // the sequence's end and columns past the width read as 0.
 template <int kLoads, int kThreads>

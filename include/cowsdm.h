@@ -902,6 +902,129 @@ int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
                                 const cowsdm_cached_query_t* query, void* workspace,
                                 int64_t workspace_bytes, void* stream);
 
+/* The life of a cache's pages besides their extension.  page_shares[p] counts
+ * the requests that hold page p beyond the first (zeros where nothing is
+ * shared); pages that requests share are full.  Inputs stay as they are, but
+ * for the free stack, which a release writes above its count: lengths, tables,
+ * counts and shares come out new and are not the inputs themselves.  At most
+ * 4,096 requests; page_tokens is 16, 32, 64, 128 or 256. */
+
+/* n new requests: child i holds the first tokens[i] tokens of request
+ * parents[i].  Its whole pages are the parent's and get a sharer more each;
+ * where its tokens end inside a page it gets a page of its own, popped from the
+ * free stack in the children's order, and sources[i] and targets[i] name the
+ * parent's page and that one (-1 else).  tables_out is [children, columns], -1
+ * past a child's pages.  Where a parent or a token count is out of range or
+ * the pages do not suffice, *overflow is 1, the children are empty and
+ * nothing else changes. */
+int32_t cowsdm_page_tables_fork(
+    const int32_t* lengths, const int32_t* page_tables, int64_t requests, int64_t columns,
+    const int32_t* page_shares, const int32_t* free_pages, int64_t pages,
+    const int32_t* free_count, const int32_t* parents, const int32_t* tokens, int64_t children,
+    int64_t page_tokens, int32_t* lengths_out, int32_t* tables_out, int32_t* shares_out,
+    int32_t* free_count_out, int32_t* sources, int32_t* targets, int32_t* overflow,
+    void* stream);
+
+/* Bytes of workspace that a call of cowsdm_page_tables_release needs. */
+int64_t cowsdm_page_tables_release_workspace_bytes(int64_t pages, int64_t columns, int64_t n);
+
+/* The n named requests let their pages go (a second naming, and a number that
+ * is no request, count for nothing).  A page that no request holds any more
+ * goes onto the free stack, in place above *free_count, in the order of the
+ * list and then of the columns; one that several named requests held, where
+ * the last of them lists it.  The named requests' lengths become 0.  (What
+ * cowsdm_pages_release does in place where nothing is shared.) */
+int32_t cowsdm_page_tables_release(
+    const int32_t* lengths, const int32_t* page_tables, int64_t requests, int64_t columns,
+    const int32_t* page_shares, int32_t* free_pages, int64_t pages, const int32_t* free_count,
+    const int32_t* named, int64_t n, int64_t page_tokens, int32_t* lengths_out,
+    int32_t* shares_out, int32_t* free_count_out, void* workspace, int64_t workspace_bytes,
+    void* stream);
+
+/* Bytes of workspace that a call of cowsdm_page_tables_compact needs. */
+int64_t cowsdm_page_tables_compact_workspace_bytes(int64_t pages);
+
+/* The U pages that requests hold get the numbers below U: those numbered U or
+ * more go, in ascending order, to the numbers below U that none holds.
+ * sources and targets [pages / 2] name the moves, -1 past the last; the free
+ * stack is the other numbers, U on top, -1 past its count. */
+int32_t cowsdm_page_tables_compact(
+    const int32_t* lengths, const int32_t* page_tables, int64_t requests, int64_t columns,
+    const int32_t* page_shares, int64_t pages, int64_t page_tokens, int32_t* tables_out,
+    int32_t* shares_out, int32_t* free_pages_out, int32_t* free_count_out, int32_t* sources,
+    int32_t* targets, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Pages sources[0 .. n - 1] copied to pages targets[0 .. n - 1], codes and
+ * scales, in `layers` caches that lie one after another in each of the
+ * cache's tensors.  Entries that are no page of the pool are left out.
+ * Targets differ from each other and from every source. */
+int32_t cowsdm_pages_copy(const cowsdm_kv_cache_t* cache, int64_t layers, const int32_t* sources,
+                          const int32_t* targets, int64_t n, void* stream);
+
+/* --------------------------------------- around the attention: projections */
+
+#define COWSDM_NO_ACTIVATION 0
+#define COWSDM_RELU 1
+#define COWSDM_GELU 2        /* y Phi(y)                                      */
+#define COWSDM_GELU_TANH 3   /* y / (1 + exp(-2 sqrt(2 / pi) (y + 0.044715 y^3))) */
+#define COWSDM_SILU 4        /* y / (1 + exp(-y))                             */
+#define COWSDM_LINEAR_MOST (1 << 20)   /* elements of a row, and between rows */
+
+/* out = residual + activation(x weight^T + bias), x [rows, inner], weight
+ * [outer, inner] (rows of both contiguous), out [rows, outer] contiguous; bias
+ * [outer] and residual [rows, outer] may be null.  All of one type; sums and
+ * the rest in 32 bits, rounded once.  Any sizes and strides; operands whose
+ * addresses, widths or strides are no multiples of 16 bytes are loaded
+ * element by element.  out is none of the inputs, but may be the residual.
+ * An inner size of 0 gives activation(bias) + residual. */
+typedef struct cowsdm_linear {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  void* out;
+  int64_t x_row, weight_row, residual_row;   /* strides, in elements */
+  int64_t rows;
+  int64_t inner;
+  int64_t outer;
+  int32_t float_type;
+  int32_t activation;
+} cowsdm_linear_t;
+
+/* Runs cowsdm_linear_t; COWSDM_ELIMIT for rows of more than
+ * COWSDM_LINEAR_MOST elements. */
+int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* stream);
+
+/* Heads normed and rotated by position: of every row x [width] of query
+ * [rows, heads, width] and key [rows, kv_heads, width]
+ *   y = x rsqrt(mean(x^2) + eps) weight    (where the norm's weight is given)
+ * and then, of its first `rotated` elements, pair j (elements j and j +
+ * rotated / 2, or 2 j and 2 j + 1 where interleaved) turned by position *
+ * turns[j] / 2^64 of a full turn, which is exact in 64-bit integers at any
+ * position.  The outputs are contiguous and none of the inputs. */
+typedef struct cowsdm_rotate_heads {
+  const void* query;
+  const void* key;
+  int64_t query_row, query_head;   /* strides, in elements                 */
+  int64_t key_row, key_head;
+  const int32_t* positions;        /* [rows]                               */
+  const uint64_t* turns;           /* [rotated / 2]                        */
+  const void* query_weight;        /* [width], or null                     */
+  const void* key_weight;          /* [width], or null                     */
+  void* query_out;
+  void* key_out;
+  int64_t rows;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t width;                   /* a multiple of 8, at most 256         */
+  int64_t rotated;                 /* a multiple of 8, at most the width   */
+  int32_t interleaved;
+  int32_t float_type;
+  float eps;
+} cowsdm_rotate_heads_t;
+
+int32_t cowsdm_rotate_heads(const cowsdm_rotate_heads_t* heads, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,183 @@
+"""Projections with bias, activation and residual against the definition in 64
+bits."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import copy_on_write_sdm_amd as cow
+from attention_cases import TINY, UNIT, wide
+from oracle import projections as ref
+
+pytestmark = pytest.mark.gpu
+
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def normal(*shape, dtype, device, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g)).to(dtype).to(device)
+
+
+def assert_linear(x, weight, bias=None, activation=None, residual=None):
+    """The sum of ``inner`` rounded products and the bias in float32 is off by
+    at most (inner + 2) 2^-24 of the terms' magnitudes.  No activation's slope
+    is over 1.13.  An activation is off by at most 2^-21 of its argument:
+    exponential and reciprocal are within 2^-22 and the rest within a few units
+    of 2^-24, or 0.75e-7 for the approximated normal distribution.  The sum
+    with the residual rounds in float32 and once in the type."""
+
+    out = cow.linear(x, weight, bias, activation=activation, residual=residual)
+    inner, outer = weight.shape[1], weight.shape[0]
+    assert out.shape == (*x.shape[:-1], outer) and out.dtype is x.dtype and out.is_contiguous()
+    rows = out.numel() // outer
+    want, before, size = ref.linear(
+        wide(x).reshape(rows, inner), wide(weight), None if bias is None else wide(bias),
+        activation, None if residual is None else wide(residual).reshape(rows, outer))
+    unit = UNIT[x.dtype]
+    error = (inner + 2) * 2.0 ** -24 * size
+    if activation is not None:
+        error = 1.13 * error + 2.0 ** -21 * np.abs(before)
+    error = error + 2.0 ** -24 * (np.abs(want) + error)
+    error = error + unit * (np.abs(want) + error) + TINY[x.dtype]
+    off = np.abs(wide(out).reshape(rows, outer) - want) - error
+    assert off.max() <= 0, (off.max(), int((off > 0).sum()), off.size)
+    return out
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,inner,outer", [
+    (1, 8, 4), (1, 4096, 1024), (5, 72, 33), (16, 128, 384), (17, 264, 130), (33, 512, 48),
+    (64, 128, 384), (64, 2056, 100), (65, 64, 65), (130, 520, 260), (300, 96, 1), (129, 1024, 513),
+    (700, 136, 640), (1, 8, 1), (2000, 64, 2100)])
+def test_sizes(device, dtype, rows, inner, outer):
+    print(f"{dtype} {rows} {inner} {outer}", flush=True)
+    x = normal(rows, inner, dtype=dtype, device=device, seed=1)
+    w = normal(outer, inner, dtype=dtype, device=device, seed=2, scale=inner ** -0.5)
+    assert_linear(x, w)
+    assert_linear(x, w, normal(outer, dtype=dtype, device=device, seed=3), "gelu",
+                  normal(rows, outer, dtype=dtype, device=device, seed=4))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_large_tiles(device, dtype):
+    """More than one workgroup of the largest tiles a CU, with odd ends."""
+
+    x = normal(4099, 200, dtype=dtype, device=device, seed=5)
+    w = normal(4102, 200, dtype=dtype, device=device, seed=6, scale=0.1)
+    assert_linear(x, w, normal(4102, dtype=dtype, device=device, seed=7), "silu")
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,inner,outer", [
+    (1, 1, 1), (3, 7, 5), (70, 131, 67), (16, 2, 129), (40, 4, 8), (200, 100, 3)])
+def test_widths_that_are_not_aligned(device, dtype, rows, inner, outer):
+    x = normal(rows, inner, dtype=dtype, device=device, seed=8)
+    w = normal(outer, inner, dtype=dtype, device=device, seed=9)
+    assert_linear(x, w, normal(outer, dtype=dtype, device=device, seed=10), "relu",
+                  normal(rows, outer, dtype=dtype, device=device, seed=11))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("activation", [None, "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [3, 150])
+def test_activations(device, dtype, activation, rows):
+    """Arguments from the smallest to where the types end."""
+
+    inner = 16
+    x = normal(rows, inner, dtype=dtype, device=device, seed=12)
+    w = normal(96, inner, dtype=dtype, device=device, seed=13)
+    w *= torch.logspace(-6, 3, 96, device=device).to(dtype)[:, None]
+    assert_linear(x, w, activation=activation)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows", [6, 40, 140])
+def test_strides(device, dtype, rows):
+    """Slices whose neighbours are NaN, rows far apart, and axes turned."""
+
+    inner, outer = 104, 70
+    nan = float("nan")
+    big = torch.full((rows + 2, 3, inner + 24), nan, dtype=dtype, device=device)
+    big[1:-1, 1, 8:8 + inner] = normal(rows, inner, dtype=dtype, device=device, seed=14)
+    x = big[1:-1, 1, 8:8 + inner]
+    store = torch.full((outer + 1, inner + 8), nan, dtype=dtype, device=device)
+    store[:outer, :inner] = normal(outer, inner, dtype=dtype, device=device, seed=15)
+    w = store[:outer, :inner]
+    both = normal(rows, 2 * outer + 1, dtype=dtype, device=device, seed=16)
+    residual = both[:, 1:outer + 1]
+    bias = normal(outer, 2, dtype=dtype, device=device, seed=17)[:, 1]
+    assert_linear(x, w, bias, None, residual)
+    odd = big[1:-1, 1, 9:8 + inner]                     # rows that are not aligned
+    assert_linear(odd, store[:outer, 1:inner], bias, "relu", residual)
+    turned = normal(inner, rows, dtype=dtype, device=device, seed=18).t()
+    assert_linear(turned, normal(inner, outer, dtype=dtype, device=device, seed=19).t())
+    one = normal(1, inner, dtype=dtype, device=device, seed=20).expand(rows, inner)
+    assert_linear(one, w[:1].expand(outer, inner), residual=residual[:1].expand(rows, outer))
+    assert_linear(x.reshape(2, rows // 2, inner), w, residual=residual.reshape(2, -1, outer))
+    assert_linear(x[0], w, residual=residual[0])
+
+
+@pytest.mark.parametrize("rows", [4, 60, 200])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_what_is_not_finite_stays_in_its_row_and_column(device, dtype, rows):
+    x = normal(rows, 72, dtype=dtype, device=device, seed=21)
+    w = normal(50, 72, dtype=dtype, device=device, seed=22)
+    x[2, 5], w[7, 70] = float("nan"), float("inf")
+    x[:, 70] = 1.0
+    residual = normal(rows, 50, dtype=dtype, device=device, seed=23)
+    residual[0, 3] = float("-inf")
+    out = cow.linear(x, w, residual=residual)
+    assert bool(torch.isnan(out[2]).all())
+    others = [r for r in range(rows) if r != 2]
+    assert bool((out[others, 7] == float("inf")).all())
+    assert out[0, 3] == float("-inf")
+    rest = torch.ones_like(out, dtype=torch.bool)
+    rest[2], rest[:, 7], rest[0, 3] = False, False, False
+    assert bool(torch.isfinite(out[rest]).all())
+
+
+def test_nothing_to_sum_and_nothing_to_write(device):
+    x = torch.zeros(3, 0, device=device)
+    bias = torch.tensor([1.0, -2.0], device=device)
+    assert cow.linear(x, torch.zeros(2, 0, device=device)).tolist() == [[0.0, 0.0]] * 3
+    out = cow.linear(x, torch.zeros(2, 0, device=device), bias, activation="relu",
+                     residual=torch.ones(3, 2, device=device))
+    assert out.tolist() == [[2.0, 1.0]] * 3
+    assert cow.linear(torch.zeros(0, 8, device=device),
+                      torch.zeros(2, 8, device=device)).shape == (0, 2)
+    assert cow.linear(torch.zeros(2, 8, device=device),
+                      torch.zeros(0, 8, device=device)).shape == (2, 0)
+
+
+def test_more_than_four_gigabytes(device):
+    """Offsets of more than 32 bits in the output and in x."""
+
+    rows, inner, outer = 70001, 8, 32768
+    x = normal(rows, inner, dtype=torch.float16, device=device, seed=24)
+    w = normal(outer, inner, dtype=torch.float16, device=device, seed=25)
+    out = cow.linear(x, w)
+    for part in (slice(0, 3), slice(32767, 32770), slice(rows - 3, rows)):
+        assert torch.equal(out[part], cow.linear(x[part], w))
+    del out
+    far = torch.zeros(2100, 1 << 20, dtype=torch.float16, device=device)
+    far[:, :inner] = x[:2100]
+    assert torch.equal(cow.linear(far[:, :inner], w[:100]), cow.linear(x[:2100], w[:100]))
+
+
+def test_the_residual_may_be_written_over(device):
+    """At the C entry, where the output is the caller's."""
+
+    from copy_on_write_sdm_amd import _native as nat
+
+    for rows in (9, 100):
+        x = normal(rows, 64, dtype=torch.bfloat16, device=device, seed=26)
+        w = normal(128, 64, dtype=torch.bfloat16, device=device, seed=27)
+        r = normal(rows, 128, dtype=torch.bfloat16, device=device, seed=28)
+        want = cow.linear(x, w, residual=r)
+        a = nat.Linear(x.data_ptr(), w.data_ptr(), None, r.data_ptr(), r.data_ptr(), 64, 64, 128,
+                       rows, 64, 128, 2, 0)
+        assert nat.lib().cowsdm_linear(a, nat.stream_handle(device)) == 0
+        assert torch.equal(r, want)
