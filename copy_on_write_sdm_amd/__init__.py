@@ -54,6 +54,7 @@ from .pages import (
     release_page_tables,
 )
 from .kv_cache import PagedAttention, PagedKVCache
+from .projections import AttentionLayer, AttentionProjections, ResidualMLP
 from .controller import (
     ControllerDecodeGraph,
     ControllerStep,
@@ -65,6 +66,8 @@ from .controller import (
 )
 
 __all__ = [
+    "AttentionLayer",
+    "AttentionProjections",
     "ControllerDecodeGraph",
     "ControllerStep",
     "DecodeTrace",
@@ -80,6 +83,7 @@ __all__ = [
     "PagedAttention",
     "PagedKVCache",
     "PagedSlotMap",
+    "ResidualMLP",
     "SDMCopyOnWriteStep",
     "SDMStepInputs",
     "allocate_dense_cache",

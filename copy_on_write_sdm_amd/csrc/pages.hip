@@ -18,7 +18,7 @@
 namespace cowsdm_impl {
 
 constexpr int kPageThreads = 512;
-constexpr int kPageRequests = 4096;    // requests of a table, children of a fork
+constexpr int kPageRequests = 4096;    // children of a fork, named requests of a release
 constexpr int kPageChunk = 4096;       // numbers that a workgroup counts and places in order
 
 // Table entries and pages up to which one workgroup runs every phase.
@@ -216,21 +216,24 @@ struct ReleaseParams {
   int32_t page_shift;
 };
 
-// A request counts where it is named first.
-__device__ void release_plan(const ReleaseParams& p, int32_t* first) {
+// A request counts where it is named first.  That is found in LDS, or in the
+// new lengths' place where there are more requests.
+__device__ void release_plan(const ReleaseParams& p, int32_t* in_lds) {
   const int tid = static_cast<int>(threadIdx.x);
+  int32_t* const first = p.requests <= kPageRequests ? in_lds : p.lengths_out;
   for (int r = tid; r < p.requests; r += kPageThreads) first[r] = INT32_MAX;
-  __syncthreads();
+  next_phase();
   for (int i = tid; i < p.n; i += kPageThreads) {
     const int32_t r = p.named[i];
     if (r >= 0 && r < p.requests) atomicMin(first + r, i);
   }
-  __syncthreads();
+  next_phase();
   for (int i = tid; i < p.n; i += kPageThreads) {
     const int32_t r = p.named[i];
     const bool is = r >= 0 && r < p.requests && first[r] == i;
     p.held[i] = is ? pages_held(p.lengths[r], p.page_shift, p.columns) : 0;
   }
+  __syncthreads();
   for (int r = tid; r < p.requests; r += kPageThreads)
     p.lengths_out[r] = first[r] == INT32_MAX ? p.lengths[r] : 0;
 }
@@ -546,12 +549,13 @@ int32_t check_tables(int64_t requests, int64_t columns, int64_t pages, int64_t n
                      int64_t page_tokens, const char* where) {
   if (requests < 0 || columns < 0 || pages < 0 || n < 0)
     return fail(COWSDM_EARG, "%s: negative size", where);
-  if (requests > kPageRequests || n > kPageRequests)
-    return fail(COWSDM_ELIMIT, "%s: at most %d requests", where, kPageRequests);
+  if (n > kPageRequests)
+    return fail(COWSDM_ELIMIT, "%s: at most %d requests a call", where, kPageRequests);
+  if (requests > INT32_MAX) return fail(COWSDM_ELIMIT, "%s: too large", where);
   if (pages > INT32_MAX / page_tokens || columns > INT32_MAX / page_tokens)
     return fail(COWSDM_ELIMIT, "%s: more than 2^31 tokens", where);
   const int64_t rows = requests > n ? requests : n;
-  if (rows * columns > INT32_MAX - kPageChunk)
+  if (columns > 0 && rows > (INT32_MAX - kPageChunk) / columns)
     return fail(COWSDM_ELIMIT, "%s: 2^31 table entries or more", where);
   return 0;
 }

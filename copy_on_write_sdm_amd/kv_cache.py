@@ -16,9 +16,10 @@ from typing import Callable, Sequence
 
 import torch
 
-from .attention import (CODES, PAGE_TOKENS, PageTableStep, cache_width, cached_attention,
-                        extend_page_tables, prompt_attention, write_kv_cache)
-from . import _native as nat
+from .attention import (CODES, MAX_REQUESTS, PAGE_TOKENS, PageTableStep, cache_width,
+                        cached_attention, extend_page_tables, prompt_attention, write_kv_cache)
+from .head_rotation import HeadRotation, rotate_heads
+from .pages import (compact_page_tables, copy_pages, fork_page_tables, release_page_tables)
 
 
 class PagedKVCache:
@@ -27,7 +28,9 @@ class PagedKVCache:
     The requests are rows of ``page_tables`` and ``lengths``, in the order of
     the decode state's batch.  How many tokens each holds is known on the host
     as well, so that running out of pages or columns is refused before a
-    launch, without reading the device.  Calls on one cache must be
+    launch, without reading the device.  Requests that ``fork`` makes share
+    the whole pages of what they have in common; such pages are full, and a
+    request's new tokens go to pages of its own.  Calls on one cache must be
     stream-ordered."""
 
     def __init__(self, layers: int, heads: int, head_width: int, *, capacity: int, pages: int,
@@ -56,7 +59,13 @@ class PagedKVCache:
         self.lengths = torch.empty(0, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), pages, dtype=torch.int32, device=device)
+        self.page_shares = torch.zeros(pages, dtype=torch.int32, device=device)
         self._lengths: list[int] = []
+        # the requests' first pages that have been shared, by numbers of the
+        # host's own, and how many requests hold each
+        self._shared: list[tuple[int, ...]] = []
+        self._holders: dict[int, int] = {}
+        self._named = 0
         self._released: set[int] = set()
         self._free = pages
         self._before: tuple | None = None       # what the last extend may be taken back to
@@ -100,6 +109,7 @@ class PagedKVCache:
         lengths = torch.cat((self.lengths, self.lengths.new_zeros(requests)))
         self.page_tables, self.lengths = tables, lengths
         self._lengths = self._lengths + [0] * requests
+        self._shared = self._shared + [()] * requests
         self._before = None
         self._added.clear()
         return list(range(first, first + requests))
@@ -108,10 +118,12 @@ class PagedKVCache:
         """What ``extend`` and ``admit`` replace, none of it in place: a table's
         entries past the pages that its request holds are not read."""
 
-        return self.page_tables, self.lengths, self.free_count, self._lengths, self._free
+        return (self.page_tables, self.lengths, self.free_count, self._lengths, self._free,
+                self._shared)
 
     def _back_to(self, before: tuple) -> None:
-        self.page_tables, self.lengths, self.free_count, self._lengths, self._free = before
+        (self.page_tables, self.lengths, self.free_count, self._lengths, self._free,
+         self._shared) = before
         self._before = None
         self._added.clear()
 
@@ -171,9 +183,67 @@ class PagedKVCache:
                                 self.page_tables, self.lengths,
                                 longest=max(self._lengths, default=0), scale=scale)
 
+    def fork(self, requests: Sequence[int], tokens: int | Sequence[int] | None = None
+             ) -> list[int]:
+        """One more request for each named one, after the others: it holds its
+        first ``tokens`` tokens (one number for all, or one each; all that it
+        holds when None), in every layer.  A request may be named more than
+        once.  Whole pages are shared; the page in which the tokens end is
+        copied.  Returns the new requests' indices."""
+
+        named = [int(r) for r in requests]
+        if any(not 0 <= r < self.requests or r in self._released for r in named):
+            raise ValueError("forked request is invalid or inactive")
+        if tokens is None:
+            counts = [self._lengths[r] for r in named]
+        elif isinstance(tokens, int):
+            counts = [tokens] * len(named)
+        else:
+            counts = [int(n) for n in tokens]
+        if len(counts) != len(named) or any(not 0 <= n <= self._lengths[r]
+                                            for r, n in zip(named, counts)):
+            raise ValueError("forked tokens must be one count per request, at most what it holds")
+        page = self.page_tokens
+        need = sum(n % page > 0 for n in counts)
+        if need > self._free:
+            raise ValueError(f"KV cache pages are exhausted: {need} needed, {self._free} free")
+        if self.requests + len(named) > MAX_REQUESTS:
+            raise ValueError(f"page tables take at most {MAX_REQUESTS} requests")
+        first = self.requests
+        if not named:
+            return []
+        both = torch.tensor([named, counts], dtype=torch.int32, device=self.device)
+        fork = fork_page_tables(self.lengths, self.page_tables, self.page_shares,
+                                self.free_pages, self.free_count, both[0], both[1],
+                                page_tokens=page)
+        if need:
+            copy_pages(self.key_pages, self.key_scales, self.value_pages, self.value_scales,
+                       fork.sources, fork.targets)
+        tables = torch.cat((self.page_tables, fork.page_tables))
+        lengths = torch.cat((self.lengths, fork.lengths))
+        self.page_tables, self.lengths = tables, lengths
+        self.page_shares, self.free_count = fork.page_shares, fork.free_count
+        shared = list(self._shared)
+        for r, n in zip(named, counts):
+            whole = n // page
+            more = range(self._named, self._named + max(0, whole - len(shared[r])))
+            self._named += len(more)
+            self._holders.update((p, 1) for p in more)
+            shared[r] = shared[r] + tuple(more)
+            shared.append(shared[r][:whole])
+            for p in shared[-1]:
+                self._holders[p] += 1
+        self._shared = shared
+        self._lengths = self._lengths + counts
+        self._free -= need
+        self._before = None
+        self._added.clear()
+        return list(range(first, first + len(named)))
+
     def release(self, requests: Sequence[int]) -> int:
-        """The pages of finished requests go back to the pool; their rows stay
-        until ``compact``.  Returns the pages freed."""
+        """The pages of finished requests go back to the pool, but for those
+        that other requests share; their rows stay until ``compact``.  Returns
+        the pages freed."""
 
         named = [int(r) for r in requests]
         if (len(set(named)) != len(named) or any(not 0 <= r < self.requests for r in named)
@@ -182,15 +252,25 @@ class PagedKVCache:
         if not named:
             return 0
         rows = torch.tensor(named, dtype=torch.int32, device=self.device)
-        nat.check(nat.lib().cowsdm_pages_release(
-            self.lengths.data_ptr(), self.page_tables.data_ptr(), self.requests,
-            self.page_tables.shape[1], rows.data_ptr(), len(named), self.free_pages.data_ptr(),
-            self.free_pages.numel(), self.free_count.data_ptr(), self.page_tokens,
-            nat.stream_handle(self.device)), "cowsdm_pages_release")
-        freed = sum(self._pages(self._lengths[r]) for r in named)
+        # a launch takes so many; the pages of what comes first lie lowest
+        for part in rows.split(MAX_REQUESTS):
+            left = release_page_tables(self.lengths, self.page_tables, self.page_shares,
+                                       self.free_pages, self.free_count, part,
+                                       page_tokens=self.page_tokens)
+            self.lengths, self.page_shares, self.free_count = left
+        self.page_tables.index_fill_(0, rows.long(), -1)
+        freed = 0
+        for r in named:
+            freed += self._pages(self._lengths[r]) - len(self._shared[r])
+            for page in self._shared[r]:
+                self._holders[page] -= 1
+                if not self._holders[page]:
+                    del self._holders[page]
+                    freed += 1
         self._before = None
         for r in named:
             self._lengths[r] = 0
+        self._shared = [() if r in set(named) else s for r, s in enumerate(self._shared)]
         self._released |= set(named)
         self._free += freed
         return freed
@@ -206,9 +286,69 @@ class PagedKVCache:
             self.page_tables, self.lengths = tables, lengths
             self._before = None
             self._lengths = [self._lengths[r] for r in kept]
+            self._shared = [self._shared[r] for r in kept]
             self._released = set()
             self._added.clear()
         return kept
+
+    def trim_pages(self, *, headroom_pages: int = 0) -> int:
+        """The pool shrunk to the pages that requests hold plus headroom (one
+        page at least): the pages in use move to its lowest numbers first, in
+        every layer.  Returns the pages given up.  The pool's tensors are
+        replaced, which takes room for both meanwhile."""
+
+        if headroom_pages < 0:
+            raise ValueError("KV cache headroom cannot be negative")
+        pages = self.free_pages.numel()
+        used = pages - self._free
+        target = max(1, used + headroom_pages)
+        if target >= pages:
+            return 0
+        moves = compact_page_tables(self.lengths, self.page_tables, self.page_shares,
+                                    page_tokens=self.page_tokens)
+        most = min(used, pages - used)
+        copy_pages(self.key_pages, self.key_scales, self.value_pages, self.value_scales,
+                   moves.sources[:most], moves.targets[:most])
+        kept = [t[:, :target].contiguous() for t in (self.key_pages, self.key_scales,
+                                                     self.value_pages, self.value_scales)]
+        shares = moves.page_shares[:target].clone()
+        # the stack's numbers fall from the pool's last one on
+        stack = moves.free_pages[pages - target:].clone()
+        count = torch.full_like(self.free_count, target - used)
+        self.key_pages, self.key_scales, self.value_pages, self.value_scales = kept
+        self.page_tables, self.page_shares = moves.page_tables, shares
+        self.free_pages, self.free_count = stack, count
+        self._free = target - used
+        self._before = None
+        return pages - target
+
+    def grow_pages(self, pages: int) -> None:
+        """``pages`` more in the pool, which are taken after those that are
+        free now.  The pool's tensors are replaced, which takes room for both
+        meanwhile."""
+
+        if pages < 0:
+            raise ValueError("added KV cache pages cannot be negative")
+        if not pages:
+            return
+        before = self.free_pages.numel()
+
+        def grown(t: torch.Tensor, value: int) -> torch.Tensor:
+            bits = t.view(torch.uint8) if t.dtype is CODES else t
+            new = bits.new_full((t.shape[0], before + pages, *t.shape[2:]), value)
+            new[:, :before] = bits
+            return new.view(t.dtype)
+
+        pool = [grown(self.key_pages, 0), grown(self.key_scales, 1),
+                grown(self.value_pages, 0), grown(self.value_scales, 1)]
+        shares = torch.cat((self.page_shares, self.page_shares.new_zeros(pages)))
+        fresh = torch.arange(before + pages - 1, before - 1, -1, dtype=torch.int32,
+                             device=self.device)
+        stack, count = torch.cat((fresh, self.free_pages)), self.free_count + pages
+        self.key_pages, self.key_scales, self.value_pages, self.value_scales = pool
+        self.page_shares, self.free_pages, self.free_count = shares, stack, count
+        self._free += pages
+        self._before = None
 
     def storage_bytes(self) -> dict[str, int]:
         """Bytes of the codes, their scales and the tables, and of the codes and
@@ -221,7 +361,7 @@ class PagedKVCache:
         return {
             "kv_codes": codes,
             "kv_scales": scales,
-            "kv_tables": 4 * (self.page_tables.numel() + self.lengths.numel() + pages + 1),
+            "kv_tables": 4 * (self.page_tables.numel() + self.lengths.numel() + 2 * pages + 1),
             "kv_live": (codes + scales) // pages * used,
         }
 
@@ -243,6 +383,11 @@ class PagedAttention:
     * ``finish(layer, tokens [T, width], mixed [T, heads, D])`` -> the block's
       residual stream [T, width] (output projection, residual add, MLP).
 
+    ``AttentionProjections`` makes both of the layers' weights.  With
+    ``rotation`` or ``head_norms`` (for each of the layers the query's and the
+    key's norm weight, or None), queries and keys go from ``project`` through
+    ``rotate_heads`` at the tokens' positions, with ``norm_eps``.
+
     ``layers`` are the positions of the "A" layers in the layout, in the order
     in which they run.  A prefill admits its requests after those that the cache holds, as
     ``FaithfulSDMDecodeState.admit`` appends them to the batch; ``release`` and
@@ -259,11 +404,17 @@ class PagedAttention:
     theirs and stays."""
 
     def __init__(self, cache: PagedKVCache, layers: Sequence[int], project: Project,
-                 finish: Finish, *, scale: float | None = None):
+                 finish: Finish, *, scale: float | None = None,
+                 rotation: HeadRotation | None = None,
+                 head_norms: Sequence[tuple[torch.Tensor | None, torch.Tensor | None]] | None
+                 = None, norm_eps: float = 1e-6):
         self.cache, self.layers = cache, tuple(layers)
         if not self.layers or len(self.layers) > cache.layers:
             raise ValueError("the cache needs a layer for every attention layer")
+        if head_norms is not None and len(head_norms) != len(self.layers):
+            raise ValueError("head norms must be one pair per attention layer")
         self.project, self.finish, self.scale = project, finish, scale
+        self.rotation, self.head_norms, self.norm_eps = rotation, head_norms, norm_eps
         self._step: PageTableStep | None = None
         self._next = 0              # the layer of the step that runs next
         self._prompt = False
@@ -353,6 +504,15 @@ class PagedAttention:
 
     # ------------------------------------------------------------ the layers
 
+    def _projected(self, layer: int, index: int, rows: torch.Tensor, positions: torch.Tensor
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        query, key, value = self.project(layer, rows, positions)
+        if self.rotation is not None or self.head_norms is not None:
+            norms = (None, None) if self.head_norms is None else self.head_norms[index]
+            query, key = rotate_heads(query, key, positions, self.rotation, query_norm=norms[0],
+                                      key_norm=norms[1], eps=self.norm_eps)
+        return query, key, value
+
     @torch.no_grad()
     def prefill(self, layer: int, tokens: torch.Tensor):
         """``attention_block``: tokens [B, T, width] of B new requests."""
@@ -361,7 +521,7 @@ class PagedAttention:
         index, step = self._enter(layer, True, self._begin_prefill, batch, time)
         try:
             rows = tokens.reshape(batch * time, width)
-            query, key, value = self.project(layer, rows, step.positions)
+            query, key, value = self._projected(layer, index, rows, step.positions)
             self.cache.write(index, key, value, step.slots)
             mixed = prompt_attention(query, key, value, step.offsets, longest=time,
                                      scale=self.scale)
@@ -382,7 +542,7 @@ class PagedAttention:
         index, step = self._enter(layer, False, self._begin_decode, batch, position)
         try:
             rows = tokens.reshape(batch, width)
-            query, key, value = self.project(layer, rows, step.positions)
+            query, key, value = self._projected(layer, index, rows, step.positions)
             self.cache.write(index, key, value, step.slots)
             mixed = self.cache.attend(index, query.unsqueeze(1), scale=self.scale)
             out = self.finish(layer, rows, mixed.squeeze(1)).reshape(batch, 1, width)

@@ -87,8 +87,6 @@ def _check_tables(lengths: torch.Tensor, page_tables: torch.Tensor, page_shares:
     _int32(page_shares, pages, index, "page shares")
     if page_tokens not in PAGE_TOKENS:
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
-    if batch > MAX_REQUESTS:
-        raise ValueError(f"page tables take at most {MAX_REQUESTS} requests")
     return batch, columns, pages, index
 
 

@@ -907,7 +907,8 @@ int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
  * shared); pages that requests share are full.  Inputs stay as they are, but
  * for the free stack, which a release writes above its count: lengths, tables,
  * counts and shares come out new and are not the inputs themselves.  At most
- * 4,096 requests; page_tokens is 16, 32, 64, 128 or 256. */
+ * 4,096 requests are forked or released at once; page_tokens is 16, 32, 64,
+ * 128 or 256. */
 
 /* n new requests: child i holds the first tokens[i] tokens of request
  * parents[i].  Its whole pages are the parent's and get a sharer more each;

@@ -82,7 +82,7 @@ def assert_compact(device, lengths, state, page):
 SIZES = [([5], 16, 3), ([0], 64, 0), ([64, 0, 1, 63, 65, 128], 64, 9),
          ([(37 * i) % 300 for i in range(70)], 32, 90),
          ([(53 * i) % 2049 for i in range(600)], 32, 900),
-         ([70000, 5, 40001], 16, 20000)]
+         ([70000, 5, 40001], 16, 20000), ([(11 * i) % 40 for i in range(5000)], 16, 700)]
 
 
 @pytest.mark.parametrize("lengths,page,spare", SIZES)
@@ -106,13 +106,15 @@ def test_a_life(device, lengths, page, spare):
         lengths = list(lengths) + new
         state = np.concatenate((tables, rows)), shares, stack, count
         ref.check(lengths, *state, page)
-    named = rng.permutation(len(lengths))[:2 * len(lengths) // 3].tolist()
+    named = rng.permutation(len(lengths))[:min(4096, 2 * len(lengths) // 3)].tolist()
     lengths, state = assert_release(device, lengths, state, named, page)
     ref.check(lengths, *state, page)
     tables, shares, stack, count, *_ = assert_compact(device, lengths, state, page)
     state = tables, shares, stack, count
     ref.check(lengths, *state, page)
-    lengths, state = assert_release(device, lengths, state, list(range(len(lengths))), page)
+    for at in range(0, len(lengths), 4096):
+        rest = list(range(at, min(len(lengths), at + 4096)))
+        lengths, state = assert_release(device, lengths, state, rest, page)
     assert state[3] == len(state[1]) and not any(state[1])
 
 
