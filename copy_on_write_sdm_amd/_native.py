@@ -515,7 +515,8 @@ SIGNATURES: dict[str, tuple] = {
     "cowsdm_page_tables_compact": (
         _I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "cowsdm_pages_copy": (_I32, [ctypes.POINTER(KVCache), _I64, _P, _P, _I64, _P]),
-    "cowsdm_linear": (_I32, [ctypes.POINTER(Linear), _P]),
+    "cowsdm_linear_workspace_bytes": (_I64, [_I64, _I64, _I64, _I32]),
+    "cowsdm_linear": (_I32, [ctypes.POINTER(Linear), _P, _I64, _P]),
     "cowsdm_rotate_heads": (_I32, [ctypes.POINTER(RotateHeads), _P]),
     "cowsdm_product_key_routes": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P]),
 }

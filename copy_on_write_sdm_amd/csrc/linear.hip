@@ -25,6 +25,9 @@ struct LinearParams {
   int32_t outer;
   int32_t activation;
   int32_t wide;                    // epilogue rows move four elements at a time
+  int32_t splits;                  // of the summed axis; more than one: sums go to `parts`
+  int32_t chunk;                   // columns of a split
+  float* parts;                    // [splits][rows][outer rounded up to four]
 };
 
 // ------------------------------------------------------- matrix instructions
@@ -77,17 +80,17 @@ constexpr float kSqrtHalf = 0.70710678118654752f;
 
 // y Phi(y) for results of 16 bits: max(y, 0) - |y| erfc(|y| / sqrt 2) / 2 with
 // the rational approximation 7.1.26 of Abramowitz and Stegun, whose error is
-// at most 1.5e-7.  About a third of erff's instructions.
+// at most 1.5e-7.  About a third of erff's instructions.  From 14 on nothing
+// is left of erfc.
 __device__ __forceinline__ float gelu_short(float y) {
-  const float a = __builtin_fabsf(y);
+  const float a = fminf(__builtin_fabsf(y), 14.0f);
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3275911f * kSqrtHalf, 1.0f));
-  float s = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
-  s = __builtin_fmaf(s, t, 1.421413741f);
-  s = __builtin_fmaf(s, t, -0.284496736f);
-  s = __builtin_fmaf(s, t, 0.254829592f);
+  float s = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  s = __builtin_fmaf(s, t, 0.5f * 1.421413741f);
+  s = __builtin_fmaf(s, t, 0.5f * -0.284496736f);
+  s = __builtin_fmaf(s, t, 0.5f * 0.254829592f);
   const float e = exp2_fast(y * y * (-0.5f * kLog2E));
-  const float h = a < 14.0f ? 0.5f * a * s * t * e : 0.0f;    // 14: below the smallest number
-  return (y < 0.0f ? 0.0f : y) - h;
+  return fmaxf(y, 0.0f) - a * s * t * e;
 }
 
 // y / (1 + exp(-z))
@@ -130,30 +133,109 @@ __device__ __forceinline__ f32x4 load4(const T* p) {
   return __builtin_convertvector(*reinterpret_cast<const vec*>(p), f32x4);
 }
 
-// Four consecutive elements of an output row, from column n on.
+// Four consecutive elements of output row m, from column n on, where they do
+// not move together.
+template <typename T>
+__device__ __forceinline__ void finish_each(const LinearParams& p, int m, int n, f32x4 y) {
+  const T* const bias = static_cast<const T*>(p.bias);
+  const T* const residual = static_cast<const T*>(p.residual);
+  const int64_t from = m * p.residual_row + n;
+  T* const out = static_cast<T*>(p.out) + static_cast<int64_t>(m) * p.outer + n;
+  const int left = p.outer - n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (bias && i < left) y[i] += static_cast<float>(bias[n + i]);
+  y = activated<T>(y, p.activation);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left)
+      out[i] = static_cast<T>(residual ? static_cast<float>(residual[from + i]) + y[i] : y[i]);
+}
+
+// The same of any row and column: nothing past the last.
 template <typename T>
 __device__ __forceinline__ void finish4(const LinearParams& p, int m, int n, f32x4 y) {
   if (m >= p.rows || n >= p.outer) return;
-  const T* const bias = static_cast<const T*>(p.bias);
-  const T* const residual =
-      p.residual ? static_cast<const T*>(p.residual) + m * p.residual_row + n : nullptr;
-  T* const out = static_cast<T*>(p.out) + static_cast<int64_t>(m) * p.outer + n;
-  if (p.wide) {                    // the outer width is a multiple of four
-    if (p.bias) y += load4(bias + n);
-    y = activated<T>(y, p.activation);
-    if (residual) y = load4(residual) + y;
-    store4(out, y);
-  } else {
-    const int left = p.outer - n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (p.bias && i < left) y[i] += static_cast<float>(bias[n + i]);
-    y = activated<T>(y, p.activation);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left)
-        out[i] = static_cast<T>(residual ? static_cast<float>(residual[i]) + y[i] : y[i]);
+  if (!p.wide) {
+    finish_each<T>(p, m, n, y);
+    return;
   }
+  if (p.bias) y += load4(static_cast<const T*>(p.bias) + n);
+  y = activated<T>(y, p.activation);
+  if (p.residual) y = load4(static_cast<const T*>(p.residual) + m * p.residual_row + n) + y;
+  store4(static_cast<T*>(p.out) + static_cast<int64_t>(m) * p.outer + n, y);
+}
+
+// A wave's sums of 32 NT columns by 32 MT rows of the output, as the products
+// leave them, through LDS (32 rows of its own at a time), so that a store
+// writes whole rows of its columns.  Chunks of four are permuted against the
+// banks.  A lane keeps to four columns, whose bias it loads once.
+template <typename T, int NT, int MT>
+__device__ __forceinline__ void finish_tile(const LinearParams& p, const f32x16 (&acc)[NT][MT],
+                                            f32x4* turned, int m0, int n0, int split) {
+  constexpr int kChunks = NT * 8, kRows = kWave / kChunks;      // rows of a step
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int row = lane & 31, half = lane >> 5;
+  const int c = lane % kChunks, n = n0 + c * 4;
+  const bool in = n < p.outer;
+  f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (p.wide && p.bias && p.splits == 1 && in) bias = load4(static_cast<const T*>(p.bias) + n);
+#pragma unroll
+  for (int u = 0; u < MT; ++u) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        turned[row * kChunks + ((t * 8 + g * 2 + half) ^ (row & (kChunks - 1)))] =
+            f32x4{acc[t][u][4 * g], acc[t][u][4 * g + 1], acc[t][u][4 * g + 2],
+                  acc[t][u][4 * g + 3]};
+    const int first = m0 + u * 32;
+    auto at = [&](int r) { return turned[r * kChunks + (c ^ (r & (kChunks - 1)))]; };
+    if (p.splits > 1) {
+      const int64_t wide = (p.outer + 3) & ~3;
+      float* const to = p.parts + (static_cast<int64_t>(split) * p.rows) * wide + n;
+#pragma unroll 4
+      for (int r = lane / kChunks; r < 32; r += kRows)
+        if (in && first + r < p.rows) *reinterpret_cast<f32x4*>(to + (first + r) * wide) = at(r);
+    } else if (!p.wide) {
+#pragma unroll 1
+      for (int r = lane / kChunks; r < 32; r += kRows)
+        if (in && first + r < p.rows) finish_each<T>(p, first + r, n, at(r));
+    } else if (p.residual) {
+      const T* const residual = static_cast<const T*>(p.residual) + n;
+#pragma unroll 4
+      for (int r = lane / kChunks; r < 32; r += kRows) {
+        const int m = first + r;
+        if (!in || m >= p.rows) continue;
+        const f32x4 more = load4(residual + m * p.residual_row);
+        const f32x4 y = activated<T>(at(r) + bias, p.activation);
+        store4(static_cast<T*>(p.out) + static_cast<int64_t>(m) * p.outer + n, more + y);
+      }
+    } else {
+#pragma unroll 4
+      for (int r = lane / kChunks; r < 32; r += kRows) {
+        const int m = first + r;
+        const f32x4 y = activated<T>(at(r) + bias, p.activation);
+        if (in && m < p.rows)
+          store4(static_cast<T*>(p.out) + static_cast<int64_t>(m) * p.outer + n, y);
+      }
+    }
+  }
+}
+
+// The splits' sums, added in their order, and the epilogue.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p) {
+  const int wide = (p.outer + 3) & ~3, chunks = wide / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t each = static_cast<int64_t>(p.rows) * wide;
+  if (at * 4 >= each) return;
+  const int m = static_cast<int>(at / chunks), n = static_cast<int>(at - m * static_cast<int64_t>(chunks)) * 4;
+  const f32x4* const from = reinterpret_cast<const f32x4*>(p.parts) + at;
+  f32x4 y = from[0];
+#pragma unroll 4
+  for (int s = 1; s < p.splits; ++s) y += from[s * (each / 4)];
+  finish4<T>(p, m, n, y);
 }
 
 // -------------------------------------------------------------- many rows
@@ -166,121 +248,268 @@ constexpr uint32_t kNowhere = 0x80000000u;   // an offset past every buffer: rea
 // of lanes reads at once fall on different banks.
 __device__ __forceinline__ int line_chunk(int row, int slot) { return slot ^ ((row >> 1) & 7); }
 
-// This thread's chunks of R rows from `first` on, columns from k on; zeros
-// past the operand's rows and columns.
-template <typename T, int R, int kThreads, bool kAligned>
-__device__ __forceinline__ void stage(const T* first, int rows, int64_t stride, int inner, int k,
-                                      lds_char* to) {
-  constexpr int kEach = 16 / static_cast<int>(sizeof(T));
-  const int tid = static_cast<int>(threadIdx.x);
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-#pragma unroll
-  for (int i = 0; i < R * kLineChunks / kThreads; ++i) {
-    const int q = i * kThreads + tid, row = q / kLineChunks;
-    const int column = k + line_chunk(row, q % kLineChunks) * kEach;
-    if constexpr (kAligned) {
-      const int bytes = static_cast<int>(((rows - 1) * stride + inner) * sizeof(T));
-      const uint32_t from =
-          column < inner ? static_cast<uint32_t>((row * stride + column) * sizeof(T)) : kNowhere;
-      load_to_lds(first, bytes, from, to + (i * kThreads + wave * kWave) * 16);
-    } else {
-      T v[kEach];
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        v[j] = row < rows && column + j < inner ? first[row * stride + column + j]
-                                                : static_cast<T>(0.0f);
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(to + q * 16) =
-          __builtin_bit_cast(u32x4, v);
-    }
-  }
-}
-
 __device__ __forceinline__ u32x4 line_read(const lds_char* lines, int row, int chunk) {
   return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
       lines + row * kLineBytes + line_chunk(row, chunk) * 16);
 }
 
-// One workgroup: BM rows of x by BN rows of W; its waves share them as MW by
-// NW.  The next step's lines are on their way to LDS while this one's are
-// used.
-template <typename T, int BM, int BN, int MW, int NW, bool kAligned>
-__global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearParams p) {
-  constexpr int kThreads = MW * NW * kWave;
-  constexpr int MT = BM / MW / 32, NT = BN / NW / 32;     // a wave's tiles of 32 by 32
-  constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));   // columns a step
-  extern __shared__ __align__(16) char s_lines[];
-  lds_char* const lines = (lds_char*)s_lines;
-  constexpr int kBuffer = (BM + BN) * kLineBytes;
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
-  const int tiles_m = (p.rows + BM - 1) / BM;
-  const int tile_n = static_cast<int>(blockIdx.x) / tiles_m;
-  const int tile_m = static_cast<int>(blockIdx.x) - tile_n * tiles_m;
-  const int m0 = tile_m * BM, n0 = tile_n * BN;
-  const T* const x = static_cast<const T*>(p.x) + m0 * p.x_row;
-  const T* const w = static_cast<const T*>(p.weight) + n0 * p.weight_row;
-  const int x_rows = p.rows - m0 < BM ? p.rows - m0 : BM;
-  const int w_rows = p.outer - n0 < BN ? p.outer - n0 : BN;
-  const int wm = wave % MW * (BM / MW), wn = wave / MW * (BN / NW);
-  f32x16 acc[NT][MT];
+// R rows of an operand on their way to LDS, kThreads chunks at a time: where
+// this thread's lie.  A thread's chunks are in one place of their rows, as
+// kThreads is a multiple of 16 rows.
+template <typename T, int R, int kThreads>
+struct Lines {
+  static constexpr int kLoads = R * kLineChunks / kThreads;
+  static_assert(kThreads % (16 * kLineChunks) == 0 && R * kLineChunks % kThreads == 0);
+  const T* first;
+  int bytes;
+  uint32_t from[kLoads];
+
+  __device__ __forceinline__ Lines(const void* base, int64_t stride, int at, int rows, int inner) {
+    const int left = rows - at < R ? rows - at : R;
+    first = static_cast<const T*>(base) + at * stride;
+    bytes = static_cast<int>(((left - 1) * stride + inner) * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
-  for (int a = 0; a < NT; ++a)
-#pragma unroll
-    for (int b = 0; b < MT; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
-  auto load = [&](int k, int buffer) {
-    lds_char* const to = lines + buffer * kBuffer;
-    stage<T, BM, kThreads, kAligned>(x, x_rows, p.x_row, p.inner, k, to);
-    stage<T, BN, kThreads, kAligned>(w, w_rows, p.weight_row, p.inner, k, to + BM * kLineBytes);
-  };
-  load(0, 0);
-  const int row = lane & 31, half = lane >> 5;
-  for (int k = 0, buffer = 0; k < p.inner; k += kEach, buffer ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this thread's part has arrived
-    __syncthreads();
-    if (k + kEach < p.inner) load(k + kEach, buffer ^ 1);
-    const lds_char* const xs = lines + buffer * kBuffer;
-    const lds_char* const ws = xs + BM * kLineBytes;
-#pragma unroll
-    for (int s = 0; s < kLineChunks / 2; ++s) {
-      u32x4 a[NT], b[MT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) a[t] = line_read(ws, wn + t * 32 + row, 2 * s + half);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) b[t] = line_read(xs, wm + t * 32 + row, 2 * s + half);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < MT; ++u) acc[t][u] = Product<T>::wide(a[t], b[u], acc[t][u]);
+    for (int i = 0; i < kLoads; ++i) {
+      const int q = i * kThreads + static_cast<int>(threadIdx.x), row = q / kLineChunks;
+      from[i] = static_cast<uint32_t>(row * stride * static_cast<int64_t>(sizeof(T))) +
+                line_chunk(row, q % kLineChunks) * 16;
     }
   }
-  // Through LDS, 32 output rows of this wave at a time, so that a store writes
-  // whole rows of its columns; chunks of four are permuted against the banks.
-  constexpr int kChunks = NT * 8;
-  __syncthreads();
-  f32x4* const turned = reinterpret_cast<f32x4*>(s_lines) + wave * 32 * kChunks;
+  // The first column of this thread's chunks in a step.
+  static __device__ __forceinline__ int column() {
+    const int q = static_cast<int>(threadIdx.x);
+    return line_chunk(q / kLineChunks, q % kLineChunks) * (16 / static_cast<int>(sizeof(T)));
+  }
+  // Loads i to e - 1 of the step from column k on; zeros from column `end` on.
+  __device__ __forceinline__ void load(lds_char* to, int k, int end, int i = 0,
+                                       int e = kLoads) const {
+    const int wave =
+        __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const uint32_t at =
+        k + column() < end ? static_cast<uint32_t>(k * static_cast<int>(sizeof(T))) : kNowhere;
 #pragma unroll
-  for (int u = 0; u < MT; ++u) {
+    for (int n = 0; n < kLoads; ++n)
+      if (n >= i && n < e)
+        load_to_lds(first, bytes, from[n] + at, to + (n * kThreads + wave * kWave) * 16);
+  }
+};
+
+// Waits until at most `kLeft` of this wave's loads are out and its LDS reads
+// are in, and then for the workgroup's other waves.  (The builtin barrier
+// alone would let the compiler move memory accesses over it, and
+// __syncthreads waits for every load.)
+template <int kLeft>
+__device__ __forceinline__ void arrive() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | ((kLeft >> 4) << 14));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// A wave's operands of one product step, and the products.
+template <typename T, int NT, int MT>
+struct Operands {
+  u32x4 a[NT], b[MT];
+  __device__ __forceinline__ void read(const lds_char* ws, const lds_char* xs, int wn, int wm,
+                                       int s) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int row = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) a[t] = line_read(ws, wn + t * 32 + row, 2 * s + half);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) b[t] = line_read(xs, wm + t * 32 + row, 2 * s + half);
+  }
+  __device__ __forceinline__ void multiply(f32x16 (&acc)[NT][MT]) const {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        turned[row * kChunks + ((t * 8 + g * 2 + half) ^ (row & (kChunks - 1)))] =
-            f32x4{acc[t][u][4 * g], acc[t][u][4 * g + 1], acc[t][u][4 * g + 2],
-                  acc[t][u][4 * g + 3]};
-#pragma unroll 2
-    for (int r = lane / kChunks; r < 32; r += kWave / kChunks) {
-      const int c = lane % kChunks;
-      finish4<T>(p, m0 + wm + u * 32 + r, n0 + wn + c * 4,
-                 turned[r * kChunks + (c ^ (r & (kChunks - 1)))]);
-    }
+      for (int u = 0; u < MT; ++u) acc[t][u] = Product<T>::wide(a[t], b[u], acc[t][u]);
   }
+};
+
+template <int NT, int MT>
+__device__ __forceinline__ void clear(f32x16 (&acc)[NT][MT]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][u][i] = 0.0f;
+}
+
+constexpr int kSteps = kLineChunks / 2;      // product steps of a line
+
+// Workgroup n runs on XCD n % 8, each of which takes a run of tiles, four rows
+// of tiles at a time, so that what an XCD works on at once shares its L2.
+template <int BM, int BN>
+__device__ __forceinline__ void tile_place(const LinearParams& p, int groups, int& m0, int& n0) {
+  constexpr int kBand = 4;
+  const int tiles_m = (p.rows + BM - 1) / BM, tiles_n = (p.outer + BN - 1) / BN;
+  const int side = static_cast<int>(blockIdx.x) % 8, each = groups / 8, rest = groups % 8;
+  const int tile = side * each + (side < rest ? side : rest) + static_cast<int>(blockIdx.x) / 8;
+  const int band = tile / (kBand * tiles_n), in = tile - band * kBand * tiles_n;
+  const int left = tiles_m - band * kBand, high = left < kBand ? left : kBand;
+  const int column = in / high;
+  m0 = (band * kBand + in - column * high) * BM;
+  n0 = column * BN;
+}
+
+// One workgroup: 256 rows of x by 256 rows of W, its eight waves 128 by 64
+// each.  LDS holds five half tiles (a step's lines of x, or of W): two are
+// used, one and a half steps' are on their way.  When a step's lines have all
+// been read, W of two steps on takes the place of its x, and x of three steps
+// on that of its W.
+template <typename T>
+__global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
+  constexpr int B = 256, kThreads = 512, MT = 4, NT = 2;
+  constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));   // columns a step
+  constexpr int kSlot = B * kLineBytes, kSlots = 5;
+  constexpr int kLoads = Lines<T, B, kThreads>::kLoads;
+  extern __shared__ __align__(16) char s_lines[];
+  lds_char* const lines = (lds_char*)s_lines;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  int m0, n0;
+  tile_place<B, B>(p, gridDim.x, m0, n0);
+  const Lines<T, B, kThreads> x(p.x, p.x_row, m0, p.rows, p.inner);
+  const Lines<T, B, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
+  const int wm = wave % 2 * 128, wn = wave / 2 * 64;
+  f32x16 acc[NT][MT];
+  clear(acc);
+  x.load(lines, 0, p.inner);
+  w.load(lines + kSlot, 0, p.inner);
+  x.load(lines + 2 * kSlot, kEach, p.inner);
+  w.load(lines + 3 * kSlot, kEach, p.inner);
+  arrive<2 * kLoads>();
+  Operands<T, NT, MT> now[2];
+  int xs = 0, ws = 1, spare = 4;           // slots of this step's x and W, and of the last one's W
+  now[0].read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, 0);
+  for (int k = 0; k < p.inner; k += kEach) {
+    const int xn = xs + 2 < kSlots ? xs + 2 : xs + 2 - kSlots;
+    const int wx = ws + 2 < kSlots ? ws + 2 : ws + 2 - kSlots;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Operands<T, NT, MT>& next = now[(s + 1) & 1];
+      if (s < kSteps - 1) {
+        next.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, s + 1);
+        // not at once with W's, so that those come first
+        if (s == 0) x.load(lines + spare * kSlot, k + 2 * kEach, p.inner);
+      } else {
+        arrive<kLoads>();                  // all but x of two steps on
+        next.read(lines + wx * kSlot, lines + xn * kSlot, wn, wm, 0);
+        w.load(lines + xs * kSlot, k + 2 * kEach, p.inner);
+      }
+      now[s & 1].multiply(acc);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    spare = ws;
+    xs = xn;
+    ws = wx;
+  }
+  arrive<0>();
+  finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 8, m0 + wm, n0 + wn,
+                 0);
+}
+
+// One workgroup: BM rows of x by BN rows of W over a split of the summed axis;
+// its waves share them as MW by NW.  LDS holds the lines of kStages steps, all
+// but one of them on their way.
+template <typename T, int BM, int BN, int MW, int NW, int kStages>
+__global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearParams p) {
+  constexpr int kThreads = MW * NW * kWave;
+  constexpr int MT = BM / MW / 32, NT = BN / NW / 32;               // a wave's tiles of 32 by 32
+  constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));   // columns a step
+  constexpr int kStage = (BM + BN) * kLineBytes;
+  constexpr int kLoads = Lines<T, BM, kThreads>::kLoads + Lines<T, BN, kThreads>::kLoads;
+  extern __shared__ __align__(16) char s_lines[];
+  lds_char* const lines = (lds_char*)s_lines;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  int m0, n0;
+  tile_place<BM, BN>(p, gridDim.x, m0, n0);
+  const int begin = static_cast<int>(blockIdx.y) * p.chunk;
+  const int end = p.inner - begin < p.chunk ? p.inner : begin + p.chunk;
+  const Lines<T, BM, kThreads> x(p.x, p.x_row, m0, p.rows, p.inner);
+  const Lines<T, BN, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
+  const int wm = wave % MW * (BM / MW), wn = wave / MW * (BN / NW);
+  f32x16 acc[NT][MT];
+  clear(acc);
+  auto load = [&](int k, int stage) {
+    lds_char* const to = lines + stage * kStage;
+    x.load(to, k, end);
+    w.load(to + BM * kLineBytes, k, end);
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load(begin + s * kEach, s);
+  arrive<(kStages - 2) * kLoads>();
+  Operands<T, NT, MT> now[2];
+  now[0].read(lines + BM * kLineBytes, lines, wn, wm, 0);
+  int stage = 0;
+  for (int k = begin; k < end; k += kEach) {
+    const int into = stage == 0 ? kStages - 1 : stage - 1;
+    const int after = stage == kStages - 1 ? 0 : stage + 1;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if (s == 0) load(k + (kStages - 1) * kEach, into);
+      if (s == kSteps - 1) arrive<(kStages - 2) * kLoads>();
+      const lds_char* const from = lines + (s == kSteps - 1 ? after : stage) * kStage;
+      now[(s + 1) & 1].read(from + BM * kLineBytes, from, wn, wm, (s + 1) % kSteps);
+      now[s & 1].multiply(acc);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    stage = after;
+  }
+  arrive<0>();
+  finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 8, m0 + wm, n0 + wn,
+                 blockIdx.y);
+}
+
+// Operands that are not aligned: element by element into LDS, a step at a
+// time; 64 rows of each.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_odd_kernel(LinearParams p) {
+  constexpr int B = 64, kThreads = 256;
+  constexpr int kEach = 16 / static_cast<int>(sizeof(T));
+  __shared__ __align__(16) char s_lines[2 * B * kLineBytes];
+  lds_char* const xs = (lds_char*)s_lines;
+  lds_char* const ws = xs + B * kLineBytes;
+  const int tid = static_cast<int>(threadIdx.x);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  int m0, n0;
+  tile_place<B, B>(p, gridDim.x, m0, n0);
+  const int wm = wave % 2 * 32, wn = wave / 2 * 32;
+  f32x16 acc[1][1];
+  clear(acc);
+  auto stage = [&](const void* base, int64_t stride, int first, int rows, int k, lds_char* to) {
+#pragma unroll
+    for (int i = 0; i < B * kLineChunks / kThreads; ++i) {
+      const int q = i * kThreads + tid, row = q / kLineChunks;
+      const int column = k + line_chunk(row, q % kLineChunks) * kEach;
+      const T* const from = static_cast<const T*>(base) + (first + row) * stride + column;
+      T v[kEach];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        v[j] = first + row < rows && column + j < p.inner ? from[j] : static_cast<T>(0.0f);
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(to + q * 16) =
+          __builtin_bit_cast(u32x4, v);
+    }
+  };
+  for (int k = 0; k < p.inner; k += kLineChunks * kEach) {
+    stage(p.x, p.x_row, m0, p.rows, k, xs);
+    stage(p.weight, p.weight_row, n0, p.outer, k, ws);
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Operands<T, 1, 1> now;
+      now.read(ws, xs, wn, wm, s);
+      now.multiply(acc);
+    }
+    __syncthreads();
+  }
+  finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * 8, m0 + wm, n0 + wn, 0);
 }
 
 // --------------------------------------------------------------- few rows
-
-typedef __amdgpu_buffer_rsrc_t buffer_t;
 
 __device__ __forceinline__ u32x4 load_chunk(const void* first, int bytes, uint32_t from) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -293,112 +522,273 @@ __device__ __forceinline__ u32x4 load_chunk(const void* first, int bytes, uint32
 #endif
 }
 
-// One workgroup: 16 NT rows of W over all of the summed axis, which its waves
-// share, by 16 MT rows of x.  Every weight is read once, from memory into
-// registers; the waves' sums meet in LDS.
-template <typename T, int NT, int MT, int kWaves>
-__global__ __launch_bounds__(kWaves * kWave) void linear_few_kernel(LinearParams p) {
+// 16 R rows of an operand, from memory into registers: a lane's four rows'
+// worth of 16 bytes in a step.
+template <typename T, int R>
+struct FewRows {
+  const T* first;
+  int bytes;
+  uint32_t from[R];
+  __device__ __forceinline__ FewRows(const void* base, int64_t stride, int at, int rows,
+                                     int inner) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int left = rows - at < 16 * R ? rows - at : 16 * R;
+    first = static_cast<const T*>(base) + at * stride;
+    bytes = static_cast<int>(((left - 1) * stride + inner) * static_cast<int64_t>(sizeof(T)));
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+      from[t] = static_cast<uint32_t>((t * 16 + (lane & 15)) * stride *
+                                      static_cast<int64_t>(sizeof(T)));
+  }
+  __device__ __forceinline__ u32x4 load(int t, uint32_t at) const {
+    return load_chunk(first, bytes, from[t] + at);
+  }
+};
+
+constexpr int kFewWaves = 8;
+constexpr int kFewRows = 64;
+
+// One workgroup: 16 rows of W over all of the summed axis, which its waves
+// share two steps (128 bytes of a row) at a time, by all of x, 16 MT rows.
+// Every weight is read once, from memory into registers, the next ones while
+// these are used; the waves' sums meet in LDS.
+//
+// What a CU can have on its way bounds it: some 36 bytes a nanosecond, of W
+// and of x.  bfloat16, a row by 4096 x 6144: 12.7 us, 4.0 TB/s.
+template <typename T, int MT>
+__global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(LinearParams p) {
   constexpr int kEach = 16 / static_cast<int>(sizeof(T));   // columns a lane
-  constexpr int kStep = 4 * kEach;                          // columns a step
-  constexpr int kAhead = 4;                                 // steps whose loads go out together
-  __shared__ f32x4 s_sums[kWaves][NT * MT][kWave];
+  constexpr int kAhead = 2;                                 // steps whose loads go out together
+  constexpr int kSpan = kAhead * 4 * kEach;                 // columns of those
+  __shared__ f32x4 s_sums[kFewWaves][MT][kWave];
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
-  const int n0 = static_cast<int>(blockIdx.x) * 16 * NT;
-  const int m0 = static_cast<int>(blockIdx.y) * 16 * MT;
-  const T* const x = static_cast<const T*>(p.x) + m0 * p.x_row;
-  const T* const w = static_cast<const T*>(p.weight) + n0 * p.weight_row;
-  const int x_rows = p.rows - m0 < 16 * MT ? p.rows - m0 : 16 * MT;
-  const int w_rows = p.outer - n0 < 16 * NT ? p.outer - n0 : 16 * NT;
-  const int x_bytes = static_cast<int>(((x_rows - 1) * p.x_row + p.inner) * sizeof(T));
-  const int w_bytes = static_cast<int>(((w_rows - 1) * p.weight_row + p.inner) * sizeof(T));
+  const int n0 = static_cast<int>(blockIdx.x) * 16;
+  const FewRows<T, MT> x(p.x, p.x_row, 0, p.rows, p.inner);
+  const FewRows<T, 1> w(p.weight, p.weight_row, n0, p.outer, p.inner);
   const int row = lane & 15, quarter = lane >> 4;
-  f32x4 acc[NT][MT];
+  f32x4 acc[MT];
 #pragma unroll
-  for (int a = 0; a < NT; ++a)
-#pragma unroll
-    for (int b = 0; b < MT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = wave * kAhead * kStep; k < p.inner; k += kWaves * kAhead * kStep) {
-    u32x4 a[kAhead][NT], b[kAhead][MT];
+  for (int u = 0; u < MT; ++u) acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  struct Set {
+    u32x4 a[kAhead], b[kAhead][MT];
+  };
+  auto load = [&](Set& set, int k) {
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      const int column = k + s * kStep + quarter * kEach;
-      const bool in = column < p.inner;
+      const int column = k + (s * 4 + quarter) * kEach;
+      const uint32_t at = column < p.inner
+                              ? static_cast<uint32_t>(column * static_cast<int>(sizeof(T)))
+                              : kNowhere;
+      set.a[s] = w.load(0, at);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int64_t at = (t * 16 + row) * p.weight_row + column;
-        a[s][t] = load_chunk(w, w_bytes, in ? static_cast<uint32_t>(at * sizeof(T)) : kNowhere);
-      }
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int64_t at = (t * 16 + row) * p.x_row + column;
-        b[s][t] = load_chunk(x, x_bytes, in ? static_cast<uint32_t>(at * sizeof(T)) : kNowhere);
-      }
+      for (int u = 0; u < MT; ++u) set.b[s][u] = x.load(u, at);
     }
+  };
+  auto multiply = [&](const Set& set) {
 #pragma unroll
     for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < MT; ++u) acc[t][u] = Product<T>::narrow(a[s][t], b[s][u], acc[t][u]);
+      for (int u = 0; u < MT; ++u) acc[u] = Product<T>::narrow(set.a[s], set.b[s][u], acc[u]);
+  };
+  constexpr int kStride = kFewWaves * kSpan;
+  Set one, two;
+  load(one, wave * kSpan);
+  for (int k = wave * kSpan; k < p.inner; k += 2 * kStride) {
+    load(two, k + kStride);                  // past the end: zeros
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(one);
+    load(one, k + 2 * kStride);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(two);
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int u = 0; u < MT; ++u) s_sums[wave][t * MT + u][lane] = acc[t][u];
+  for (int u = 0; u < MT; ++u) s_sums[wave][u][lane] = acc[u];
   __syncthreads();
-  for (int j = wave; j < NT * MT; j += kWaves) {
-    f32x4 y = s_sums[0][j][lane];
+  if (wave < MT) {
+    f32x4 y = s_sums[0][wave][lane];
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) y += s_sums[v][j][lane];
-    const int t = j / MT, u = j - t * MT;
-    finish4<T>(p, m0 + u * 16 + row, n0 + t * 16 + quarter * 4, y);
+    for (int v = 1; v < kFewWaves; ++v) y += s_sums[v][wave][lane];
+    finish4<T>(p, wave * 16 + row, n0 + quarter * 4, y);
   }
 }
 
 // ----------------------------------------------------------------- launch
 
-template <typename T, int BM, int BN, int MW, int NW, bool kAligned>
-int32_t launch_tiles(const LinearParams& p, hipStream_t s) {
-  const int64_t groups = static_cast<int64_t>((p.rows + BM - 1) / BM) * ((p.outer + BN - 1) / BN);
-  constexpr int kThreads = MW * NW * kWave;
-  if (groups > UINT32_MAX / kThreads) return fail(COWSDM_ELIMIT, "linear: output too large");
-  constexpr int kBytes = 2 * (BM + BN) * kLineBytes;
-  auto* const kernel = linear_tile_kernel<T, BM, BN, MW, NW, kAligned>;
-  if constexpr (kBytes > 64 * 1024) {
+int32_t launch_groups(void (*kernel)(LinearParams), int64_t groups, int splits, int threads,
+                      int bytes, const LinearParams& p, hipStream_t s) {
+  // a launch counts its threads in 32 bits
+  if (groups > UINT32_MAX / threads) return fail(COWSDM_ELIMIT, "linear: output too large");
+  if (bytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess)
       return fail(static_cast<int32_t>(e), "linear: %s", hipGetErrorString(e));
   }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), kBytes, s, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups), static_cast<uint32_t>(splits)),
+                     dim3(threads), bytes, s, p);
   return launch_status("linear");
 }
 
-template <typename T, int NT, int MT, int kWaves>
+constexpr int64_t tiles_of(int64_t rows, int64_t outer, int bm, int bn) {
+  return ((rows + bm - 1) / bm) * ((outer + bn - 1) / bn);
+}
+
+enum class LinearForm { kFew, k64, k64x128, k128, k256 };
+struct LinearPlan {
+  LinearForm form;
+  int splits;
+};
+
+LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size);
+
+template <typename T, int BM, int BN, int MW, int NW, int kStages>
+int32_t launch_tiles(const LinearParams& p, hipStream_t s) {
+  constexpr int kLines = kStages * (BM + BN) * kLineBytes;
+  constexpr int kTurned = MW * NW * 32 * (BN / NW) * 4;
+  return launch_groups(&linear_tile_kernel<T, BM, BN, MW, NW, kStages>,
+                       tiles_of(p.rows, p.outer, BM, BN), p.splits, MW * NW * kWave,
+                       kLines > kTurned ? kLines : kTurned, p, s);
+}
+
+template <typename T, int MT>
 int32_t launch_few(const LinearParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((linear_few_kernel<T, NT, MT, kWaves>),
-                     dim3((p.outer + 16 * NT - 1) / (16 * NT), (p.rows + 16 * MT - 1) / (16 * MT)),
-                     dim3(kWaves * kWave), 0, s, p);
-  return launch_status("linear");
+  return launch_groups(&linear_few_kernel<T, MT>, (p.outer + 15) / 16, 1, kFewWaves * kWave, 0, p,
+                       s);
 }
 
 template <typename T>
-int32_t launch_linear(const LinearParams& p, bool aligned, hipStream_t s) {
-  if (!aligned) return launch_tiles<T, 64, 64, 2, 2, false>(p, s);
-  if (p.rows <= 16) return launch_few<T, 1, 1, 8>(p, s);
-  if (p.rows <= 32) return launch_few<T, 2, 2, 8>(p, s);
-  if (p.rows <= 64) return launch_few<T, 2, 4, 8>(p, s);
-  const int64_t large = static_cast<int64_t>((p.rows + 255) / 256) * ((p.outer + 255) / 256);
-  if (sizeof(T) == 2 && large >= 256) return launch_tiles<T, 256, 256, 2, 4, true>(p, s);
-  return launch_tiles<T, 128, 128, 2, 2, true>(p, s);
+int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipStream_t s) {
+  p.splits = 1;
+  p.chunk = p.inner;
+  if (!aligned)
+    return launch_groups(&linear_odd_kernel<T>, tiles_of(p.rows, p.outer, 64, 64), 1, 256, 0, p,
+                         s);
+  if (plan.splits > 1) {
+    constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));
+    const int steps = (p.inner + kEach - 1) / kEach;
+    p.splits = plan.splits;
+    p.chunk = (steps + plan.splits - 1) / plan.splits * kEach;
+  }
+  int32_t e = 0;
+  switch (plan.form) {
+    case LinearForm::kFew:
+      if (p.rows <= 16) return launch_few<T, 1>(p, s);
+      if (p.rows <= 32) return launch_few<T, 2>(p, s);
+      return launch_few<T, 4>(p, s);
+    case LinearForm::k64: e = launch_tiles<T, 64, 64, 2, 2, 4>(p, s); break;
+    case LinearForm::k64x128: e = launch_tiles<T, 64, 128, 2, 2, 4>(p, s); break;
+    case LinearForm::k128: e = launch_tiles<T, 128, 128, 2, 2, 4>(p, s); break;
+    case LinearForm::k256:
+      e = launch_groups(&linear_large_kernel<T>, tiles_of(p.rows, p.outer, 256, 256), 1, 512,
+                        5 * 256 * kLineBytes, p, s);
+      break;
+  }
+  if (e || p.splits == 1) return e;
+  const int64_t chunks = static_cast<int64_t>(p.rows) * ((p.outer + 3) / 4);
+  return launch_groups(&linear_join_kernel<T>, (chunks + 255) / 256, 1, 256, 0, p, s);
+}
+
+// What a form takes of a call's sizes, in microseconds: rounds of workgroups,
+// each so long a step of 128 bytes and so long at its ends, or the memory's
+// time, and, where the summed axis is split, the join's launch and traffic.
+// The least one runs.  The constants are fitted to calls on one MI355X, which
+// they give within some 20 %; in bfloat16, by the forms (splits):
+//   64 rows, 128 x 384: few 3.2, tiles of 64 3.8; 32 rows, 8192 x 512: few 23,
+//   64 (16) 9.6; a row, 4096 x 6144: few 12.7, 64 x 128 (5) 12.5; 64 rows: few
+//   38, 64 (2) 15.3, 64 x 128 (4) 15.0, 64 x 128 (1) 24
+//   100 rows, 4000 x 100: 64 (16) 7.4, 64 (1) 19
+//   1,111 rows, 2304 x 1544: 64 17.8, 64 x 128 17.0, 128 23, 256 44
+//   2,048 rows, 2048 x 2048: 64 31, 64 x 128 30, 128 24, 256 42
+//   4,096 rows, 4096 x 4096: 64 216, 64 x 128 200, 128 162, 256 108
+// and in float32 4,000 rows, 4000 x 4000: 1176, 1077, 1013, 911.
+struct FormCost {
+  LinearForm form;
+  int rows, columns;               // of a tile
+  float step[2], ends;             // of 16-bit types, and of float32
+};
+constexpr FormCost kFormCosts[] = {
+    {LinearForm::k64, 64, 64, {0.30f, 0.57f}, 1.0f},
+    {LinearForm::k64x128, 64, 128, {0.38f, 1.05f}, 1.0f},
+    {LinearForm::k128, 128, 128, {0.58f, 2.0f}, 2.5f},
+    {LinearForm::k256, 256, 256, {1.58f, 7.2f}, 4.0f},
+};
+constexpr int64_t kChipCus = 256;
+constexpr int kMostSplits = 16;
+
+LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size) {
+  const float memory =
+      static_cast<float>((rows * inner + inner * outer + rows * outer) * size) * (1.0f / 5.0e6f);
+  LinearPlan best{LinearForm::k128, 1};
+  float least = 3.0e38f;
+  auto consider = [&](LinearForm form, int splits, float us) {
+    if (us < least) {
+      least = us;
+      best = {form, splits};
+    }
+  };
+  if (rows <= kFewRows) {
+    const int64_t rounds = ((outer + 15) / 16 + kChipCus - 1) / kChipCus;
+    const float us = static_cast<float>(rounds * (16 + rows) * inner * size) * (1.0f / 36.0e3f);
+    consider(LinearForm::kFew, 1, 2.3f + (us > memory ? us : memory));
+  }
+  const int64_t steps = (inner * size + kLineBytes - 1) / kLineBytes;
+  for (const FormCost& f : kFormCosts) {
+    const int64_t tiles = tiles_of(rows, outer, f.rows, f.columns);
+    // the largest tiles' kernel does not split
+    const int most = f.form == LinearForm::k256 || tiles >= kChipCus ? 1 : kMostSplits;
+    for (int splits = 1; splits <= most && splits <= steps; ++splits) {
+      const int64_t groups = tiles * splits, each = (steps + splits - 1) / splits;
+      float step = f.step[size == 4];
+      int64_t rounds = (groups + kChipCus - 1) / kChipCus;
+      if (f.form == LinearForm::k64 && size == 2 && rounds > 1) {   // two a CU
+        rounds = (rounds + 1) / 2;
+        step = 0.45f;
+      }
+      const float us = static_cast<float>(rounds) * (static_cast<float>(each) * step + f.ends);
+      const float join =
+          splits == 1 ? 0.0f
+                      : 3.0f + static_cast<float>(8 * splits * rows * outer) * (1.0f / 4.5e6f);
+      consider(f.form, splits, 2.0f + (us > memory ? us : memory) + join);
+    }
+  }
+  // no split is left without columns
+  if (best.splits > 1) {
+    const int64_t each = (steps + best.splits - 1) / best.splits;
+    best.splits = static_cast<int>((steps + each - 1) / each);
+  }
+  return best;
 }
 
 }  // namespace cowsdm_impl
 
 using namespace cowsdm_impl;
 
-extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* stream) {
+namespace {
+
+int64_t workspace_of(const LinearPlan& plan, int64_t rows, int64_t outer) {
+  return plan.splits == 1 ? 0 : plan.splits * rows * ((outer + 3) / 4 * 16);
+}
+
+// 16-byte loads of both operands
+bool linear_aligned(const cowsdm_linear_t& l) {
+  const int64_t unit = l.float_type == COWSDM_FLOAT32 ? 4 : 8;
+  return (reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.weight)) % 16 == 0 &&
+         l.inner % unit == 0 && l.x_row % unit == 0 && l.weight_row % unit == 0;
+}
+
+}  // namespace
+
+extern "C" int64_t cowsdm_linear_workspace_bytes(int64_t rows, int64_t inner, int64_t outer,
+                                                 int32_t float_type) {
+  if (rows < 0 || inner < 0 || outer < 0 || rows > INT32_MAX || outer > INT32_MAX) return -1;
+  if (rows == 0 || outer == 0) return 0;
+  const LinearPlan plan = plan_linear(rows, inner, outer, float_type == COWSDM_FLOAT32 ? 4 : 2);
+  return workspace_of(plan, rows, outer);
+}
+
+extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
   if (!linear) return fail(COWSDM_EARG, "linear: null argument");
   const cowsdm_linear_t& l = *linear;
   if (l.rows < 0 || l.inner < 0 || l.outer < 0) return fail(COWSDM_EARG, "linear: negative size");
@@ -418,18 +808,37 @@ extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* stream) {
   if (l.rows == 0 || l.outer == 0) return 0;
   if (!l.out || (l.inner > 0 && (!l.x || !l.weight)))
     return fail(COWSDM_EARG, "linear: null pointer argument");
-  const int64_t unit = l.float_type == COWSDM_FLOAT32 ? 4 : 8;
-  const int64_t size = 16 / unit;
+  const int64_t size = l.float_type == COWSDM_FLOAT32 ? 4 : 2;
   auto address = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-  const bool aligned = (address(l.x) | address(l.weight)) % 16 == 0 && l.inner % unit == 0 &&
-                       l.x_row % unit == 0 && l.weight_row % unit == 0;
   const bool wide = l.outer % 4 == 0 && l.residual_row % 4 == 0 &&
                     (address(l.out) | address(l.bias) | address(l.residual)) % (4 * size) == 0;
-  LinearParams p{l.x, l.weight, l.bias, l.residual, l.out, l.x_row, l.weight_row,
-                 l.residual_row, static_cast<int32_t>(l.rows), static_cast<int32_t>(l.inner),
-                 static_cast<int32_t>(l.outer), l.activation, wide};
+  const bool aligned = linear_aligned(l);
+  const LinearPlan plan = plan_linear(l.rows, l.inner, l.outer, static_cast<int>(size));
+  if (aligned && plan.splits > 1) {
+    const int64_t need = workspace_of(plan, l.rows, l.outer);
+    if (!workspace || workspace_bytes < need)
+      return fail(COWSDM_EARG, "linear: workspace of %lld bytes needed",
+                  static_cast<long long>(need));
+    if (address(workspace) % 16)
+      return fail(COWSDM_EARG, "linear: the workspace must be 16-byte aligned");
+  }
+  LinearParams p{};
+  p.x = l.x;
+  p.weight = l.weight;
+  p.bias = l.bias;
+  p.residual = l.residual;
+  p.out = l.out;
+  p.x_row = l.x_row;
+  p.weight_row = l.weight_row;
+  p.residual_row = l.residual_row;
+  p.rows = static_cast<int32_t>(l.rows);
+  p.inner = static_cast<int32_t>(l.inner);
+  p.outer = static_cast<int32_t>(l.outer);
+  p.activation = l.activation;
+  p.wide = wide;
+  p.parts = static_cast<float*>(workspace);
   const auto s = static_cast<hipStream_t>(stream);
-  if (l.float_type == COWSDM_FLOAT32) return launch_linear<float>(p, aligned, s);
-  if (l.float_type == COWSDM_FLOAT16) return launch_linear<_Float16>(p, aligned, s);
-  return launch_linear<__bf16>(p, aligned, s);
+  if (l.float_type == COWSDM_FLOAT32) return launch_linear<float>(p, aligned, plan, s);
+  if (l.float_type == COWSDM_FLOAT16) return launch_linear<_Float16>(p, aligned, plan, s);
+  return launch_linear<__bf16>(p, aligned, plan, s);
 }

@@ -81,7 +81,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     a = nat.Linear(x.data_ptr(), weight.data_ptr(), nat.ptr(bias), nat.ptr(residual),
                    out.data_ptr(), x_row, weight_row, residual_row, rows, inner, outer, float_type,
                    code)
-    rc = nat.lib().cowsdm_linear(a, nat.stream_handle(device))
+    lib = nat.lib()
+    need = lib.cowsdm_linear_workspace_bytes(rows, inner, outer, float_type)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    rc = lib.cowsdm_linear(a, nat.ptr(workspace), need, nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_linear")
     return out

@@ -992,9 +992,15 @@ typedef struct cowsdm_linear {
   int32_t activation;
 } cowsdm_linear_t;
 
+/* Bytes of workspace that a call of cowsdm_linear needs (0: none), 16-byte
+ * aligned. */
+int64_t cowsdm_linear_workspace_bytes(int64_t rows, int64_t inner, int64_t outer,
+                                      int32_t float_type);
+
 /* Runs cowsdm_linear_t; COWSDM_ELIMIT for rows of more than
  * COWSDM_LINEAR_MOST elements. */
-int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* stream);
+int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace, int64_t workspace_bytes,
+                      void* stream);
 
 /* Heads normed and rotated by position: of every row x [width] of query
  * [rows, heads, width] and key [rows, kv_heads, width]

@@ -65,9 +65,44 @@ def test_sizes(device, dtype, rows, inner, outer):
 def test_large_tiles(device, dtype):
     """More than one workgroup of the largest tiles a CU, with odd ends."""
 
-    x = normal(4099, 200, dtype=dtype, device=device, seed=5)
-    w = normal(4102, 200, dtype=dtype, device=device, seed=6, scale=0.1)
-    assert_linear(x, w, normal(4102, dtype=dtype, device=device, seed=7), "silu")
+    assert_large(device, dtype, 4099, 200, 4102)
+
+
+@pytest.mark.parametrize("inner", [8, 64, 72, 128, 136, 320, 328, 512, 1032])
+def test_large_tiles_of_few_steps(device, inner):
+    """The ring of half tiles from one step on, whole and with an end."""
+
+    assert_large(device, torch.bfloat16, 2500, inner, 8196)
+
+
+def assert_large(device, dtype, rows, inner, outer):
+    x = normal(rows, inner, dtype=dtype, device=device, seed=5)
+    w = normal(outer, inner, dtype=dtype, device=device, seed=6, scale=0.1)
+    assert_linear(x, w, normal(outer, dtype=dtype, device=device, seed=7), "silu")
+
+
+def workspace(rows, inner, outer, dtype):
+    from copy_on_write_sdm_amd import _native as nat
+
+    return nat.lib().cowsdm_linear_workspace_bytes(rows, inner, outer, nat.FLOAT_TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,inner,outer", [
+    (100, 4000, 100), (20, 8192, 515), (70, 2056, 66), (128, 8192, 512), (64, 4096, 1024),
+    (256, 2568, 256), (1, 16384, 64), (65, 1096, 1)])
+def test_splits_of_the_summed_axis(device, dtype, rows, inner, outer):
+    """Sums joined in a workspace: of aligned and of odd widths, with the
+    epilogue in the join."""
+
+    assert workspace(rows, inner, outer, dtype) > 0
+    x = normal(rows, inner, dtype=dtype, device=device, seed=30)
+    w = normal(outer, inner, dtype=dtype, device=device, seed=31, scale=inner ** -0.5)
+    out = assert_linear(x, w, normal(outer, dtype=dtype, device=device, seed=32), "gelu_tanh",
+                        normal(rows, outer, dtype=dtype, device=device, seed=33))
+    assert torch.equal(out, cow.linear(
+        x, w, normal(outer, dtype=dtype, device=device, seed=32), activation="gelu_tanh",
+        residual=normal(rows, outer, dtype=dtype, device=device, seed=33)))
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
@@ -179,5 +214,5 @@ def test_the_residual_may_be_written_over(device):
         want = cow.linear(x, w, residual=r)
         a = nat.Linear(x.data_ptr(), w.data_ptr(), None, r.data_ptr(), r.data_ptr(), 64, 64, 128,
                        rows, 64, 128, 2, 0)
-        assert nat.lib().cowsdm_linear(a, nat.stream_handle(device)) == 0
+        assert nat.lib().cowsdm_linear(a, None, 0, nat.stream_handle(device)) == 0
         assert torch.equal(r, want)

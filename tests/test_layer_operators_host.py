@@ -184,8 +184,9 @@ def test_c_entries_refuse_without_launching():
             setattr(struct, field, kept)
 
     a = nat.Linear(FAKE, FAKE, None, None, FAKE, 16, 16, 0, 3, 16, 8, 0, 0)
-    assert lib.cowsdm_linear(None, None) == -1
-    each(lib.cowsdm_linear, a, (
+    run = lambda a, stream: lib.cowsdm_linear(a, None, 0, stream)     # noqa: E731
+    assert run(None, None) == -1
+    each(run, a, (
         ("rows", -1, -1, b"negative size"), ("inner", -1, -1, b"negative size"),
         ("float_type", 3, -1, b"float type"), ("activation", 5, -1, b"activation"),
         ("activation", -1, -1, b"activation"), ("x_row", -16, -1, b"negative stride"),
@@ -193,7 +194,10 @@ def test_c_entries_refuse_without_launching():
         ("rows", 1 << 31, -2, b"too large"), ("outer", 1 << 31, -2, b"too large"),
         ("x", None, -1, b"null"), ("weight", None, -1, b"null"), ("out", None, -1, b"null")))
     a.rows = 0
-    assert lib.cowsdm_linear(a, None) == 0
+    assert run(a, None) == 0
+    size = lib.cowsdm_linear_workspace_bytes
+    assert size(0, 16, 16, 0) == 0 and size(64, 128, 384, 0) == 0 and size(-1, 16, 16, 0) == -1
+    assert size(1 << 31, 16, 16, 0) == -1 and size(16, 16, 1 << 31, 0) == -1
 
     h = nat.RotateHeads(FAKE, FAKE, 128, 32, 64, 32, FAKE, FAKE, None, None, FAKE, FAKE, 3, 4, 2,
                         32, 32, 0, 0, 1e-6)
