@@ -5,7 +5,7 @@
 // both are read 16 bytes at a time and nothing is transposed.  Products are
 // computed as W x^T, so that a lane ends with consecutive elements of one
 // output row.  Sums, bias, activation and residual are in 32 bits, rounded
-// once.
+// once.  Float32 numbers go through the matrix cores as three of bfloat16.
 
 #include <type_traits>
 
@@ -198,9 +198,26 @@ __device__ __forceinline__ void finish_tile(const LinearParams& p, const f32x16 
       for (int r = lane / kChunks; r < 32; r += kRows)
         if (in && first + r < p.rows) *reinterpret_cast<f32x4*>(to + (first + r) * wide) = at(r);
     } else if (!p.wide) {
-#pragma unroll 1
-      for (int r = lane / kChunks; r < 32; r += kRows)
-        if (in && first + r < p.rows) finish_each<T>(p, first + r, n, at(r));
+      // a column a lane, so that a store still writes what lies together
+      constexpr int kWide = NT * 32;
+      const int d = lane % kWide, column = n0 + d;
+      if (column < p.outer) {
+        const float own =
+            p.bias ? static_cast<float>(static_cast<const T*>(p.bias)[column]) : 0.0f;
+        const T* const residual = static_cast<const T*>(p.residual) + column;
+        T* const out = static_cast<T*>(p.out) + column;
+#pragma unroll 4
+        for (int r = lane / kWide; r < 32; r += kWave / kWide) {
+          const int m = first + r;
+          if (m >= p.rows) continue;
+          float more = 0.0f;
+          if (p.residual) more = static_cast<float>(residual[m * p.residual_row]);
+          const float sum =
+              turned[r * kChunks + ((d / 4) ^ (r & (kChunks - 1)))][d % 4] + own;
+          const float y = activated<T>(f32x4{sum, 0.0f, 0.0f, 0.0f}, p.activation)[0];
+          out[static_cast<int64_t>(m) * p.outer] = static_cast<T>(p.residual ? more + y : y);
+        }
+      }
     } else if (p.residual) {
       const T* const residual = static_cast<const T*>(p.residual) + n;
 #pragma unroll 4
@@ -230,7 +247,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t each = static_cast<int64_t>(p.rows) * wide;
   if (at * 4 >= each) return;
-  const int m = static_cast<int>(at / chunks), n = static_cast<int>(at - m * static_cast<int64_t>(chunks)) * 4;
+  const int m = static_cast<int>(at / chunks);
+  const int n = static_cast<int>(at - m * static_cast<int64_t>(chunks)) * 4;
   const f32x4* const from = reinterpret_cast<const f32x4*>(p.parts) + at;
   f32x4 y = from[0];
 #pragma unroll 4
@@ -329,6 +347,114 @@ struct Operands {
   }
 };
 
+// The same of float32: half a line's numbers, eight a lane of each row.
+template <int NT, int MT>
+struct FloatOperands {
+  u32x4 a[NT][2], b[MT][2];
+  __device__ __forceinline__ void read(const lds_char* ws, const lds_char* xs, int wn, int wm,
+                                       int j) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int row = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        a[t][c] = line_read(ws, wn + t * 32 + row, 4 * j + 2 * c + half);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        b[t][c] = line_read(xs, wm + t * 32 + row, 4 * j + 2 * c + half);
+    }
+  }
+  // By float32 products.
+  __device__ __forceinline__ void multiply(f32x16 (&acc)[NT][MT]) const {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+          acc[t][u] = Product<float>::wide(a[t][c], b[u][c], acc[t][u]);
+  }
+};
+
+// A float32 number as the sum of three of bfloat16, whose products the matrix
+// cores do at sixteen times float32's rate.  Of the nine products of two
+// numbers the six that count are taken, smallest first; what is left out is
+// within 2^-23 of the product (a third is within 2^-8 of the one before).  A
+// number that is not finite, or within 2^-9 of the largest, gives NaN this
+// way: such sums are done again by float32 products.  4,000 rows by 4000 x
+// 4000, tiles of 256: 627 us, and 911 by float32 products; 2,048 by 2048 x
+// 2048, tiles of 128: 96 and 135.
+//
+// Pairs are rounded together, and a third is taken off as it stands in the
+// upper half of a word.
+__device__ __forceinline__ void to_thirds(const u32x4 (&v)[2], u32x4 (&out)[3]) {
+  typedef float pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    pair rest = {__uint_as_float(v[i / 2][i % 2 * 2]), __uint_as_float(v[i / 2][i % 2 * 2 + 1])};
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      const uint32_t part = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, bf16x2));
+      out[n][i] = part;
+      if (n < 2) {
+        rest[0] -= __uint_as_float(part << 16);
+        rest[1] -= __uint_as_float(part & 0xffff0000u);
+      }
+    }
+  }
+}
+
+// One row of W's thirds by one of x's.
+__device__ __forceinline__ f32x16 thirds_product(const u32x4 (&p)[3], const u32x4 (&q)[3],
+                                                 f32x16 c) {
+  constexpr int kLeft[6] = {2, 0, 1, 1, 0, 0}, kRight[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) c = Product<__bf16>::wide(p[kLeft[i]], q[kRight[i]], c);
+  return c;
+}
+
+template <int NT, int MT>
+struct Thirds {
+  u32x4 a[NT][3], b[MT][3];
+  __device__ __forceinline__ void take(const FloatOperands<NT, MT>& raw) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) to_thirds(raw.a[t], a[t]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) to_thirds(raw.b[t], b[t]);
+  }
+  __device__ __forceinline__ void multiply(f32x16 (&acc)[NT][MT]) const {
+    constexpr int kLeft[6] = {2, 0, 1, 1, 0, 0}, kRight[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int i = 0; i < 6; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+          acc[t][u] = Product<__bf16>::wide(a[t][kLeft[i]], b[u][kRight[i]], acc[t][u]);
+  }
+};
+
+// Whether a sum of the workgroup's is not finite; by way of a word of the LDS
+// that its lines have left.
+template <int NT, int MT>
+__device__ __forceinline__ bool any_not_finite(const f32x16 (&acc)[NT][MT], int* word) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[t][u][i], 0.0f, sum);
+  if (threadIdx.x == 0) *word = 0;
+  __syncthreads();
+  if (sum != 0.0f) *word = 1;
+  __syncthreads();
+  const bool any = *word != 0;
+  __syncthreads();
+  return any;
+}
+
 template <int NT, int MT>
 __device__ __forceinline__ void clear(f32x16 (&acc)[NT][MT]) {
 #pragma unroll
@@ -372,44 +498,86 @@ __global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   int m0, n0;
   tile_place<B, B>(p, gridDim.x, m0, n0);
+  const int begin = static_cast<int>(blockIdx.y) * p.chunk;
+  const int end = p.inner - begin < p.chunk ? p.inner : begin + p.chunk;
   const Lines<T, B, kThreads> x(p.x, p.x_row, m0, p.rows, p.inner);
   const Lines<T, B, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
   const int wm = wave % 2 * 128, wn = wave / 2 * 64;
   f32x16 acc[NT][MT];
-  clear(acc);
-  x.load(lines, 0, p.inner);
-  w.load(lines + kSlot, 0, p.inner);
-  x.load(lines + 2 * kSlot, kEach, p.inner);
-  w.load(lines + 3 * kSlot, kEach, p.inner);
-  arrive<2 * kLoads>();
-  Operands<T, NT, MT> now[2];
-  int xs = 0, ws = 1, spare = 4;           // slots of this step's x and W, and of the last one's W
-  now[0].read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, 0);
-  for (int k = 0; k < p.inner; k += kEach) {
-    const int xn = xs + 2 < kSlots ? xs + 2 : xs + 2 - kSlots;
-    const int wx = ws + 2 < kSlots ? ws + 2 : ws + 2 - kSlots;
+  auto start = [&]() {
+    clear(acc);
+    x.load(lines, begin, end);
+    w.load(lines + kSlot, begin, end);
+    x.load(lines + 2 * kSlot, begin + kEach, end);
+    w.load(lines + 3 * kSlot, begin + kEach, end);
+    arrive<2 * kLoads>();
+  };
+  auto further = [&](int slot) { return slot + 2 < kSlots ? slot + 2 : slot + 2 - kSlots; };
+  if constexpr (sizeof(T) == 4) {
+    auto sums = [&](auto thirds) {
+      start();
+      x.load(lines + 4 * kSlot, begin + 2 * kEach, end);
+      for (int k = begin, xs = 0, ws = 1; k < end; k += kEach) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      Operands<T, NT, MT>& next = now[(s + 1) & 1];
-      if (s < kSteps - 1) {
-        next.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, s + 1);
-        // not at once with W's, so that those come first
-        if (s == 0) x.load(lines + spare * kSlot, k + 2 * kEach, p.inner);
-      } else {
+        for (int j = 0; j < kSteps / 2; ++j) {
+          FloatOperands<NT, MT> now;
+          now.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, j);
+          if constexpr (decltype(thirds)::value) {
+            // one row of tiles' thirds at a time, as registers allow
+            u32x4 a[NT][3], b[3];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) to_thirds(now.a[t], a[t]);
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+              to_thirds(now.b[u], b);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) acc[t][u] = thirds_product(a[t], b, acc[t][u]);
+            }
+          } else {
+            now.multiply(acc);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
         arrive<kLoads>();                  // all but x of two steps on
-        next.read(lines + wx * kSlot, lines + xn * kSlot, wn, wm, 0);
-        w.load(lines + xs * kSlot, k + 2 * kEach, p.inner);
+        w.load(lines + xs * kSlot, k + 2 * kEach, end);
+        x.load(lines + ws * kSlot, k + 3 * kEach, end);
+        xs = further(xs);
+        ws = further(ws);
       }
-      now[s & 1].multiply(acc);
-      __builtin_amdgcn_sched_barrier(0);
+      arrive<0>();
+    };
+    sums(std::true_type());
+    if (any_not_finite(acc, reinterpret_cast<int*>(s_lines))) sums(std::false_type());
+  } else {
+    start();
+    Operands<T, NT, MT> now[2];
+    int xs = 0, ws = 1, spare = 4;         // slots of this step's x and W, and of the last one's W
+    now[0].read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, 0);
+    for (int k = begin; k < end; k += kEach) {
+      const int xn = further(xs), wx = further(ws);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        Operands<T, NT, MT>& next = now[(s + 1) & 1];
+        if (s < kSteps - 1) {
+          next.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, s + 1);
+          // not at once with W's, so that those come first
+          if (s == 0) x.load(lines + spare * kSlot, k + 2 * kEach, end);
+        } else {
+          arrive<kLoads>();                // all but x of two steps on
+          next.read(lines + wx * kSlot, lines + xn * kSlot, wn, wm, 0);
+          w.load(lines + xs * kSlot, k + 2 * kEach, end);
+        }
+        now[s & 1].multiply(acc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      spare = ws;
+      xs = xn;
+      ws = wx;
     }
-    spare = ws;
-    xs = xn;
-    ws = wx;
+    arrive<0>();
   }
-  arrive<0>();
   finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 8, m0 + wm, n0 + wn,
-                 0);
+                 blockIdx.y);
 }
 
 // One workgroup: BM rows of x by BN rows of W over a split of the summed axis;
@@ -433,33 +601,84 @@ __global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearPara
   const Lines<T, BN, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
   const int wm = wave % MW * (BM / MW), wn = wave / MW * (BN / NW);
   f32x16 acc[NT][MT];
-  clear(acc);
   auto load = [&](int k, int stage) {
     lds_char* const to = lines + stage * kStage;
     x.load(to, k, end);
     w.load(to + BM * kLineBytes, k, end);
   };
+  auto start = [&](int stages) {
+    clear(acc);
+    for (int s = 0; s < stages; ++s) load(begin + s * kEach, s);
+  };
+  if constexpr (sizeof(T) == 4) {
+    // Half a line's products run while the next half's thirds are made of what
+    // has been read, and the half after that is read: in one wave, as a CU
+    // holds four.
+    start(kStages);
+    arrive<(kStages - 1) * kLoads>();
+    FloatOperands<NT, MT> raw[2];
+    Thirds<NT, MT> now[2];
+    raw[0].read(lines + BM * kLineBytes, lines, wn, wm, 0);
+    raw[1].read(lines + BM * kLineBytes, lines, wn, wm, 1);
+    now[0].take(raw[0]);
+    for (int k = begin, stage = 0; k < end; k += kEach) {
+      arrive<(kStages - 2) * kLoads>();
+      load(k + kStages * kEach, stage);
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      const lds_char* const from = lines + stage * kStage;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load(begin + s * kEach, s);
-  arrive<(kStages - 2) * kLoads>();
-  Operands<T, NT, MT> now[2];
-  now[0].read(lines + BM * kLineBytes, lines, wn, wm, 0);
-  int stage = 0;
-  for (int k = begin; k < end; k += kEach) {
-    const int into = stage == 0 ? kStages - 1 : stage - 1;
-    const int after = stage == kStages - 1 ? 0 : stage + 1;
+      for (int j = 0; j < 2; ++j) {
+        raw[j].read(from + BM * kLineBytes, from, wn, wm, j);
+        now[j ^ 1].take(raw[j ^ 1]);
+        now[j].multiply(acc);
+        constexpr int kProducts = 6 * NT * MT, kOthers = 44 * (NT + MT) / kProducts;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      if (s == 0) load(k + (kStages - 1) * kEach, into);
-      if (s == kSteps - 1) arrive<(kStages - 2) * kLoads>();
-      const lds_char* const from = lines + (s == kSteps - 1 ? after : stage) * kStage;
-      now[(s + 1) & 1].read(from + BM * kLineBytes, from, wn, wm, (s + 1) % kSteps);
-      now[s & 1].multiply(acc);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < kProducts; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);          // a product
+          __builtin_amdgcn_sched_group_barrier(0x002, kOthers, 0);    // vector instructions
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    stage = after;
+    arrive<0>();
+    if (any_not_finite(acc, reinterpret_cast<int*>(s_lines))) {
+      start(kStages - 1);
+      for (int k = begin, stage = 0; k < end; k += kEach) {
+        arrive<(kStages - 2) * kLoads>();
+        load(k + (kStages - 1) * kEach, stage == 0 ? kStages - 1 : stage - 1);
+        const lds_char* const from = lines + stage * kStage;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          FloatOperands<NT, MT> again;
+          again.read(from + BM * kLineBytes, from, wn, wm, j);
+          again.multiply(acc);
+        }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+      }
+      arrive<0>();
+    }
+  } else {
+    start(kStages - 1);
+    arrive<(kStages - 2) * kLoads>();
+    Operands<T, NT, MT> now[2];
+    now[0].read(lines + BM * kLineBytes, lines, wn, wm, 0);
+    int stage = 0;
+    for (int k = begin; k < end; k += kEach) {
+      const int into = stage == 0 ? kStages - 1 : stage - 1;
+      const int after = stage == kStages - 1 ? 0 : stage + 1;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (s == 0) load(k + (kStages - 1) * kEach, into);
+        if (s == kSteps - 1) arrive<(kStages - 2) * kLoads>();
+        const lds_char* const from = lines + (s == kSteps - 1 ? after : stage) * kStage;
+        now[(s + 1) & 1].read(from + BM * kLineBytes, from, wn, wm, (s + 1) % kSteps);
+        now[s & 1].multiply(acc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      stage = after;
+    }
+    arrive<0>();
   }
-  arrive<0>();
   finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 8, m0 + wm, n0 + wn,
                  blockIdx.y);
 }
@@ -680,7 +899,7 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
     case LinearForm::k64x128: e = launch_tiles<T, 64, 128, 2, 2, 4>(p, s); break;
     case LinearForm::k128: e = launch_tiles<T, 128, 128, 2, 2, 4>(p, s); break;
     case LinearForm::k256:
-      e = launch_groups(&linear_large_kernel<T>, tiles_of(p.rows, p.outer, 256, 256), 1, 512,
+      e = launch_groups(&linear_large_kernel<T>, tiles_of(p.rows, p.outer, 256, 256), p.splits, 512,
                         5 * 256 * kLineBytes, p, s);
       break;
   }
@@ -698,10 +917,12 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
 //   64 (16) 9.6; a row, 4096 x 6144: few 12.7, 64 x 128 (5) 12.5; 64 rows: few
 //   38, 64 (2) 15.3, 64 x 128 (4) 15.0, 64 x 128 (1) 24
 //   100 rows, 4000 x 100: 64 (16) 7.4, 64 (1) 19
+//   2,910 rows, 7848 x 1420: 128 149, 128 (3) 116, 256 148, 256 (3) 81
 //   1,111 rows, 2304 x 1544: 64 17.8, 64 x 128 17.0, 128 23, 256 44
 //   2,048 rows, 2048 x 2048: 64 31, 64 x 128 30, 128 24, 256 42
 //   4,096 rows, 4096 x 4096: 64 216, 64 x 128 200, 128 162, 256 108
-// and in float32 4,000 rows, 4000 x 4000: 1176, 1077, 1013, 911.
+//   and in float32 4,000 rows, 4000 x 4000: 64 962, 64 x 128 909, 128 704, 256
+//   627; 256 rows, 2048 x 2048: 64 42, 64 (4) 26, 64 x 128 (4) 25.
 struct FormCost {
   LinearForm form;
   int rows, columns;               // of a tile
@@ -709,9 +930,9 @@ struct FormCost {
 };
 constexpr FormCost kFormCosts[] = {
     {LinearForm::k64, 64, 64, {0.30f, 0.57f}, 1.0f},
-    {LinearForm::k64x128, 64, 128, {0.38f, 1.05f}, 1.0f},
-    {LinearForm::k128, 128, 128, {0.58f, 2.0f}, 2.5f},
-    {LinearForm::k256, 256, 256, {1.58f, 7.2f}, 4.0f},
+    {LinearForm::k64x128, 64, 128, {0.38f, 0.85f}, 1.0f},
+    {LinearForm::k128, 128, 128, {0.58f, 1.4f}, 2.5f},
+    {LinearForm::k256, 256, 256, {1.58f, 4.9f}, 4.0f},
 };
 constexpr int64_t kChipCus = 256;
 constexpr int kMostSplits = 16;
@@ -735,8 +956,7 @@ LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size) {
   const int64_t steps = (inner * size + kLineBytes - 1) / kLineBytes;
   for (const FormCost& f : kFormCosts) {
     const int64_t tiles = tiles_of(rows, outer, f.rows, f.columns);
-    // the largest tiles' kernel does not split
-    const int most = f.form == LinearForm::k256 || tiles >= kChipCus ? 1 : kMostSplits;
+    const int most = tiles >= kChipCus ? 4 : kMostSplits;
     for (int splits = 1; splits <= most && splits <= steps; ++splits) {
       const int64_t groups = tiles * splits, each = (steps + splits - 1) / splits;
       float step = f.step[size == 4];

@@ -9,21 +9,27 @@
 // Every operator leaves its inputs as they are and writes new lengths,
 // tables, counts and shares (release pushes onto the free stack above its
 // count, where nothing reads), so that a step can be taken back by keeping
-// what was there.  Each runs in phases that need all of the one before: one
-// workgroup runs them all where the numbers are few (a launch is most of
-// such a call), else they are launches of their own.
+// what was there.  Each runs in phases that need all of the one before.  Where
+// the numbers are few, one workgroup runs them all with the pages' numbers in
+// LDS and its entries in registers, so that a phase costs a barrier and not a
+// launch or a round trip to memory; else they are launches of their own.
 
 #include "common.h"
 
 namespace cowsdm_impl {
 
 constexpr int kPageThreads = 512;
-constexpr int kPageRequests = 4096;    // children of a fork, named requests of a release
-constexpr int kPageChunk = 4096;       // numbers that a workgroup counts and places in order
+constexpr int kPageNamed = 4096;       // children of a fork, named requests of a release
 
-// Table entries and pages up to which one workgroup runs every phase.
-// Measured in microseconds, one workgroup and launches: see the entries.
-constexpr int64_t kPageOneGroup = 16384;
+// What one workgroup takes: entries of tables and pages (LDS holds two
+// numbers a page), and children or named requests.
+constexpr int kOneThreads = 1024;
+constexpr int kOneWaves = kOneThreads / kWave;
+constexpr int kOneEach = 16;
+constexpr int kOneNumbers = kOneThreads * kOneEach;
+constexpr int kOnePages = 12288;
+constexpr int kOneNamed = 1024;
+constexpr int kOneRequests = 4096;
 
 // Exclusive sum of v over the workgroup and, in `total`, the sum.
 __device__ __forceinline__ int group_exclusive(int v, int* parts, int& total) {
@@ -65,10 +71,43 @@ __device__ __forceinline__ int pages_held(int32_t length, int page_shift, int co
   return n < columns ? n : columns;
 }
 
-// What one phase wrote is there for the next, in the same workgroup.
-__device__ __forceinline__ void next_phase() {
-  __threadfence();
+// Places in order for one workgroup's numbers, number i * kOneThreads + thread
+// being the thread's i-th: s_places[i][wave] becomes how many of the flagged
+// (bit i of a thread's `flags`) come before that wave's i-th ones.  Returns
+// how many there are.
+__device__ __forceinline__ int one_places(uint32_t flags, int (*s_places)[kOneWaves]) {
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & (kWave - 1);
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const uint64_t mask = __ballot(flags >> i & 1);
+    if (lane == 0) s_places[i][tid / kWave] = __builtin_popcountll(mask);
+  }
   __syncthreads();
+  constexpr int kCounts = kOneEach * kOneWaves, kMine = kCounts / kWave;
+  int* const flat = &s_places[0][0];
+  if (tid < kWave) {
+    int v[kMine], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) sum += v[j] = flat[tid * kMine + j];
+    const int all = wave_inclusive(sum);
+    int before = all - sum;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      flat[tid * kMine + j] = before;
+      before += v[j];
+    }
+    if (tid == kWave - 1) s_places[kOneEach][0] = all;
+  }
+  __syncthreads();
+  return s_places[kOneEach][0];
+}
+
+// The place of this thread's i-th number among the flagged.
+__device__ __forceinline__ int one_place(uint32_t flags, int i,
+                                         const int (*s_places)[kOneWaves]) {
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & (kWave - 1);
+  const uint64_t below = __ballot(flags >> i & 1) & ((uint64_t{1} << lane) - 1);
+  return s_places[i][tid / kWave] + __builtin_popcountll(below);
 }
 
 // ------------------------------------------------------------------- fork
@@ -174,12 +213,76 @@ __device__ void fork_tables(const ForkParams& p, int block, int blocks) {
   }
 }
 
-__global__ __launch_bounds__(kPageThreads) void fork_one_kernel(ForkParams p) {
-  __shared__ int s_parts[kPageThreads / kWave];
-  fork_plan(p, s_parts);
-  fork_shares(p, 0, 1);
-  next_phase();
-  fork_tables(p, 0, 1);
+// The same in one workgroup: a child to a thread, the pages' shares in LDS.
+// What is left are the dependent loads of a child's parent, its length, the
+// tables and the free pages.
+__global__ __launch_bounds__(kOneThreads) void fork_one_kernel(ForkParams p) {
+  extern __shared__ __align__(16) int32_t s_shares[];             // [pages]
+  __shared__ int s_places[2][kOneWaves];
+  __shared__ int32_t s_parent[kOneNamed], s_whole[kOneNamed], s_target[kOneNamed];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & (kWave - 1), wave = tid / kWave;
+  const int32_t count = *p.free_count;
+  int32_t n = 0, r = 0;
+  int rest = 0, wrong = 0;
+  if (tid < p.children) {
+    r = p.parents[tid];
+    n = p.tokens[tid];
+  }
+  for (int i = tid; i < p.pages; i += kOneThreads) s_shares[i] = p.page_shares[i];
+  if (tid < p.children) {
+    const int32_t held = r >= 0 && r < p.requests ? p.lengths[r] : -1;
+    wrong = n < 0 || n > held || pages_held(n, p.page_shift, INT32_MAX) > p.columns;
+    rest = (n & ((1 << p.page_shift) - 1)) != 0;
+  }
+  const uint64_t rests = __ballot(rest);
+  if (lane == 0) {
+    s_places[0][wave] = __builtin_popcountll(rests);
+    s_places[1][wave] = 0;
+  }
+  if (__ballot(wrong) && lane == 0) s_places[1][wave] = 1;
+  __syncthreads();
+  int before = 0, need = 0, bad = 0;
+#pragma unroll
+  for (int w = 0; w < kOneWaves; ++w) {
+    if (w < wave) before += s_places[0][w];
+    need += s_places[0][w];
+    bad |= s_places[1][w];
+  }
+  before += __builtin_popcountll(rests & ((uint64_t{1} << lane) - 1));
+  const bool fits = !bad && need <= count && count <= p.pages;
+  if (tid < p.children) {
+    int32_t source = -1, target = -1;
+    if (fits && rest) {
+      source = p.page_tables[static_cast<int64_t>(r) * p.columns + (n >> p.page_shift)];
+      target = p.free_pages[count - 1 - before];
+    }
+    s_parent[tid] = fits ? r : 0;
+    s_whole[tid] = fits ? n >> p.page_shift : 0;
+    s_target[tid] = target;
+    p.lengths_out[tid] = fits ? n : 0;
+    p.sources[tid] = source;
+    p.targets[tid] = target;
+  }
+  if (tid == 0) {
+    *p.free_count_out = fits ? count - need : count;
+    *p.overflow = fits ? 0 : 1;
+  }
+  __syncthreads();
+  const int entries = p.children * p.columns;
+#pragma unroll 4
+  for (int e = tid; e < entries; e += kOneThreads) {
+    const int i = e / p.columns, j = e - i * p.columns, whole = s_whole[i];
+    int32_t id = -1;
+    if (j < whole) {
+      id = p.page_tables[static_cast<int64_t>(s_parent[i]) * p.columns + j];
+      if (id >= 0 && id < p.pages) atomicAdd(s_shares + id, 1);
+    } else if (j == whole) {
+      id = s_target[i];
+    }
+    p.tables_out[e] = id;
+  }
+  __syncthreads();
+  for (int i = tid; i < p.pages; i += kOneThreads) p.shares_out[i] = s_shares[i];
 }
 
 __global__ __launch_bounds__(kPageThreads) void fork_plan_kernel(ForkParams p) {
@@ -212,29 +315,32 @@ struct ReleaseParams {
   int32_t pages;
   int32_t n;
   int32_t entries;        // n * columns
-  int32_t chunks;
+  int32_t chunks, chunk;  // of entries, and the entries of one
   int32_t page_shift;
 };
 
-// A request counts where it is named first.  That is found in LDS, or in the
+// A request counts where it is named first, which is found in LDS, or in the
 // new lengths' place where there are more requests.
 __device__ void release_plan(const ReleaseParams& p, int32_t* in_lds) {
-  const int tid = static_cast<int>(threadIdx.x);
-  int32_t* const first = p.requests <= kPageRequests ? in_lds : p.lengths_out;
-  for (int r = tid; r < p.requests; r += kPageThreads) first[r] = INT32_MAX;
-  next_phase();
-  for (int i = tid; i < p.n; i += kPageThreads) {
+  const int tid = static_cast<int>(threadIdx.x), step = static_cast<int>(blockDim.x);
+  const bool few = p.requests <= kOneRequests;
+  int32_t* const first = few ? in_lds : p.lengths_out;
+  for (int r = tid; r < p.requests; r += step) first[r] = INT32_MAX;
+  if (!few) __threadfence();
+  __syncthreads();
+  for (int i = tid; i < p.n; i += step) {
     const int32_t r = p.named[i];
     if (r >= 0 && r < p.requests) atomicMin(first + r, i);
   }
-  next_phase();
-  for (int i = tid; i < p.n; i += kPageThreads) {
+  if (!few) __threadfence();
+  __syncthreads();
+  for (int i = tid; i < p.n; i += step) {
     const int32_t r = p.named[i];
     const bool is = r >= 0 && r < p.requests && first[r] == i;
     p.held[i] = is ? pages_held(p.lengths[r], p.page_shift, p.columns) : 0;
   }
   __syncthreads();
-  for (int r = tid; r < p.requests; r += kPageThreads)
+  for (int r = tid; r < p.requests; r += step)
     p.lengths_out[r] = first[r] == INT32_MAX ? p.lengths[r] : 0;
 }
 
@@ -272,54 +378,111 @@ __device__ __forceinline__ int release_freed(const ReleaseParams& p, int e) {
   return id >= 0 && p.last[id] == e && p.shares_out[id] < 0 ? id : -1;
 }
 
-__device__ void release_count(const ReleaseParams& p, int block, int blocks, int* parts) {
-  for (int c = block; c < p.chunks; c += blocks) {
-    int mine = 0;
-    for (int at = 0; at < kPageChunk; at += kPageThreads)
-      mine += release_freed(p, c * kPageChunk + at + static_cast<int>(threadIdx.x)) >= 0;
-    int total;
-    group_exclusive(mine, parts, total);
-    if (threadIdx.x == 0) p.counts[c] = total;
-  }
+__device__ void release_count(const ReleaseParams& p, int* parts) {
+  int mine = 0;
+  const int from = static_cast<int>(blockIdx.x) * p.chunk + static_cast<int>(threadIdx.x);
+  for (int at = 0; at < p.chunk; at += kPageThreads) mine += release_freed(p, from + at) >= 0;
+  int total;
+  group_exclusive(mine, parts, total);
+  if (threadIdx.x == 0) p.counts[blockIdx.x] = total;
 }
 
-__device__ void release_push(const ReleaseParams& p, int block, int blocks, int* parts) {
+__device__ void release_push(const ReleaseParams& p, int* parts) {
   const int32_t count = *p.free_count;
-  for (int c = block; c < p.chunks; c += blocks) {
-    int all;
-    int64_t to = static_cast<int64_t>(count) + sum_before(p.counts, p.chunks, c, parts, all);
-    if (c == 0 && threadIdx.x == 0) {
-      const int64_t top = static_cast<int64_t>(count) + all;
-      *p.free_count_out = static_cast<int32_t>(top < p.pages ? top : p.pages);
+  const int c = static_cast<int>(blockIdx.x);
+  int all;
+  int64_t to = static_cast<int64_t>(count) + sum_before(p.counts, p.chunks, c, parts, all);
+  if (c == 0 && threadIdx.x == 0) {
+    const int64_t top = static_cast<int64_t>(count) + all;
+    *p.free_count_out = static_cast<int32_t>(top < p.pages ? top : p.pages);
+  }
+  const int from = c * p.chunk + static_cast<int>(threadIdx.x);
+  for (int at = 0; at < p.chunk; at += kPageThreads) {
+    const int id = release_freed(p, from + at);
+    int total;
+    const int64_t mine = to + group_exclusive(id >= 0, parts, total);
+    if (id >= 0) {
+      if (mine >= 0 && mine < p.pages) p.free_pages[mine] = id;
+      p.shares_out[id] = 0;
     }
-    for (int at = 0; at < kPageChunk; at += kPageThreads) {
-      const int id = release_freed(p, c * kPageChunk + at + static_cast<int>(threadIdx.x));
-      int total;
-      const int64_t mine = to + group_exclusive(id >= 0, parts, total);
-      if (id >= 0) {
-        if (mine >= 0 && mine < p.pages) p.free_pages[mine] = id;
-        p.shares_out[id] = 0;
-      }
-      to += total;
-    }
+    to += total;
   }
 }
 
-__global__ __launch_bounds__(kPageThreads) void release_one_kernel(ReleaseParams p) {
-  __shared__ int s_parts[kPageThreads / kWave];
-  __shared__ int32_t s_first[kPageRequests];
-  release_plan(p, s_first);
-  release_shares(p, 0, 1);
-  next_phase();
-  release_take(p, 0, 1);
-  next_phase();
-  release_count(p, 0, 1, s_parts);
-  next_phase();
-  release_push(p, 0, 1, s_parts);
+// The same in one workgroup: the pages' shares and last entries in LDS, its
+// entries in registers.
+__global__ __launch_bounds__(kOneThreads) void release_one_kernel(ReleaseParams p) {
+  extern __shared__ __align__(16) int32_t s_pages[];              // [2][pages]
+  __shared__ int32_t s_first[kOneRequests];
+  __shared__ int32_t s_row[kOneNamed], s_held[kOneNamed];
+  __shared__ int s_places[kOneEach + 1][kOneWaves];
+  int32_t* const s_shares = s_pages;
+  int32_t* const s_last = s_pages + p.pages;
+  const int tid = static_cast<int>(threadIdx.x);
+  const int32_t count = *p.free_count;
+  const int32_t name = tid < p.n ? p.named[tid] : -1;
+  const bool is_name = name >= 0 && name < p.requests;
+  const int32_t length = is_name ? p.lengths[name] : 0;
+  for (int r = tid; r < p.requests; r += kOneThreads) s_first[r] = INT32_MAX;
+  for (int i = tid; i < p.pages; i += kOneThreads) {
+    s_shares[i] = p.page_shares[i];
+    s_last[i] = -1;
+  }
+  __syncthreads();
+  if (is_name) atomicMin(s_first + name, tid);
+  __syncthreads();
+  if (tid < p.n) {
+    s_row[tid] = name;
+    s_held[tid] = is_name && s_first[name] == tid ? pages_held(length, p.page_shift, p.columns) : 0;
+  }
+  for (int r = tid; r < p.requests; r += kOneThreads)
+    p.lengths_out[r] = s_first[r] == INT32_MAX ? p.lengths[r] : 0;
+  __syncthreads();
+  int32_t id[kOneEach];
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int e = i * kOneThreads + tid;
+    id[i] = -1;
+    if (e < p.entries) {
+      const int named = e / p.columns, j = e - named * p.columns;
+      if (j < s_held[named])
+        id[i] = p.page_tables[static_cast<int64_t>(s_row[named]) * p.columns + j];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    if (id[i] < 0 || id[i] >= p.pages) {
+      id[i] = -1;
+    } else {
+      atomicSub(s_shares + id[i], 1);
+      atomicMax(s_last + id[i], i * kOneThreads + tid);
+    }
+  }
+  __syncthreads();
+  uint32_t freed = 0;
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i)
+    if (id[i] >= 0 && s_last[id[i]] == i * kOneThreads + tid && s_shares[id[i]] < 0)
+      freed |= 1u << i;
+  const int all = one_places(freed, s_places);
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int64_t to = static_cast<int64_t>(count) + one_place(freed, i, s_places);
+    if (freed >> i & 1) {
+      if (to >= 0 && to < p.pages) p.free_pages[to] = id[i];
+      s_shares[id[i]] = 0;
+    }
+  }
+  if (tid == 0) {
+    const int64_t top = static_cast<int64_t>(count) + all;
+    *p.free_count_out = static_cast<int32_t>(top < p.pages ? top : p.pages);
+  }
+  __syncthreads();
+  for (int i = tid; i < p.pages; i += kOneThreads) p.shares_out[i] = s_shares[i];
 }
 
 __global__ __launch_bounds__(kPageThreads) void release_plan_kernel(ReleaseParams p) {
-  __shared__ int32_t s_first[kPageRequests];
+  __shared__ int32_t s_first[kOneRequests];
   if (blockIdx.x == 0) release_plan(p, s_first);
   else release_shares(p, blockIdx.x - 1, gridDim.x - 1);
 }
@@ -330,12 +493,12 @@ __global__ __launch_bounds__(kPageThreads) void release_take_kernel(ReleaseParam
 
 __global__ __launch_bounds__(kPageThreads) void release_count_kernel(ReleaseParams p) {
   __shared__ int s_parts[kPageThreads / kWave];
-  release_count(p, blockIdx.x, gridDim.x, s_parts);
+  release_count(p, s_parts);
 }
 
 __global__ __launch_bounds__(kPageThreads) void release_push_kernel(ReleaseParams p) {
   __shared__ int s_parts[kPageThreads / kWave];
-  release_push(p, blockIdx.x, gridDim.x, s_parts);
+  release_push(p, s_parts);
 }
 
 // ---------------------------------------------------------------- compact
@@ -356,7 +519,7 @@ struct CompactParams {
   int32_t columns;
   int32_t pages;
   int32_t entries;
-  int32_t chunks;
+  int32_t chunks, chunk;  // of pages, and the pages of one
   int32_t page_shift;
 };
 
@@ -384,49 +547,46 @@ __device__ void compact_mark(const CompactParams& p, int block, int blocks) {
   }
 }
 
-__device__ void compact_count(const CompactParams& p, int block, int blocks, int* parts) {
-  for (int c = block; c < p.chunks; c += blocks) {
-    int mine = 0;
-    for (int at = 0; at < kPageChunk; at += kPageThreads) {
-      const int i = c * kPageChunk + at + static_cast<int>(threadIdx.x);
-      mine += i < p.pages ? p.used[i] : 0;
-    }
-    int total;
-    group_exclusive(mine, parts, total);
-    if (threadIdx.x == 0) p.counts[c] = total;
+__device__ void compact_count(const CompactParams& p, int* parts) {
+  int mine = 0;
+  for (int at = 0; at < p.chunk; at += kPageThreads) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * p.chunk + at + threadIdx.x;
+    mine += i < p.pages ? p.used[i] : 0;
   }
+  int total;
+  group_exclusive(mine, parts, total);
+  if (threadIdx.x == 0) p.counts[blockIdx.x] = total;
 }
 
 // U pages are in use.  The k-th of those numbered U or more goes to the k-th
 // number below U that is free: as many of the one as of the other.  Of page i
 // with b pages in use before it, i - b are free before it.
-__device__ void compact_place(const CompactParams& p, int block, int blocks, int* parts) {
-  for (int c = block; c < p.chunks; c += blocks) {
-    int all;
-    int before = sum_before(p.counts, p.chunks, c, parts, all);
-    if (c == 0 && threadIdx.x == 0) *p.free_count = p.pages - all;
-    // those in use below U
-    int low = sum_before(p.counts, p.chunks, all / kPageChunk, parts, all);
-    {
-      int mine = 0, total;
-      for (int i = all / kPageChunk * kPageChunk + static_cast<int>(threadIdx.x); i < all;
-           i += kPageThreads)
-        mine += p.used[i] != 0;
-      group_exclusive(mine, parts, total);
-      low += total;
-    }
-    for (int at = 0; at < kPageChunk; at += kPageThreads) {
-      const int i = c * kPageChunk + at + static_cast<int>(threadIdx.x);
-      const int is = i < p.pages ? p.used[i] : 0;
-      int total;
-      const int rank = before + group_exclusive(is, parts, total);
-      before += total;
-      if (is && i >= all) {
-        p.sources[rank - low] = i;
-        p.used[i] = rank - low;        // read by no one before the next phase
-      } else if (!is && i < all) {
-        p.targets[i - rank] = i;
-      }
+__device__ void compact_place(const CompactParams& p, int* parts) {
+  const int c = static_cast<int>(blockIdx.x);
+  int all;
+  int before = sum_before(p.counts, p.chunks, c, parts, all);
+  if (c == 0 && threadIdx.x == 0) *p.free_count = p.pages - all;
+  // those in use below U
+  int low = sum_before(p.counts, p.chunks, all / p.chunk, parts, all);
+  {
+    int mine = 0, total;
+    for (int i = all / p.chunk * p.chunk + static_cast<int>(threadIdx.x); i < all;
+         i += kPageThreads)
+      mine += p.used[i] != 0;
+    group_exclusive(mine, parts, total);
+    low += total;
+  }
+  for (int at = 0; at < p.chunk; at += kPageThreads) {
+    const int64_t i = static_cast<int64_t>(c) * p.chunk + at + threadIdx.x;
+    const int is = i < p.pages ? p.used[i] : 0;
+    int total;
+    const int rank = before + group_exclusive(is, parts, total);
+    before += total;
+    if (is && i >= all) {
+      p.sources[rank - low] = static_cast<int32_t>(i);
+      p.used[i] = rank - low;          // read by no one before the next phase
+    } else if (!is && i < all) {
+      p.targets[i - rank] = static_cast<int32_t>(i);
     }
   }
 }
@@ -450,17 +610,68 @@ __device__ void compact_rewrite(const CompactParams& p, int block, int blocks) {
   }
 }
 
-__global__ __launch_bounds__(kPageThreads) void compact_one_kernel(CompactParams p) {
-  __shared__ int s_parts[kPageThreads / kWave];
-  compact_clear(p, 0, 1);
-  next_phase();
-  compact_mark(p, 0, 1);
-  next_phase();
-  compact_count(p, 0, 1, s_parts);
-  next_phase();
-  compact_place(p, 0, 1, s_parts);
-  next_phase();
-  compact_rewrite(p, 0, 1);
+// The same in one workgroup: what is in use, then the moved pages' ranks and
+// the free numbers below U, in LDS.
+__global__ __launch_bounds__(kOneThreads) void compact_one_kernel(CompactParams p) {
+  extern __shared__ __align__(16) int32_t s_pages[];              // [2][pages]
+  __shared__ int s_places[kOneEach + 1][kOneWaves];
+  __shared__ int s_low;
+  int32_t* const s_used = s_pages;
+  int32_t* const s_targets = s_pages + p.pages;
+  const int tid = static_cast<int>(threadIdx.x);
+  for (int i = tid; i < p.pages; i += kOneThreads) s_used[i] = 0;
+  int32_t id[kOneEach];
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int e = i * kOneThreads + tid;
+    id[i] = e < p.entries ? compact_entry(p, e) : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i)
+    if (id[i] >= 0) s_used[id[i]] = 1;
+  __syncthreads();
+  uint32_t used = 0;
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int page = i * kOneThreads + tid;
+    if (page < p.pages && s_used[page]) used |= 1u << i;
+  }
+  const int all = one_places(used, s_places);
+  if (tid == 0 && all == p.pages) s_low = all;
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int page = i * kOneThreads + tid, rank = one_place(used, i, s_places);
+    if (page == all && all < p.pages) s_low = rank;
+    if (page < all && !(used >> i & 1)) {
+      s_targets[page - rank] = page;
+      p.targets[page - rank] = page;
+    }
+  }
+  __syncthreads();
+  const int low = s_low, moves = all - low;
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int page = i * kOneThreads + tid, rank = one_place(used, i, s_places) - low;
+    if (page >= p.pages) continue;
+    const bool is = used >> i & 1;
+    if (is && page >= all) {
+      s_used[page] = rank;
+      p.sources[rank] = page;
+    }
+    // every page's shares in their new place
+    if (is) p.shares_out[page < all ? page : s_targets[rank]] = p.page_shares[page];
+    if (page >= all) p.shares_out[page] = 0;
+    p.free_pages[page] = page < p.pages - all ? p.pages - 1 - page : -1;
+    if (page >= moves && page < p.pages / 2) p.sources[page] = p.targets[page] = -1;
+  }
+  if (tid == 0) *p.free_count = p.pages - all;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kOneEach; ++i) {
+    const int e = i * kOneThreads + tid;
+    if (e < p.entries) p.tables_out[e] = id[i] < all ? id[i] : s_targets[s_used[id[i]]];
+  }
 }
 
 __global__ __launch_bounds__(kPageThreads) void compact_clear_kernel(CompactParams p) {
@@ -473,12 +684,12 @@ __global__ __launch_bounds__(kPageThreads) void compact_mark_kernel(CompactParam
 
 __global__ __launch_bounds__(kPageThreads) void compact_count_kernel(CompactParams p) {
   __shared__ int s_parts[kPageThreads / kWave];
-  compact_count(p, blockIdx.x, gridDim.x, s_parts);
+  compact_count(p, s_parts);
 }
 
 __global__ __launch_bounds__(kPageThreads) void compact_place_kernel(CompactParams p) {
   __shared__ int s_parts[kPageThreads / kWave];
-  compact_place(p, blockIdx.x, gridDim.x, s_parts);
+  compact_place(p, s_parts);
 }
 
 __global__ __launch_bounds__(kPageThreads) void compact_rewrite_kernel(CompactParams p) {
@@ -544,18 +755,20 @@ int32_t page_shift_of(int64_t page_tokens, const char* where, int& shift) {
   return 0;
 }
 
+constexpr int64_t kMostChunk = int64_t{1} << 22;    // chunk_of(2^31)
+
 // Sizes that every table operator has; n rows of `columns` entries.
 int32_t check_tables(int64_t requests, int64_t columns, int64_t pages, int64_t n,
                      int64_t page_tokens, const char* where) {
   if (requests < 0 || columns < 0 || pages < 0 || n < 0)
     return fail(COWSDM_EARG, "%s: negative size", where);
-  if (n > kPageRequests)
-    return fail(COWSDM_ELIMIT, "%s: at most %d requests a call", where, kPageRequests);
+  if (n > kPageNamed)
+    return fail(COWSDM_ELIMIT, "%s: at most %d requests a call", where, kPageNamed);
   if (requests > INT32_MAX) return fail(COWSDM_ELIMIT, "%s: too large", where);
   if (pages > INT32_MAX / page_tokens || columns > INT32_MAX / page_tokens)
     return fail(COWSDM_ELIMIT, "%s: more than 2^31 tokens", where);
   const int64_t rows = requests > n ? requests : n;
-  if (columns > 0 && rows > (INT32_MAX - kPageChunk) / columns)
+  if (columns > 0 && rows > (INT32_MAX - kMostChunk) / columns)
     return fail(COWSDM_ELIMIT, "%s: 2^31 table entries or more", where);
   return 0;
 }
@@ -565,8 +778,25 @@ uint32_t groups_of(int64_t numbers) {
   return static_cast<uint32_t>(n < 1 ? 1 : n > 4096 ? 4096 : n);
 }
 
+// Numbers that a workgroup counts and then places in order: one a thread, or
+// more where 1,024 workgroups would not do, each of which adds up the others'
+// counts.
+int64_t chunk_of(int64_t numbers) {
+  const int64_t each = (numbers + kPageThreads * 1024 - 1) / (kPageThreads * 1024);
+  return kPageThreads * (each < 1 ? 1 : each);
+}
+
 int64_t chunks_of(int64_t numbers) {
-  return numbers <= kPageChunk ? 1 : (numbers + kPageChunk - 1) / kPageChunk;
+  return numbers <= kPageThreads ? 1 : (numbers + chunk_of(numbers) - 1) / chunk_of(numbers);
+}
+
+// Dynamic LDS past what a kernel may have by itself, beside its own.
+int32_t allow_lds(const void* kernel, int bytes, const char* where) {
+  if (bytes <= 32 * 1024) return 0;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           bytes);
+  return e == hipSuccess ? 0
+                         : fail(static_cast<int32_t>(e), "%s: %s", where, hipGetErrorString(e));
 }
 
 }  // namespace cowsdm_impl
@@ -597,8 +827,12 @@ extern "C" int32_t cowsdm_page_tables_fork(
                static_cast<int32_t>(pages), static_cast<int32_t>(children), shift};
   const auto s = static_cast<hipStream_t>(stream);
   const int64_t entries = children * columns;
-  if (entries + pages <= kPageOneGroup) {
-    hipLaunchKernelGGL(fork_one_kernel, dim3(1), dim3(kPageThreads), 0, s, p);
+  if (entries <= kOneNumbers && pages <= kOnePages && children <= kOneNamed) {
+    const int bytes = static_cast<int>(4 * pages);
+    if (int32_t e = allow_lds(reinterpret_cast<const void*>(&fork_one_kernel), bytes,
+                              "page_tables_fork"))
+      return e;
+    hipLaunchKernelGGL(fork_one_kernel, dim3(1), dim3(kOneThreads), bytes, s, p);
     return launch_status("page_tables_fork");
   }
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1 + groups_of(pages)), dim3(kPageThreads), 0, s, p);
@@ -610,7 +844,7 @@ extern "C" int32_t cowsdm_page_tables_fork(
 extern "C" int64_t cowsdm_page_tables_release_workspace_bytes(int64_t pages, int64_t columns,
                                                               int64_t n) {
   if (pages < 0 || columns < 0 || n < 0 || pages > INT32_MAX || columns > INT32_MAX ||
-      n > kPageRequests)
+      n > kPageNamed)
     return -1;
   return 4 * (pages + n + chunks_of(n * columns));
 }
@@ -640,11 +874,16 @@ extern "C" int32_t cowsdm_page_tables_release(
                   static_cast<int32_t>(requests), static_cast<int32_t>(columns),
                   static_cast<int32_t>(pages), static_cast<int32_t>(n),
                   static_cast<int32_t>(entries), static_cast<int32_t>(chunks),
-                  shift};
+                  static_cast<int32_t>(chunk_of(entries)), shift};
   const auto s = static_cast<hipStream_t>(stream);
   const auto groups = dim3(static_cast<uint32_t>(p.chunks));
-  if (entries + pages <= kPageOneGroup) {
-    hipLaunchKernelGGL(release_one_kernel, dim3(1), dim3(kPageThreads), 0, s, p);
+  if (entries <= kOneNumbers && pages <= kOnePages && n <= kOneNamed &&
+      requests <= kOneRequests) {
+    const int bytes = static_cast<int>(8 * pages);
+    if (int32_t e = allow_lds(reinterpret_cast<const void*>(&release_one_kernel), bytes,
+                              "page_tables_release"))
+      return e;
+    hipLaunchKernelGGL(release_one_kernel, dim3(1), dim3(kOneThreads), bytes, s, p);
     return launch_status("page_tables_release");
   }
   hipLaunchKernelGGL(release_plan_kernel, dim3(1 + groups_of(pages)), dim3(kPageThreads), 0, s,
@@ -686,10 +925,14 @@ extern "C" int32_t cowsdm_page_tables_compact(
                   free_count_out, sources, targets, used, used + pages,
                   static_cast<int32_t>(requests), static_cast<int32_t>(columns),
                   static_cast<int32_t>(pages), static_cast<int32_t>(entries),
-                  static_cast<int32_t>(chunks), shift};
+                  static_cast<int32_t>(chunks), static_cast<int32_t>(chunk_of(pages)), shift};
   const auto s = static_cast<hipStream_t>(stream);
-  if (entries + pages <= kPageOneGroup) {
-    hipLaunchKernelGGL(compact_one_kernel, dim3(1), dim3(kPageThreads), 0, s, p);
+  if (entries <= kOneNumbers && pages <= kOnePages) {
+    const int bytes = static_cast<int>(8 * pages);
+    if (int32_t e = allow_lds(reinterpret_cast<const void*>(&compact_one_kernel), bytes,
+                              "page_tables_compact"))
+      return e;
+    hipLaunchKernelGGL(compact_one_kernel, dim3(1), dim3(kOneThreads), bytes, s, p);
     return launch_status("page_tables_compact");
   }
   const auto groups = dim3(static_cast<uint32_t>(chunks));

@@ -9,6 +9,8 @@ recorded) and no CPU path.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _native as nat
@@ -19,16 +21,23 @@ ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _MOST = 1 << 20          # elements of a row, and between rows
 
 
-def _matrix(tensor: torch.Tensor) -> tuple[torch.Tensor, int]:
+@lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, inner: int, outer: int, float_type: int) -> int:
+    """By the sizes alone: asked for once."""
+
+    return nat.lib().cowsdm_linear_workspace_bytes(rows, inner, outer, float_type)
+
+
+def _matrix(tensor: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
     """A matrix whose rows can be read, and the elements between them: itself
     or a contiguous copy.  (Rows that are contiguous but not aligned are read
     element by element by the kernel, which costs less than a copy.)"""
 
-    if tensor.stride(1) != 1 and tensor.shape[1] > 1 or tensor.stride(0) > _MOST:
+    row, column = tensor.stride()
+    if column != 1 and columns > 1 or row > _MOST:
         tensor = tensor.contiguous()
-    if tensor.shape[0] == 1:
-        return tensor, 0
-    return tensor, tensor.stride(0)
+        row = columns
+    return tensor, 0 if tensor.shape[0] == 1 else row
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -47,44 +56,50 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         raise ValueError("linear takes x [...,K] and weight [N,K]")
     outer, inner = weight.shape
     shape = (*x.shape[:-1], outer)
-    if bias is not None and bias.shape != (outer,):
-        raise ValueError("linear bias must be [N]")
-    if residual is not None and residual.shape != shape:
-        raise ValueError("linear residual must be [...,N]")
     if inner > _MOST:
         raise ValueError(f"linear sums over at most {_MOST} elements")
-    others = [t for t in (weight, bias, residual) if t is not None]
-    _need_no_gradient(x, *others)
-    dtype = x.dtype
+    dtype, index = x.dtype, x.get_device()
+    alike = weight.dtype is dtype
+    together = weight.get_device() == index
+    if bias is not None:
+        if bias.shape != (outer,):
+            raise ValueError("linear bias must be [N]")
+        alike, together = alike and bias.dtype is dtype, together and bias.get_device() == index
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError("linear residual must be [...,N]")
+        alike = alike and residual.dtype is dtype
+        together = together and residual.get_device() == index
+    if torch.is_grad_enabled():
+        _need_no_gradient(*[t for t in (x, weight, bias, residual) if t is not None])
     float_type = nat.FLOAT_TYPES.get(dtype)
     if float_type is None:
         raise TypeError("linear takes float32, float16 or bfloat16")
-    if any([t.dtype is not dtype for t in others]):
+    if not alike:
         raise TypeError("linear inputs share one type")
-    if not x.is_cuda:
+    if index < 0:
         raise RuntimeError("linear inputs must be on the GPU: the kernels have no CPU path")
-    device, index = x.device, x.get_device()
-    if any([t.get_device() != index for t in others]):
+    if not together:
         raise ValueError("linear inputs must be on one device")
     out = x.new_empty(shape)
-    if not out.numel():
+    rows = out.numel() // outer if outer else 0
+    if not rows:
         return out
-    rows = out.numel() // outer
-    x, x_row = _matrix(x if x.ndim == 2 else x.reshape(rows, inner))
-    weight, weight_row = _matrix(weight)
+    device = out.device
+    x, x_row = _matrix(x if x.ndim == 2 else x.reshape(rows, inner), inner)
+    weight, weight_row = _matrix(weight, inner)
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
     residual_row = 0
     if residual is not None:
         residual, residual_row = _matrix(
-            residual if residual.ndim == 2 else residual.reshape(rows, outer))
+            residual if residual.ndim == 2 else residual.reshape(rows, outer), outer)
+    need = _workspace_bytes(rows, inner, outer, float_type)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     a = nat.Linear(x.data_ptr(), weight.data_ptr(), nat.ptr(bias), nat.ptr(residual),
                    out.data_ptr(), x_row, weight_row, residual_row, rows, inner, outer, float_type,
                    code)
-    lib = nat.lib()
-    need = lib.cowsdm_linear_workspace_bytes(rows, inner, outer, float_type)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    rc = lib.cowsdm_linear(a, nat.ptr(workspace), need, nat.stream_handle(device))
+    rc = nat.lib().cowsdm_linear(a, nat.ptr(workspace), need, nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_linear")
     return out

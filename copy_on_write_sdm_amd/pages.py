@@ -78,9 +78,10 @@ def _check_tables(lengths: torch.Tensor, page_tables: torch.Tensor, page_shares:
         raise ValueError("page tables take lengths [B], page_tables [B,columns], "
                          "page_shares [pages]")
     _need_device(lengths, "page tables")
-    batch, index = lengths.numel(), lengths.get_device()
-    columns, pages = page_tables.shape[1], page_shares.numel()
-    if page_tables.shape[0] != batch:
+    index = lengths.get_device()
+    batch, columns = page_tables.shape
+    pages = page_shares.shape[0]
+    if batch != lengths.shape[0]:
         raise ValueError("page tables must have a row for every request")
     _int32(lengths, batch, index, "lengths")
     _int32(page_tables, batch * columns, index, "page tables")
@@ -88,19 +89,6 @@ def _check_tables(lengths: torch.Tensor, page_tables: torch.Tensor, page_shares:
     if page_tokens not in PAGE_TOKENS:
         raise ValueError("a page holds 16, 32, 64, 128 or 256 tokens")
     return batch, columns, pages, index
-
-
-def _outputs(device: torch.device, *shapes: tuple[int, ...]) -> list[torch.Tensor]:
-    """int32 tensors of the shapes, in one allocation."""
-
-    sizes = []
-    for shape in shapes:
-        n = 1
-        for s in shape:
-            n *= s
-        sizes.append(n)
-    parts = torch.empty(sum(sizes), dtype=_INT32, device=device).split(sizes)
-    return [p if len(s) == 1 else p.view(s) for p, s in zip(parts, shapes)]
 
 
 def fork_page_tables(lengths: torch.Tensor, page_tables: torch.Tensor, page_shares: torch.Tensor,
@@ -127,11 +115,15 @@ def fork_page_tables(lengths: torch.Tensor, page_tables: torch.Tensor, page_shar
     _int32(tokens, n, index, "shared tokens")
     if n > MAX_REQUESTS:
         raise ValueError(f"at most {MAX_REQUESTS} requests are forked at once")
-    fork = PageFork(*_outputs(device, (n,), (n, columns), (pages,), (1,), (n,), (n,), (1,)))
+    sizes = (n, n * columns, pages, 1, n, n, 1)
+    held, tables, shares, count, sources, targets, overflow = torch.split_with_sizes(
+        torch.empty(sum(sizes), dtype=_INT32, device=device), sizes)
+    fork = PageFork(held, tables.view(n, columns), shares, count, sources, targets, overflow)
     rc = nat.lib().cowsdm_page_tables_fork(
         lengths.data_ptr(), page_tables.data_ptr(), batch, columns, page_shares.data_ptr(),
         free_pages.data_ptr(), pages, free_count.data_ptr(), parents.data_ptr(),
-        tokens.data_ptr(), n, page_tokens, *(t.data_ptr() for t in fork),
+        tokens.data_ptr(), n, page_tokens, held.data_ptr(), tables.data_ptr(), shares.data_ptr(),
+        count.data_ptr(), sources.data_ptr(), targets.data_ptr(), overflow.data_ptr(),
         nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_page_tables_fork")
@@ -161,8 +153,9 @@ def release_page_tables(lengths: torch.Tensor, page_tables: torch.Tensor,
         raise ValueError(f"at most {MAX_REQUESTS} requests are released at once")
     lib = nat.lib()
     need = lib.cowsdm_page_tables_release_workspace_bytes(pages, columns, n)
-    new_lengths, shares, count, workspace = _outputs(device, (batch,), (pages,), (1,),
-                                                     (need // 4,))
+    sizes = (batch, pages, 1, need // 4)
+    new_lengths, shares, count, workspace = torch.split_with_sizes(
+        torch.empty(sum(sizes), dtype=_INT32, device=device), sizes)
     rc = lib.cowsdm_page_tables_release(
         lengths.data_ptr(), page_tables.data_ptr(), batch, columns, page_shares.data_ptr(),
         free_pages.data_ptr(), pages, free_count.data_ptr(), requests.data_ptr(), n, page_tokens,
@@ -184,12 +177,14 @@ def compact_page_tables(lengths: torch.Tensor, page_tables: torch.Tensor,
     batch, columns, pages, index = _check_tables(lengths, page_tables, page_shares, page_tokens)
     device, lib = lengths.device, nat.lib()
     need = lib.cowsdm_page_tables_compact_workspace_bytes(pages)
-    *moves, workspace = _outputs(device, (batch, columns), (pages,), (pages,), (1,),
-                                 (pages // 2,), (pages // 2,), (need // 4,))
-    moves = PageMoves(*moves)
+    sizes = (batch * columns, pages, pages, 1, pages // 2, pages // 2, need // 4)
+    tables, shares, stack, count, sources, targets, workspace = torch.split_with_sizes(
+        torch.empty(sum(sizes), dtype=_INT32, device=device), sizes)
+    moves = PageMoves(tables.view(batch, columns), shares, stack, count, sources, targets)
     rc = lib.cowsdm_page_tables_compact(
         lengths.data_ptr(), page_tables.data_ptr(), batch, columns, page_shares.data_ptr(), pages,
-        page_tokens, *(t.data_ptr() for t in moves), workspace.data_ptr(), need,
+        page_tokens, tables.data_ptr(), shares.data_ptr(), stack.data_ptr(), count.data_ptr(),
+        sources.data_ptr(), targets.data_ptr(), workspace.data_ptr(), need,
         nat.stream_handle(device))
     if rc:
         nat.check(rc, "cowsdm_page_tables_compact")
@@ -208,11 +203,12 @@ def copy_pages(key_pages: torch.Tensor, key_scales: torch.Tensor, value_pages: t
         raise ValueError("cache keys must be [pages,heads,page_tokens,width], of all layers "
                          "with the layers before")
     _need_device(key_pages, "cache pages")
-    shape = tuple(key_pages.shape)
-    layers = shape[0] if len(shape) == 5 else 1
-    pages, heads, page_tokens, width = shape[-4:]
-    if (value_pages.shape != (*shape[:-2], width, page_tokens)
-            or key_scales.shape != shape[:-2] or value_scales.shape != shape[:-2]):
+    shape = key_pages.shape
+    *lead, pages, heads, page_tokens, width = shape
+    layers = lead[0] if lead else 1
+    each = shape[:-2]
+    if (value_pages.shape != (*each, width, page_tokens) or key_scales.shape != each
+            or value_scales.shape != each):
         raise ValueError("cache tensors do not align")
     if (key_pages.dtype is not CODES or value_pages.dtype is not CODES
             or key_scales.dtype is not _FLOAT32 or value_scales.dtype is not _FLOAT32):

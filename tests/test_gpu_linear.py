@@ -23,11 +23,14 @@ def normal(*shape, dtype, device, seed, scale=1.0):
 
 def assert_linear(x, weight, bias=None, activation=None, residual=None):
     """The sum of ``inner`` rounded products and the bias in float32 is off by
-    at most (inner + 2) 2^-24 of the terms' magnitudes.  No activation's slope
+    at most (inner + 2) 2^-24 of the terms' magnitudes (and by 2^-23 more
+    where float32 products are made of three parts of each number, whose least
+    products are left out).  No activation's slope
     is over 1.13.  An activation is off by at most 2^-21 of its argument:
     exponential and reciprocal are within 2^-22 and the rest within a few units
     of 2^-24, or 0.75e-7 for the approximated normal distribution.  The sum
-    with the residual rounds in float32 and once in the type."""
+    with the residual rounds in float32 and once in the type; what may lie
+    past its largest number may be infinite."""
 
     out = cow.linear(x, weight, bias, activation=activation, residual=residual)
     inner, outer = weight.shape[1], weight.shape[0]
@@ -37,12 +40,15 @@ def assert_linear(x, weight, bias=None, activation=None, residual=None):
         wide(x).reshape(rows, inner), wide(weight), None if bias is None else wide(bias),
         activation, None if residual is None else wide(residual).reshape(rows, outer))
     unit = UNIT[x.dtype]
-    error = (inner + 2) * 2.0 ** -24 * size
+    error = (inner + (4 if x.dtype is torch.float32 else 2)) * 2.0 ** -24 * size
     if activation is not None:
         error = 1.13 * error + 2.0 ** -21 * np.abs(before)
     error = error + 2.0 ** -24 * (np.abs(want) + error)
     error = error + unit * (np.abs(want) + error) + TINY[x.dtype]
-    off = np.abs(wide(out).reshape(rows, outer) - want) - error
+    got = wide(out).reshape(rows, outer)
+    past = np.abs(want) + error >= torch.finfo(x.dtype).max
+    past &= np.isinf(got) & ((got > 0) == (want > 0))
+    off = np.abs(np.where(past, want, got) - want) - error
     assert off.max() <= 0, (off.max(), int((off > 0).sum()), off.size)
     return out
 
@@ -90,7 +96,7 @@ def workspace(rows, inner, outer, dtype):
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("rows,inner,outer", [
     (100, 4000, 100), (20, 8192, 515), (70, 2056, 66), (128, 8192, 512), (64, 4096, 1024),
-    (256, 2568, 256), (1, 16384, 64), (65, 1096, 1)])
+    (256, 2568, 256), (1, 16384, 64), (65, 1096, 1), (2910, 7848, 1421)])
 def test_splits_of_the_summed_axis(device, dtype, rows, inner, outer):
     """Sums joined in a workspace: of aligned and of odd widths, with the
     epilogue in the join."""
@@ -153,6 +159,23 @@ def test_strides(device, dtype, rows):
     assert_linear(one, w[:1].expand(outer, inner), residual=residual[:1].expand(rows, outer))
     assert_linear(x.reshape(2, rows // 2, inner), w, residual=residual.reshape(2, -1, outer))
     assert_linear(x[0], w, residual=residual[0])
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(70, 64, 50), (300, 520, 260), (130, 4096, 40),
+                                              (4100, 40, 4100)])
+def test_float32_of_all_sizes(device, rows, inner, outer):
+    """Numbers of every binary order in one sum, the largest among them: what
+    three parts of 16 bits cannot hold is summed as it is."""
+
+    g = torch.Generator().manual_seed(40)
+    x = torch.randn(rows, inner, generator=g) * 2.0 ** torch.randint(-60, 20, (rows, inner),
+                                                                    generator=g)
+    w = torch.randn(outer, inner, generator=g) * 2.0 ** torch.randint(-20, 20, (outer, inner),
+                                                                     generator=g)
+    x[3, 1], w[5, 1] = 3.4028234e38, 0.5
+    x, w = x.to(device), w.to(device)
+    out = assert_linear(x, w)
+    assert bool(torch.isfinite(out[:, 5]).all()) and float(out[3, 5]) > 1.7e38
 
 
 @pytest.mark.parametrize("rows", [4, 60, 200])
