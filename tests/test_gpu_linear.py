@@ -178,6 +178,16 @@ def test_float32_of_all_sizes(device, rows, inner, outer):
     assert bool(torch.isfinite(out[:, 5]).all()) and float(out[3, 5]) > 1.7e38
 
 
+@pytest.mark.parametrize("power", [-100, -108, -116])
+def test_float32_near_the_smallest(device, power):
+    """Numbers whose later parts are below bfloat16's normal ones."""
+
+    x = normal(130, 72, dtype=torch.float32, device=device, seed=41) * 2.0 ** power
+    w = normal(200, 72, dtype=torch.float32, device=device, seed=42)
+    assert_linear(x, w)
+    assert_linear(w, x)
+
+
 @pytest.mark.parametrize("rows", [4, 60, 200])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_what_is_not_finite_stays_in_its_row_and_column(device, dtype, rows):
