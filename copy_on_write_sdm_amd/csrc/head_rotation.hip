@@ -15,6 +15,7 @@ namespace cowsdm_impl {
 constexpr int kHeadWaves = 4;
 constexpr int kHeadThreads = kHeadWaves * kWave;
 constexpr int kHeadMostWidth = 256;
+constexpr int kHeadTokens = 16, kHeadBytes = 16384, kHeadGroups = 4096;
 
 struct HeadParams {
   const void* query;
@@ -78,7 +79,11 @@ __device__ __forceinline__ void store_head(T* p, const float (&x)[C]) {
 // A workgroup takes some tokens: their points on the circle go to LDS, one a
 // thread, and then every row of a head is a few lanes', each with two chunks
 // of C elements that are rotated with each other (or, interleaved, each in
-// itself), so that nothing crosses lanes but the norm's sum.
+// itself), so that nothing crosses lanes but the norm's sum.  16 bytes a lane
+// are read and written where the width allows it.  Memory bounds it from some
+// 4,096 tokens on: 16,383 tokens of 40 heads 128 wide in bfloat16 (336 MB read
+// and written) take 63 us, 5.3 TB/s, what a large copy reaches.  64 of them
+// take 4.6 us: latency of a launch, the positions, the rows and the stores.
 template <typename T, int C, bool kInterleaved>
 __global__ __launch_bounds__(kHeadThreads) void rotate_heads_kernel(HeadParams p) {
   extern __shared__ __align__(16) char s_heads[];
@@ -172,7 +177,18 @@ void launch_heads(HeadParams p, bool interleaved, hipStream_t s) {
   const int need = p.width / (2 * C);
   p.lanes = 1;
   while (p.lanes < need) p.lanes *= 2;
-  p.tokens = p.rows >= 4096 ? 4 : 1;
+  // Tokens of a workgroup: few enough that its waves take their heads in one
+  // step (64 tokens of 40 heads 128 wide: 4.6 us with one each, 7.9 with four),
+  // but where there are many tokens enough that a workgroup's work outlasts its
+  // launch, some 2 ns (65,536 tokens, with one each and with 16 KB read and
+  // written each: 6 heads 64 wide in bfloat16 58 and 21 us, 24 heads 80 wide
+  // 134 and 104).
+  const int bytes_each = 2 * p.all_heads * p.width * static_cast<int>(sizeof(T));
+  const int one_step = kHeadWaves * kWave / p.lanes / p.all_heads;
+  const int enough = (kHeadBytes + bytes_each - 1) / bytes_each;
+  p.tokens = one_step < 1 ? 1 : one_step;
+  if (p.rows > kHeadGroups * p.tokens && p.tokens < enough) p.tokens = enough;
+  if (p.tokens > kHeadTokens) p.tokens = kHeadTokens;
   const int groups = (p.rows + p.tokens - 1) / p.tokens;
   const int bytes = 8 * p.width + 4 * p.tokens * p.rotated;
   if (interleaved)

@@ -88,6 +88,17 @@ def test_rows_and_heads(device, dtype, rows, heads, kv_heads):
         [(i * 7) % 2560 for i in range(rows)])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows", [4097, 4100])
+def test_some_tokens_to_a_workgroup(device, rows, interleaved):
+    """Heads whose tokens take a workgroup a step each, and more tokens than
+    that many workgroups are launched for: the last has one or two left."""
+
+    rotation = cow.HeadRotation(80, interleaved=interleaved, device=device)
+    run(device, torch.float16, rows, 16, 8, 80, rotation, (True, True),
+        [(i * 31) % 70000 for i in range(rows)])
+
+
 def test_sizes_of_the_norm(device):
     """Rows of zeros, the smallest and the largest numbers, with eps and none."""
 

@@ -118,6 +118,30 @@ def test_a_life(device, lengths, page, spare):
     assert state[3] == len(state[1]) and not any(state[1])
 
 
+@pytest.mark.parametrize("entries,pages,n", [
+    (8192, 8192, 1024), (8192 + 8, 8000, 1025), (8192, 8193, 64), (8184, 8192, 1023)])
+def test_where_one_workgroup_ends(device, entries, pages, n):
+    """The most entries, pages and requests that one workgroup takes, all of
+    them held, and one more of each."""
+
+    page, batch = 16, n
+    columns = entries // n
+    lengths = [page * columns - (i % 3) for i in range(batch)]
+    held = batch * columns
+    shares = [0] * pages
+    order = np.random.default_rng(n).permutation(pages)[:min(pages, held)]
+    tables = np.resize(order, held).reshape(batch, columns)      # wraps: shared pages
+    for p, c in zip(*np.unique(tables, return_counts=True)):
+        shares[p] = int(c) - 1
+    free = [p for p in range(pages) if p not in set(order.tolist())]
+    state = tables, shares, free + [-1] * (pages - len(free)), len(free)
+    assert_fork(device, lengths, state, list(range(batch))[::-1],
+                [page * (columns - 1)] * batch, page)
+    assert_compact(device, lengths, state, page)
+    _, left = assert_release(device, lengths, state, list(range(batch))[::-1], page)
+    assert left[3] == pages and not any(left[1])
+
+
 def test_fork_refused_as_a_whole(device):
     lengths, page = [40, 16, 0], 16
     state = pool(lengths, page, 2, 5)
