@@ -249,3 +249,22 @@ def test_the_residual_may_be_written_over(device):
                        rows, 64, 128, 2, 0)
         assert nat.lib().cowsdm_linear(a, None, 0, nat.stream_handle(device)) == 0
         assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("activation", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_activations_of_what_is_not_finite(device, dtype, activation):
+    """As the formulas have it: NaN stays, infinity stays, and minus infinity
+    times nothing is NaN (of relu 0); the largest numbers stay or vanish."""
+
+    x = torch.zeros(70, 8, dtype=dtype, device=device)
+    w = torch.zeros(6, 8, dtype=dtype, device=device)
+    most = torch.finfo(dtype).max
+    bias = torch.tensor([float("nan"), float("inf"), float("-inf"), most, -most, 0.0],
+                        dtype=dtype, device=device)
+    out = cow.linear(x, w, bias, activation=activation)
+    want = torch.tensor([float("nan"), float("inf"), 0.0 if activation == "relu" else float("nan"),
+                         most, 0.0, 0.0], dtype=dtype, device=device)
+    assert torch.equal(out.isnan(), want.isnan().expand(70, 6))
+    assert torch.equal(out.nan_to_num(nan=1.0, posinf=2.0), want.nan_to_num(nan=1.0, posinf=2.0)
+                       .expand(70, 6))
