@@ -699,49 +699,73 @@ __global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearPara
                  blockIdx.y);
 }
 
-// Operands that are not aligned: element by element into LDS, a step at a
-// time; 64 rows of each.  The loads' latency bounds it, as nothing is ahead.
+// Operands whose rows do not start on 16 bytes: 64 rows of each by a split of
+// the summed axis, from memory into registers, which a load of 16 bytes reaches
+// from any address, and on into LDS, a step ahead of the products.  What one
+// step ahead brings in bounds it: a row by 4095 x 6144 in bfloat16 14.7 us, 64
+// rows 30 (4096: 12.7 and 15), 1,111 rows by 2303 x 1544 in float16 34 (2304:
+// 18).  Element by element and nothing ahead they took 125, 173 and 117.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_odd_kernel(LinearParams p) {
   constexpr int B = 64, kThreads = 256;
-  constexpr int kEach = 16 / static_cast<int>(sizeof(T));
-  __shared__ __align__(16) char s_lines[2 * B * kLineBytes];
-  lds_char* const xs = (lds_char*)s_lines;
-  lds_char* const ws = xs + B * kLineBytes;
+  constexpr int kEach = 16 / static_cast<int>(sizeof(T)), kColumns = kLineChunks * kEach;
+  constexpr int kLoads = B * kLineChunks / kThreads, kStage = 2 * B * kLineBytes;
+  __shared__ __align__(16) char s_lines[2 * kStage];
+  lds_char* const lines = (lds_char*)s_lines;
   const int tid = static_cast<int>(threadIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   int m0, n0;
   tile_place<B, B>(p, gridDim.x, m0, n0);
+  const int begin = static_cast<int>(blockIdx.y) * p.chunk;
+  const int end = p.inner - begin < p.chunk ? p.inner : begin + p.chunk;
   const int wm = wave % 2 * 32, wn = wave / 2 * 32;
   f32x16 acc[1][1];
   clear(acc);
-  auto stage = [&](const void* base, int64_t stride, int first, int rows, int k, lds_char* to) {
+  u32x4 held[2][kLoads];
+  auto load = [&](int of, const void* base, int64_t stride, int first, int rows, int k) {
 #pragma unroll
-    for (int i = 0; i < B * kLineChunks / kThreads; ++i) {
-      const int q = i * kThreads + tid, row = q / kLineChunks;
-      const int column = k + line_chunk(row, q % kLineChunks) * kEach;
-      const T* const from = static_cast<const T*>(base) + (first + row) * stride + column;
-      T v[kEach];
+    for (int i = 0; i < kLoads; ++i) {
+      const int q = i * kThreads + tid, row = first + q / kLineChunks;
+      const int column = k + line_chunk(q / kLineChunks, q % kLineChunks) * kEach;
+      const T* const from = static_cast<const T*>(base) + row * stride + column;
+      u32x4 v = {0, 0, 0, 0};
+      if (row < rows && column + kEach <= end) {
+        __builtin_memcpy(&v, from, 16);
+      } else if (row < rows && column < end) {
+        T each[kEach];
 #pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        v[j] = first + row < rows && column + j < p.inner ? from[j] : static_cast<T>(0.0f);
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(to + q * 16) =
-          __builtin_bit_cast(u32x4, v);
+        for (int j = 0; j < kEach; ++j) each[j] = column + j < end ? from[j] : static_cast<T>(0.0f);
+        v = __builtin_bit_cast(u32x4, each);
+      }
+      held[of][i] = v;
     }
   };
-  for (int k = 0; k < p.inner; k += kLineChunks * kEach) {
-    stage(p.x, p.x_row, m0, p.rows, k, xs);
-    stage(p.weight, p.weight_row, n0, p.outer, k, ws);
+  auto load_step = [&](int k) {
+    load(0, p.x, p.x_row, m0, p.rows, k);
+    load(1, p.weight, p.weight_row, n0, p.outer, k);
+  };
+  load_step(begin);
+  for (int k = begin, stage = 0; k < end; k += kColumns, stage ^= 1) {
+    lds_char* const xs = lines + stage * kStage;
+    lds_char* const ws = xs + B * kLineBytes;
+#pragma unroll
+    for (int of = 0; of < 2; ++of)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(
+            (of ? ws : xs) + (i * kThreads + tid) * 16) = held[of][i];
     __syncthreads();
+    load_step(k + kColumns);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       Operands<T, 1, 1> now;
       now.read(ws, xs, wn, wm, s);
       now.multiply(acc);
     }
-    __syncthreads();
   }
-  finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * 8, m0 + wm, n0 + wn, 0);
+  __syncthreads();
+  finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * 8, m0 + wm, n0 + wn,
+                 blockIdx.y);
 }
 
 // --------------------------------------------------------------- few rows
@@ -869,7 +893,7 @@ constexpr int64_t tiles_of(int64_t rows, int64_t outer, int bm, int bn) {
   return ((rows + bm - 1) / bm) * ((outer + bn - 1) / bn);
 }
 
-enum class LinearForm { kFew, k64, k64x128, k128, k256 };
+enum class LinearForm { kOdd, kFew, k64, k64x128, k128, k256 };
 struct LinearPlan {
   LinearForm form;
   int splits;
@@ -896,9 +920,6 @@ template <typename T>
 int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipStream_t s) {
   p.splits = 1;
   p.chunk = p.inner;
-  if (!aligned)
-    return launch_groups(&linear_odd_kernel<T>, tiles_of(p.rows, p.outer, 64, 64), 1, 256, 0, p,
-                         s);
   if (plan.splits > 1) {
     constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));
     const int steps = (p.inner + kEach - 1) / kEach;
@@ -906,7 +927,11 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
     p.chunk = (steps + plan.splits - 1) / plan.splits * kEach;
   }
   int32_t e = 0;
-  switch (plan.form) {
+  switch (aligned ? plan.form : LinearForm::kOdd) {
+    case LinearForm::kOdd:
+      e = launch_groups(&linear_odd_kernel<T>, tiles_of(p.rows, p.outer, 64, 64), p.splits, 256, 0,
+                        p, s);
+      break;
     case LinearForm::kFew:
       if (p.rows <= 16) return launch_few<T, 1>(p, s);
       if (p.rows <= 32) return launch_few<T, 2>(p, s);
@@ -927,7 +952,8 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
 // What a form takes of a call's sizes, in microseconds: rounds of workgroups,
 // each so long a step of 128 bytes and so long at its ends, or the memory's
 // time, and, where the summed axis is split, the join's launch and traffic.
-// The least one runs.  The constants are fitted to calls on one MI355X, which
+// The least one runs; where rows cannot all be aligned, the odd form's splits
+// are chosen the same way.  The constants are fitted to calls on one MI355X, which
 // they give within some 20 %; in bfloat16, by the forms (splits):
 //   64 rows, 128 x 384: few 3.2, tiles of 64 3.8; 32 rows, 8192 x 512: few 23,
 //   64 (16) 9.6; a row, 4096 x 6144: few 12.7, 64 x 128 (5) 12.5; 64 rows: few
@@ -945,6 +971,7 @@ struct FormCost {
   float step[2], ends;             // of 16-bit types, and of float32
 };
 constexpr FormCost kFormCosts[] = {
+    {LinearForm::kOdd, 64, 64, {0.45f, 0.8f}, 1.0f},
     {LinearForm::k64, 64, 64, {0.30f, 0.57f}, 1.0f},
     {LinearForm::k64x128, 64, 128, {0.38f, 0.85f}, 1.0f},
     {LinearForm::k128, 128, 128, {0.58f, 1.4f}, 2.5f},
@@ -964,13 +991,15 @@ LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size) {
       best = {form, splits};
     }
   };
-  if (rows <= kFewRows) {
+  const bool odd = inner * size % 16 != 0;
+  if (rows <= kFewRows && !odd) {
     const int64_t rounds = ((outer + 15) / 16 + kChipCus - 1) / kChipCus;
     const float us = static_cast<float>(rounds * (16 + rows) * inner * size) * (1.0f / 36.0e3f);
     consider(LinearForm::kFew, 1, 2.3f + (us > memory ? us : memory));
   }
   const int64_t steps = (inner * size + kLineBytes - 1) / kLineBytes;
   for (const FormCost& f : kFormCosts) {
+    if (odd != (f.form == LinearForm::kOdd)) continue;
     const int64_t tiles = tiles_of(rows, outer, f.rows, f.columns);
     const int most = tiles >= kChipCus ? 4 : kMostSplits;
     for (int splits = 1; splits <= most && splits <= steps; ++splits) {
@@ -1050,7 +1079,7 @@ extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace,
                     (address(l.out) | address(l.bias) | address(l.residual)) % (4 * size) == 0;
   const bool aligned = linear_aligned(l);
   const LinearPlan plan = plan_linear(l.rows, l.inner, l.outer, static_cast<int>(size));
-  if (aligned && plan.splits > 1) {
+  if (plan.splits > 1) {
     const int64_t need = workspace_of(plan, l.rows, l.outer);
     if (!workspace || workspace_bytes < need)
       return fail(COWSDM_EARG, "linear: workspace of %lld bytes needed",

@@ -30,8 +30,8 @@ def _workspace_bytes(rows: int, inner: int, outer: int, float_type: int) -> int:
 
 def _matrix(tensor: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
     """A matrix whose rows can be read, and the elements between them: itself
-    or a contiguous copy.  (Rows that are contiguous but not aligned are read
-    element by element by the kernel, which costs less than a copy.)"""
+    or a contiguous copy.  (Rows that are contiguous but not aligned go through
+    a kernel of their own, which costs less than a copy.)"""
 
     row, column = tensor.stride()
     if column != 1 and columns > 1 or row > _MOST:

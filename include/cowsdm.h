@@ -975,8 +975,8 @@ int32_t cowsdm_pages_copy(const cowsdm_kv_cache_t* cache, int64_t layers, const 
  * [outer, inner] (rows of both contiguous), out [rows, outer] contiguous; bias
  * [outer] and residual [rows, outer] may be null.  All of one type; sums and
  * the rest in 32 bits, rounded once.  Any sizes and strides; operands whose
- * addresses, widths or strides are no multiples of 16 bytes are loaded
- * element by element.  out is none of the inputs, but may be the residual.
+ * addresses, widths and strides are multiples of 16 bytes are read fastest.
+ * out is none of the inputs, but may be the residual (of the same strides).
  * An inner size of 0 gives activation(bias) + residual. */
 typedef struct cowsdm_linear {
   const void* x;

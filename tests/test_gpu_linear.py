@@ -268,3 +268,23 @@ def test_activations_of_what_is_not_finite(device, dtype, activation):
     assert torch.equal(out.isnan(), want.isnan().expand(70, 6))
     assert torch.equal(out.nan_to_num(nan=1.0, posinf=2.0), want.nan_to_num(nan=1.0, posinf=2.0)
                        .expand(70, 6))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,inner,outer", [
+    (100, 4001, 100), (1, 8191, 65), (70, 2055, 66), (64, 4096, 1024), (2910, 2504, 131),
+    (130, 63, 600), (130, 65, 600)])
+def test_splits_of_rows_that_are_not_aligned(device, dtype, rows, inner, outer):
+    """Widths that no row of which is aligned, and operands that start one
+    element past an aligned address, between NaN."""
+
+    def loose(count, seed, scale=1.0):
+        flat = torch.full((count * inner + 16,), float("nan"), dtype=dtype, device=device)
+        part = flat[1:1 + count * inner].view(count, inner)
+        part.copy_(normal(count, inner, dtype=dtype, device=device, seed=seed, scale=scale))
+        return part
+
+    x, w = loose(rows, 50), loose(outer, 51, inner ** -0.5)
+    assert x.data_ptr() % 16 and w.data_ptr() % 16
+    assert_linear(x, w, normal(outer, dtype=dtype, device=device, seed=52), "silu",
+                  normal(rows, outer, dtype=dtype, device=device, seed=53))
