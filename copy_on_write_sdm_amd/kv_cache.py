@@ -246,8 +246,9 @@ class PagedKVCache:
         the pages freed."""
 
         named = [int(r) for r in requests]
-        if (len(set(named)) != len(named) or any(not 0 <= r < self.requests for r in named)
-                or self._released & set(named)):
+        gone = set(named)
+        if (len(gone) != len(named) or any(not 0 <= r < self.requests for r in named)
+                or self._released & gone):
             raise ValueError("released sequence is invalid, duplicated, or inactive")
         if not named:
             return 0
@@ -270,8 +271,8 @@ class PagedKVCache:
         self._before = None
         for r in named:
             self._lengths[r] = 0
-        self._shared = [() if r in set(named) else s for r, s in enumerate(self._shared)]
-        self._released |= set(named)
+        self._shared = [() if r in gone else s for r, s in enumerate(self._shared)]
+        self._released |= gone
         self._free += freed
         return freed
 
