@@ -166,28 +166,24 @@ __device__ __forceinline__ void finish4(const LinearParams& p, int m, int n, f32
 }
 
 // A wave's sums of 32 NT columns by 32 MT rows of the output, as the products
-// leave them, through LDS (32 rows of its own at a time), so that a store
-// writes whole rows of its columns.  Chunks of four are permuted against the
-// banks.  A lane keeps to four columns, whose bias it loads once.
-template <typename T, int NT, int MT>
-__device__ __forceinline__ void finish_tile(const LinearParams& p, const f32x16 (&acc)[NT][MT],
-                                            f32x4* turned, int m0, int n0, int split) {
+// leave them, through LDS (32 rows of its own at a time, which `put` writes in
+// chunks of four columns), so that a store writes whole rows of its columns.
+// Chunks are permuted against the banks.  A lane keeps to four columns, whose
+// bias it loads once.
+template <typename T, int NT, int MT, typename Put>
+__device__ __forceinline__ void finish_rows(const LinearParams& p, Put put, f32x4* turned, int m0,
+                                            int n0, int split) {
   constexpr int kChunks = NT * 8, kRows = kWave / kChunks;      // rows of a step
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const int row = lane & 31, half = lane >> 5;
   const int c = lane % kChunks, n = n0 + c * 4;
   const bool in = n < p.outer;
   f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
   if (p.wide && p.bias && p.splits == 1 && in) bias = load4(static_cast<const T*>(p.bias) + n);
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        turned[row * kChunks + ((t * 8 + g * 2 + half) ^ (row & (kChunks - 1)))] =
-            f32x4{acc[t][u][4 * g], acc[t][u][4 * g + 1], acc[t][u][4 * g + 2],
-                  acc[t][u][4 * g + 3]};
+    put(u, [&](int r, int chunk) -> f32x4& {
+      return turned[r * kChunks + (chunk ^ (r & (kChunks - 1)))];
+    });
     const int first = m0 + u * 32;
     auto at = [&](int r) { return turned[r * kChunks + (c ^ (r & (kChunks - 1)))]; };
     if (p.splits > 1) {
@@ -237,6 +233,23 @@ __device__ __forceinline__ void finish_tile(const LinearParams& p, const f32x16 
       }
     }
   }
+}
+
+// The same of sums that lie as products of 32 by 32 leave them.
+template <typename T, int NT, int MT>
+__device__ __forceinline__ void finish_tile(const LinearParams& p, const f32x16 (&acc)[NT][MT],
+                                            f32x4* turned, int m0, int n0, int split) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int row = lane & 31, half = lane >> 5;
+  auto put = [&](int u, auto place) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        place(row, t * 8 + g * 2 + half) = f32x4{acc[t][u][4 * g], acc[t][u][4 * g + 1],
+                                                 acc[t][u][4 * g + 2], acc[t][u][4 * g + 3]};
+  };
+  finish_rows<T, NT, MT>(p, put, turned, m0, n0, split);
 }
 
 // The splits' sums, added in their order, and the epilogue: a launch and one
@@ -469,8 +482,8 @@ constexpr int kSteps = kLineChunks / 2;      // product steps of a line
 
 // Workgroup n runs on XCD n % 8, each of which takes a run of tiles, some rows
 // of tiles at a time, so that what an XCD works on at once shares its L2.  Rows
-// of 256 at a time: 7,919 x 4,096 by 16,384 takes 862 us with 1, 813 with 3, 816
-// with 4, 842 with 8.  Smaller tiles, 4 against 8: 1,024 x 4,096 by 4,096 in
+// of 256 at a time (by products of 32 by 32): 7,919 x 4,096 by 16,384 takes 862
+// us with 1, 813 with 3, 816 with 4, 842 with 8.  Smaller tiles, 4 against 8: 1,024 x 4,096 by 4,096 in
 // 128 x 128 39.4 against 38.9 us, 1,111 x 2,304 by 1,544 in 64 x 128 17.8 against
 // 17.5, in 64 x 64 17.4 against 16.8.
 template <int BM, int BN>
@@ -491,15 +504,103 @@ __device__ __forceinline__ void tile_place(const LinearParams& p, int groups, in
 // used, one and a half steps' are on their way.  When a step's lines have all
 // been read, W of two steps on takes the place of its x, and x of three steps
 // on that of its W.  (With two whole steps in LDS, each waited for as a whole,
-// the first case below took 1,030 us; with steps of 64 bytes, or four waves of
-// 128 by 128, more than 940.)
+// the first case below took a quarter longer; with steps of 64 bytes, or four
+// waves of 128 by 128, a sixth.)
 //
-// The matrix cores bound it, at the clock that the power leaves: 7,919 rows by
-// 4096 x 16384 in bfloat16 take 806 us, 1,320 TFLOP/s, with the matrix cores
-// busy two thirds of the cycles at 1.7 GHz.  GELU in the epilogue adds 80: it
-// fills the vector units, and no other workgroup is on the CU meanwhile.
+// Half of a wave's rows of x are multiplied while the other half's next ones
+// are read.  The matrix cores bound it, at the clock that the power leaves:
+// 7,919 rows by 4096 x 16384 in bfloat16 take 772 us, 1,380 TFLOP/s.  Products of
+// 32 by 32 by 16, which do as much a cycle, took 843, with the matrix cores busy
+// two thirds of the cycles at 1.7 GHz.  GELU in the epilogue adds 35: it fills
+// the vector units, and no other workgroup is on the CU meanwhile.
 template <typename T>
 __global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
+  constexpr int B = 256, kThreads = 512, MT = 8, NT = 4, kHalf = MT / 2;
+  constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));   // columns a step
+  constexpr int kSlot = B * kLineBytes, kSlots = 5;
+  constexpr int kLoads = Lines<T, B, kThreads>::kLoads;
+  extern __shared__ __align__(16) char s_lines[];
+  lds_char* const lines = (lds_char*)s_lines;
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  int m0, n0;
+  tile_place<B, B>(p, gridDim.x, m0, n0);
+  const int begin = static_cast<int>(blockIdx.y) * p.chunk;
+  const int end = p.inner - begin < p.chunk ? p.inner : begin + p.chunk;
+  const Lines<T, B, kThreads> x(p.x, p.x_row, m0, p.rows, p.inner);
+  const Lines<T, B, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
+  const int wm = wave % 2 * 128, wn = wave / 2 * 64;
+  const int row = lane & 15, quarter = lane >> 4;
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  u32x4 a[2][NT], b[MT];
+  // a wave's rows of W, and half of its rows of x, half a line each
+  auto read_w = [&](u32x4 (&to)[NT], int slot, int s) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      to[t] = line_read(lines + slot * kSlot, wn + t * 16 + row, 4 * s + quarter);
+  };
+  auto read_x = [&](int half, int slot, int s) {
+#pragma unroll
+    for (int u = half * kHalf; u < half * kHalf + kHalf; ++u)
+      b[u] = line_read(lines + slot * kSlot, wm + u * 16 + row, 4 * s + quarter);
+  };
+  auto multiply = [&](const u32x4 (&v)[NT], int half) {
+#pragma unroll
+    for (int u = half * kHalf; u < half * kHalf + kHalf; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t][u] = Product<T>::narrow(v[t], b[u], acc[t][u]);
+  };
+  auto further = [&](int slot) { return slot + 2 < kSlots ? slot + 2 : slot + 2 - kSlots; };
+  x.load(lines, begin, end);
+  w.load(lines + kSlot, begin, end);
+  x.load(lines + 2 * kSlot, begin + kEach, end);
+  w.load(lines + 3 * kSlot, begin + kEach, end);
+  arrive<2 * kLoads>();
+  int xs = 0, ws = 1, spare = 4;           // slots of this step's x and W, and of the last one's W
+  read_w(a[0], ws, 0);
+  read_x(0, xs, 0);
+  read_x(1, xs, 0);
+  for (int k = begin; k < end; k += kEach) {
+    const int xn = further(xs), wx = further(ws);
+    read_w(a[1], ws, 1);
+    // not at once with W's, so that those come first
+    x.load(lines + spare * kSlot, k + 2 * kEach, end);
+    multiply(a[0], 0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_x(0, xs, 1);
+    multiply(a[0], 1);
+    __builtin_amdgcn_sched_barrier(0);
+    read_x(1, xs, 1);
+    multiply(a[1], 0);
+    arrive<kLoads>();                      // all but x of two steps on
+    read_w(a[0], wx, 0);
+    read_x(0, xn, 0);
+    w.load(lines + xs * kSlot, k + 2 * kEach, end);
+    multiply(a[1], 1);
+    __builtin_amdgcn_sched_barrier(0);
+    read_x(1, xn, 0);
+    spare = ws;
+    xs = xn;
+    ws = wx;
+  }
+  arrive<0>();
+  auto put = [&](int u, auto place) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) place(g * 16 + row, t * 4 + quarter) = acc[t][2 * u + g];
+  };
+  finish_rows<T, NT / 2, MT / 2>(p, put, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 4,
+                                 m0 + wm, n0 + wn, blockIdx.y);
+}
+
+// The same of float32, by thirds.
+__global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p) {
+  typedef float T;
   constexpr int B = 256, kThreads = 512, MT = 4, NT = 2;
   constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));   // columns a step
   constexpr int kSlot = B * kLineBytes, kSlots = 5;
@@ -515,78 +616,46 @@ __global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
   const Lines<T, B, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
   const int wm = wave % 2 * 128, wn = wave / 2 * 64;
   f32x16 acc[NT][MT];
-  auto start = [&]() {
+  auto further = [&](int slot) { return slot + 2 < kSlots ? slot + 2 : slot + 2 - kSlots; };
+  auto sums = [&](auto thirds) {
     clear(acc);
     x.load(lines, begin, end);
     w.load(lines + kSlot, begin, end);
     x.load(lines + 2 * kSlot, begin + kEach, end);
     w.load(lines + 3 * kSlot, begin + kEach, end);
     arrive<2 * kLoads>();
-  };
-  auto further = [&](int slot) { return slot + 2 < kSlots ? slot + 2 : slot + 2 - kSlots; };
-  if constexpr (sizeof(T) == 4) {
-    auto sums = [&](auto thirds) {
-      start();
-      x.load(lines + 4 * kSlot, begin + 2 * kEach, end);
-      for (int k = begin, xs = 0, ws = 1; k < end; k += kEach) {
+    x.load(lines + 4 * kSlot, begin + 2 * kEach, end);
+    for (int k = begin, xs = 0, ws = 1; k < end; k += kEach) {
 #pragma unroll
-        for (int j = 0; j < kSteps / 2; ++j) {
-          FloatOperands<NT, MT> now;
-          now.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, j);
-          if constexpr (decltype(thirds)::value) {
-            // one row of tiles' thirds at a time, as registers allow
-            u32x4 a[NT][3], b[3];
+      for (int j = 0; j < kSteps / 2; ++j) {
+        FloatOperands<NT, MT> now;
+        now.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, j);
+        if constexpr (decltype(thirds)::value) {
+          // one row of tiles' thirds at a time, as registers allow
+          u32x4 a[NT][3], b[3];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) to_thirds(now.a[t], a[t]);
+          for (int t = 0; t < NT; ++t) to_thirds(now.a[t], a[t]);
 #pragma unroll
-            for (int u = 0; u < MT; ++u) {
-              to_thirds(now.b[u], b);
+          for (int u = 0; u < MT; ++u) {
+            to_thirds(now.b[u], b);
 #pragma unroll
-              for (int t = 0; t < NT; ++t) acc[t][u] = thirds_product(a[t], b, acc[t][u]);
-            }
-          } else {
-            now.multiply(acc);
+            for (int t = 0; t < NT; ++t) acc[t][u] = thirds_product(a[t], b, acc[t][u]);
           }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        arrive<kLoads>();                  // all but x of two steps on
-        w.load(lines + xs * kSlot, k + 2 * kEach, end);
-        x.load(lines + ws * kSlot, k + 3 * kEach, end);
-        xs = further(xs);
-        ws = further(ws);
-      }
-      arrive<0>();
-    };
-    sums(std::true_type());
-    if (any_not_finite(acc, reinterpret_cast<int*>(s_lines))) sums(std::false_type());
-  } else {
-    start();
-    Operands<T, NT, MT> now[2];
-    int xs = 0, ws = 1, spare = 4;         // slots of this step's x and W, and of the last one's W
-    now[0].read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, 0);
-    for (int k = begin; k < end; k += kEach) {
-      const int xn = further(xs), wx = further(ws);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        Operands<T, NT, MT>& next = now[(s + 1) & 1];
-        if (s < kSteps - 1) {
-          next.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, s + 1);
-          // not at once with W's, so that those come first
-          if (s == 0) x.load(lines + spare * kSlot, k + 2 * kEach, end);
         } else {
-          arrive<kLoads>();                // all but x of two steps on
-          next.read(lines + wx * kSlot, lines + xn * kSlot, wn, wm, 0);
-          w.load(lines + xs * kSlot, k + 2 * kEach, end);
+          now.multiply(acc);
         }
-        now[s & 1].multiply(acc);
         __builtin_amdgcn_sched_barrier(0);
       }
-      spare = ws;
-      xs = xn;
-      ws = wx;
+      arrive<kLoads>();                    // all but x of two steps on
+      w.load(lines + xs * kSlot, k + 2 * kEach, end);
+      x.load(lines + ws * kSlot, k + 3 * kEach, end);
+      xs = further(xs);
+      ws = further(ws);
     }
     arrive<0>();
-  }
+  };
+  sums(std::true_type());
+  if (any_not_finite(acc, reinterpret_cast<int*>(s_lines))) sums(std::false_type());
   finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 8, m0 + wm, n0 + wn,
                  blockIdx.y);
 }
@@ -939,10 +1008,13 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
     case LinearForm::k64: e = launch_tiles<T, 64, 64, 2, 2, 4>(p, s); break;
     case LinearForm::k64x128: e = launch_tiles<T, 64, 128, 2, 2, 4>(p, s); break;
     case LinearForm::k128: e = launch_tiles<T, 128, 128, 2, 2, 4>(p, s); break;
-    case LinearForm::k256:
-      e = launch_groups(&linear_large_kernel<T>, tiles_of(p.rows, p.outer, 256, 256), p.splits, 512,
+    case LinearForm::k256: {
+      void (*kernel)(LinearParams) = &linear_large_float_kernel;
+      if constexpr (sizeof(T) == 2) kernel = &linear_large_kernel<T>;
+      e = launch_groups(kernel, tiles_of(p.rows, p.outer, 256, 256), p.splits, 512,
                         5 * 256 * kLineBytes, p, s);
       break;
+    }
   }
   if (e || p.splits == 1) return e;
   const int64_t chunks = static_cast<int64_t>(p.rows) * ((p.outer + 3) / 4);
@@ -959,10 +1031,10 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
 //   64 (16) 9.6; a row, 4096 x 6144: few 12.7, 64 x 128 (5) 12.5; 64 rows: few
 //   38, 64 (2) 15.3, 64 x 128 (4) 15.0, 64 x 128 (1) 24
 //   100 rows, 4000 x 100: 64 (16) 7.4, 64 (1) 19
-//   2,910 rows, 7848 x 1420: 128 149, 128 (3) 116, 256 148, 256 (3) 81
-//   1,111 rows, 2304 x 1544: 64 17.8, 64 x 128 17.0, 128 23, 256 44
-//   2,048 rows, 2048 x 2048: 64 31, 64 x 128 30, 128 24, 256 42
-//   4,096 rows, 4096 x 4096: 64 216, 64 x 128 200, 128 162, 256 108
+//   2,910 rows, 7848 x 1420: 128 148, 128 (3) 121, 256 151, 256 (3) 76
+//   1,111 rows, 2304 x 1544: 64 16.7, 64 x 128 16.4, 128 23, 256 46
+//   2,048 rows, 2048 x 2048: 64 29, 64 x 128 29, 128 23, 256 44
+//   4,096 rows, 4096 x 4096: 64 209, 64 x 128 197, 128 153, 256 100
 //   and in float32 4,000 rows, 4000 x 4000: 64 962, 64 x 128 909, 128 704, 256
 //   627; 256 rows, 2048 x 2048: 64 42, 64 (4) 26, 64 x 128 (4) 25.
 struct FormCost {
@@ -975,7 +1047,7 @@ constexpr FormCost kFormCosts[] = {
     {LinearForm::k64, 64, 64, {0.30f, 0.57f}, 1.0f},
     {LinearForm::k64x128, 64, 128, {0.38f, 0.85f}, 1.0f},
     {LinearForm::k128, 128, 128, {0.58f, 1.4f}, 2.5f},
-    {LinearForm::k256, 256, 256, {1.58f, 4.9f}, 4.0f},
+    {LinearForm::k256, 256, 256, {1.45f, 4.9f}, 4.0f},
 };
 constexpr int64_t kChipCus = 256;
 constexpr int kMostSplits = 16;
