@@ -396,7 +396,7 @@ struct FloatOperands {
 // within 2^-23 of the product (a third is within 2^-8 of the one before).  A
 // number that is not finite, or within 2^-9 of the largest, gives NaN this
 // way: such sums are done again by float32 products.  4,000 rows by 4000 x
-// 4000, tiles of 256: 627 us, and 911 by float32 products; 2,048 by 2048 x
+// 4000, tiles of 256: 579 us, and 911 by float32 products; 2,048 by 2048 x
 // 2048, tiles of 128: 96 and 135.
 //
 // Pairs are rounded together, and a third is taken off as it stands in the
@@ -418,14 +418,9 @@ __device__ __forceinline__ void to_thirds(const u32x4 (&v)[2], u32x4 (&out)[3]) 
   }
 }
 
-// One row of W's thirds by one of x's.
-__device__ __forceinline__ f32x16 thirds_product(const u32x4 (&p)[3], const u32x4 (&q)[3],
-                                                 f32x16 c) {
-  constexpr int kLeft[6] = {2, 0, 1, 1, 0, 0}, kRight[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-  for (int i = 0; i < 6; ++i) c = Product<__bf16>::wide(p[kLeft[i]], q[kRight[i]], c);
-  return c;
-}
+// The products that count: which thirds of the left and of the right.
+constexpr int kThirds = 6;
+constexpr int kOfLeft[kThirds] = {2, 0, 1, 1, 0, 0}, kOfRight[kThirds] = {0, 2, 1, 0, 1, 0};
 
 template <int NT, int MT>
 struct Thirds {
@@ -437,28 +432,28 @@ struct Thirds {
     for (int t = 0; t < MT; ++t) to_thirds(raw.b[t], b[t]);
   }
   __device__ __forceinline__ void multiply(f32x16 (&acc)[NT][MT]) const {
-    constexpr int kLeft[6] = {2, 0, 1, 1, 0, 0}, kRight[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-    for (int i = 0; i < 6; ++i)
+    for (int i = 0; i < kThirds; ++i)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int u = 0; u < MT; ++u)
-          acc[t][u] = Product<__bf16>::wide(a[t][kLeft[i]], b[u][kRight[i]], acc[t][u]);
+          acc[t][u] = Product<__bf16>::wide(a[t][kOfLeft[i]], b[u][kOfRight[i]], acc[t][u]);
   }
 };
 
 // Whether a sum of the workgroup's is not finite; by way of a word of the LDS
 // that its lines have left.
-template <int NT, int MT>
-__device__ __forceinline__ bool any_not_finite(const f32x16 (&acc)[NT][MT], int* word) {
+template <typename Acc, int NT, int MT>
+__device__ __forceinline__ bool any_not_finite(const Acc (&acc)[NT][MT], int* word) {
   float sum = 0.0f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int u = 0; u < MT; ++u)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[t][u][i], 0.0f, sum);
+      for (int i = 0; i < static_cast<int>(sizeof(Acc) / 4); ++i)
+        sum = __builtin_fmaf(acc[t][u][i], 0.0f, sum);
   if (threadIdx.x == 0) *word = 0;
   __syncthreads();
   if (sum != 0.0f) *word = 1;
@@ -468,14 +463,14 @@ __device__ __forceinline__ bool any_not_finite(const f32x16 (&acc)[NT][MT], int*
   return any;
 }
 
-template <int NT, int MT>
-__device__ __forceinline__ void clear(f32x16 (&acc)[NT][MT]) {
+template <typename Acc, int NT, int MT>
+__device__ __forceinline__ void clear(Acc (&acc)[NT][MT]) {
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int u = 0; u < MT; ++u)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][u][i] = 0.0f;
+      for (int i = 0; i < static_cast<int>(sizeof(Acc) / 4); ++i) acc[t][u][i] = 0.0f;
 }
 
 constexpr int kSteps = kLineChunks / 2;      // product steps of a line
@@ -483,9 +478,9 @@ constexpr int kSteps = kLineChunks / 2;      // product steps of a line
 // Workgroup n runs on XCD n % 8, each of which takes a run of tiles, some rows
 // of tiles at a time, so that what an XCD works on at once shares its L2.  Rows
 // of 256 at a time (by products of 32 by 32): 7,919 x 4,096 by 16,384 takes 862
-// us with 1, 813 with 3, 816 with 4, 842 with 8.  Smaller tiles, 4 against 8: 1,024 x 4,096 by 4,096 in
-// 128 x 128 39.4 against 38.9 us, 1,111 x 2,304 by 1,544 in 64 x 128 17.8 against
-// 17.5, in 64 x 64 17.4 against 16.8.
+// us with 1, 813 with 3, 816 with 4, 842 with 8.  Smaller tiles, 4 against 8:
+// 1,024 x 4,096 by 4,096 in 128 x 128 39.4 against 38.9 us, 1,111 x 2,304 by 1,544
+// in 64 x 128 17.8 against 17.5, in 64 x 64 17.4 against 16.8.
 template <int BM, int BN>
 __device__ __forceinline__ void tile_place(const LinearParams& p, int groups, int& m0, int& n0) {
   constexpr int kBand = BM == 256 ? 4 : 8;
@@ -532,10 +527,7 @@ __global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
   const int wm = wave % 2 * 128, wn = wave / 2 * 64;
   const int row = lane & 15, quarter = lane >> 4;
   f32x4 acc[NT][MT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int u = 0; u < MT; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  clear(acc);
   u32x4 a[2][NT], b[MT];
   // a wave's rows of W, and half of its rows of x, half a line each
   auto read_w = [&](u32x4 (&to)[NT], int slot, int s) {
@@ -598,15 +590,19 @@ __global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
                                  m0 + wm, n0 + wn, blockIdx.y);
 }
 
-// The same of float32, by thirds.
+// The same of float32, by thirds: of a line of W's rows at once, and of one row
+// of tiles of x's at a time, as registers allow.  Matrix cores and vector units
+// (the thirds) bound it: 4,000 rows by 4000 x 4000 take 579 us, 221 TFLOP/s (633
+// by products of 32 by 32).
 __global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p) {
   typedef float T;
-  constexpr int B = 256, kThreads = 512, MT = 4, NT = 2;
+  constexpr int B = 256, kThreads = 512, MT = 8, NT = 4;
   constexpr int kEach = kLineBytes / static_cast<int>(sizeof(T));   // columns a step
   constexpr int kSlot = B * kLineBytes, kSlots = 5;
   constexpr int kLoads = Lines<T, B, kThreads>::kLoads;
   extern __shared__ __align__(16) char s_lines[];
   lds_char* const lines = (lds_char*)s_lines;
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   int m0, n0;
   tile_place<B, B>(p, gridDim.x, m0, n0);
@@ -615,8 +611,14 @@ __global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p)
   const Lines<T, B, kThreads> x(p.x, p.x_row, m0, p.rows, p.inner);
   const Lines<T, B, kThreads> w(p.weight, p.weight_row, n0, p.outer, p.inner);
   const int wm = wave % 2 * 128, wn = wave / 2 * 64;
-  f32x16 acc[NT][MT];
+  const int row = lane & 15, quarter = lane >> 4;
+  f32x4 acc[NT][MT];
   auto further = [&](int slot) { return slot + 2 < kSlots ? slot + 2 : slot + 2 - kSlots; };
+  auto read = [&](u32x4 (&to)[2], int slot, int first) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      to[c] = line_read(lines + slot * kSlot, first + row, 2 * quarter + c);
+  };
   auto sums = [&](auto thirds) {
     clear(acc);
     x.load(lines, begin, end);
@@ -626,25 +628,33 @@ __global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p)
     arrive<2 * kLoads>();
     x.load(lines + 4 * kSlot, begin + 2 * kEach, end);
     for (int k = begin, xs = 0, ws = 1; k < end; k += kEach) {
+      u32x4 a[NT][2], b[2];
 #pragma unroll
-      for (int j = 0; j < kSteps / 2; ++j) {
-        FloatOperands<NT, MT> now;
-        now.read(lines + ws * kSlot, lines + xs * kSlot, wn, wm, j);
-        if constexpr (decltype(thirds)::value) {
-          // one row of tiles' thirds at a time, as registers allow
-          u32x4 a[NT][3], b[3];
+      for (int t = 0; t < NT; ++t) read(a[t], ws, wn + t * 16);
+      if constexpr (decltype(thirds)::value) {
+        u32x4 as[NT][3], bs[3];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) to_thirds(now.a[t], a[t]);
+        for (int t = 0; t < NT; ++t) to_thirds(a[t], as[t]);
 #pragma unroll
-          for (int u = 0; u < MT; ++u) {
-            to_thirds(now.b[u], b);
+        for (int u = 0; u < MT; ++u) {
+          read(b, xs, wm + u * 16);
+          to_thirds(b, bs);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t][u] = thirds_product(a[t], b, acc[t][u]);
-          }
-        } else {
-          now.multiply(acc);
+          for (int i = 0; i < kThirds; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              acc[t][u] = Product<__bf16>::narrow(as[t][kOfLeft[i]], bs[kOfRight[i]], acc[t][u]);
         }
-        __builtin_amdgcn_sched_barrier(0);
+      } else {
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
+          read(b, xs, wm + u * 16);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              acc[t][u] = Product<float>::narrow(a[t][c], b[c], acc[t][u]);
+        }
       }
       arrive<kLoads>();                    // all but x of two steps on
       w.load(lines + xs * kSlot, k + 2 * kEach, end);
@@ -656,8 +666,14 @@ __global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p)
   };
   sums(std::true_type());
   if (any_not_finite(acc, reinterpret_cast<int*>(s_lines))) sums(std::false_type());
-  finish_tile<T>(p, acc, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 8, m0 + wm, n0 + wn,
-                 blockIdx.y);
+  auto put = [&](int u, auto place) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) place(g * 16 + row, t * 4 + quarter) = acc[t][2 * u + g];
+  };
+  finish_rows<T, NT / 2, MT / 2>(p, put, reinterpret_cast<f32x4*>(s_lines) + wave * 32 * NT * 4,
+                                 m0 + wm, n0 + wn, blockIdx.y);
 }
 
 // One workgroup: BM rows of x by BN rows of W over a split of the summed axis;
@@ -716,7 +732,7 @@ __global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearPara
         raw[j].read(from + BM * kLineBytes, from, wn, wm, j);
         now[j ^ 1].take(raw[j ^ 1]);
         now[j].multiply(acc);
-        constexpr int kProducts = 6 * NT * MT, kOthers = 44 * (NT + MT) / kProducts;
+        constexpr int kProducts = kThirds * NT * MT, kOthers = 44 * (NT + MT) / kProducts;
 #pragma unroll
         for (int i = 0; i < kProducts; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);          // a product
@@ -1036,7 +1052,7 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
 //   2,048 rows, 2048 x 2048: 64 29, 64 x 128 29, 128 23, 256 44
 //   4,096 rows, 4096 x 4096: 64 209, 64 x 128 197, 128 153, 256 100
 //   and in float32 4,000 rows, 4000 x 4000: 64 962, 64 x 128 909, 128 704, 256
-//   627; 256 rows, 2048 x 2048: 64 42, 64 (4) 26, 64 x 128 (4) 25.
+//   579; 256 rows, 2048 x 2048: 64 42, 64 (4) 26, 64 x 128 (4) 25.
 struct FormCost {
   LinearForm form;
   int rows, columns;               // of a tile
@@ -1047,7 +1063,7 @@ constexpr FormCost kFormCosts[] = {
     {LinearForm::k64, 64, 64, {0.30f, 0.57f}, 1.0f},
     {LinearForm::k64x128, 64, 128, {0.38f, 0.85f}, 1.0f},
     {LinearForm::k128, 128, 128, {0.58f, 1.4f}, 2.5f},
-    {LinearForm::k256, 256, 256, {1.45f, 4.9f}, 4.0f},
+    {LinearForm::k256, 256, 256, {1.45f, 4.55f}, 4.0f},
 };
 constexpr int64_t kChipCus = 256;
 constexpr int kMostSplits = 16;
