@@ -504,10 +504,11 @@ __device__ __forceinline__ void tile_place(const LinearParams& p, int groups, in
 //
 // Half of a wave's rows of x are multiplied while the other half's next ones
 // are read.  The matrix cores bound it, at the clock that the power leaves:
-// 7,919 rows by 4096 x 16384 in bfloat16 take 772 us, 1,380 TFLOP/s.  Products of
-// 32 by 32 by 16, which do as much a cycle, took 843, with the matrix cores busy
-// two thirds of the cycles at 1.7 GHz.  GELU in the epilogue adds 35: it fills
-// the vector units, and no other workgroup is on the CU meanwhile.
+// 7,919 rows by 4096 x 16384 in bfloat16 take 772 us, 1,380 TFLOP/s, with the
+// matrix cores busy 64 % of the cycles at 1.9 GHz.  Products of 32 by 32 by 16,
+// which do as much a cycle, took 843: 67 % at 1.7 GHz.  GELU in the epilogue adds
+// some 40: it fills the vector units, and no other workgroup is on the CU
+// meanwhile.
 template <typename T>
 __global__ __launch_bounds__(512) void linear_large_kernel(LinearParams p) {
   constexpr int B = 256, kThreads = 512, MT = 8, NT = 4, kHalf = MT / 2;
