@@ -232,3 +232,17 @@ def test_copies_past_four_gigabytes(device):
     assert bool((keys[14, 70] == 5).all()) and bool((values[14, 70] == 6).all())
     assert bool((scales[0][14, 70] == 0.25).all()) and int(keys[:14].amax()) == 0
     assert int(keys[14, :70].amax()) == 0 and int(values[14, :70].amax()) == 0
+
+
+@pytest.mark.parametrize("requests,columns,pages", [(0, 0, 0), (0, 3, 0), (2, 0, 0), (2, 0, 5),
+                                                    (2, 3, 0), (3, 2, 1), (0, 3, 4)])
+def test_tables_of_nothing(device, requests, columns, pages):
+    """No requests, columns or pages, alone and together: empty requests are
+    forked and released, and the stack is the pool."""
+
+    page, lengths = 16, [0] * requests
+    state = np.full((requests, columns), -1), [0] * pages, list(range(pages)), pages
+    named = list(range(requests))
+    assert assert_fork(device, lengths, state, named * 2, [0] * (2 * requests), page)[6] == 0
+    assert_release(device, lengths, state, named[::-1] + named, page)
+    assert_compact(device, lengths, state, page)
