@@ -127,18 +127,21 @@ __device__ __forceinline__ f32x4 activated(f32x4 y, int activation) {
 
 // Four elements at any address.
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p) {
+struct Four {
   typedef T vec __attribute__((ext_vector_type(4)));
-  vec v;
-  __builtin_memcpy(&v, p, sizeof(v));
+  typedef vec loose __attribute__((aligned(sizeof(T))));
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* p) {
+  const typename Four<T>::vec v = *reinterpret_cast<const typename Four<T>::loose*>(p);
   return __builtin_convertvector(v, f32x4);
 }
 
 template <typename T>
 __device__ __forceinline__ void put4(T* p, f32x4 y) {
-  typedef T vec __attribute__((ext_vector_type(4)));
-  const vec v = __builtin_convertvector(y, vec);
-  __builtin_memcpy(p, &v, sizeof(v));
+  *reinterpret_cast<typename Four<T>::loose*>(p) =
+      __builtin_convertvector(y, typename Four<T>::vec);
 }
 
 // Columns n to n + 3 of output row m, as far as there are any: nothing past
