@@ -672,7 +672,7 @@ __global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p)
 // What a CU takes in from beyond its L2 bounds it where there are few rows, some
 // 50 to 60 bytes a nanosecond whatever the stages' number, and else the steps'
 // round: 64 rows by 4096 x 6144 in bfloat16, in two splits of 64 x 64, 14.2 us
-// with the join; 1,111 rows by 2304 x 1544 in float16, 64 x 128, 17.5 us.
+// with the join; 1,111 rows by 2304 x 1544 in float16, 64 x 128, 18 us.
 template <typename T, int BM, int BN, int MW, int NW, int kStages>
 __global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearParams p) {
   constexpr int kThreads = MW * NW * kWave;
