@@ -310,14 +310,16 @@ class PagedKVCache:
         most = min(used, pages - used)
         copy_pages(self.key_pages, self.key_scales, self.value_pages, self.value_scales,
                    moves.sources[:most], moves.targets[:most])
-        kept = [t[:, :target].contiguous() for t in (self.key_pages, self.key_scales,
-                                                     self.value_pages, self.value_scales)]
-        shares = moves.page_shares[:target].clone()
+        # copies: a slice of a pool of one layer is contiguous as it is, and
+        # would keep all of that pool's memory
+        kept = [t[:, :target].clone(memory_format=torch.contiguous_format)
+                for t in (self.key_pages, self.key_scales, self.value_pages, self.value_scales)]
+        tables, shares = moves.page_tables.clone(), moves.page_shares[:target].clone()
         # the stack's numbers fall from the pool's last one on
         stack = moves.free_pages[pages - target:].clone()
         count = torch.full_like(self.free_count, target - used)
         self.key_pages, self.key_scales, self.value_pages, self.value_scales = kept
-        self.page_tables, self.page_shares = moves.page_tables, shares
+        self.page_tables, self.page_shares = tables, shares
         self.free_pages, self.free_count = stack, count
         self._free = target - used
         self._before = None
