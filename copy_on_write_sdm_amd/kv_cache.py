@@ -13,6 +13,7 @@ from __future__ import annotations
 
 from contextlib import contextmanager
 from typing import Callable, Sequence
+from weakref import ref
 
 import torch
 
@@ -31,7 +32,13 @@ class PagedKVCache:
     launch, without reading the device.  Requests that ``fork`` makes share
     the whole pages of what they have in common; such pages are full, and a
     request's new tokens go to pages of its own.  Calls on one cache must be
-    stream-ordered."""
+    stream-ordered.
+
+    ``fork``, ``trim_pages`` and ``grow_pages`` are refused while a step of a
+    ``PagedAttention`` over this cache has layers left to run, or the stack is
+    within one.  Who calls ``extend`` and ``write`` by hand writes every layer
+    before them: a fork copies what has been written, and a trim makes a step's
+    slots void."""
 
     def __init__(self, layers: int, heads: int, head_width: int, *, capacity: int, pages: int,
                  page_tokens: int = 64, device: torch.device | str = "cuda"):
@@ -70,6 +77,7 @@ class PagedKVCache:
         self._free = pages
         self._before: tuple | None = None       # what the last extend may be taken back to
         self._added: dict[tuple[int, ...], torch.Tensor] = {}
+        self._blocks: list[ref[PagedAttention]] = []     # those that run on this cache
 
     @property
     def layers(self) -> int:
@@ -183,6 +191,17 @@ class PagedKVCache:
                                 self.page_tables, self.lengths,
                                 longest=max(self._lengths, default=0), scale=scale)
 
+    def _no_open_step(self) -> None:
+        """Refuses what would copy or move pages, or replace the pool, while a
+        step's slots are yet to be written or it may yet be taken back."""
+
+        for known in self._blocks:
+            block = known()
+            if block is not None:
+                block._none_unfinished()
+                if block._whole:
+                    raise ValueError("the stack is within a step of the KV cache")
+
     def fork(self, requests: Sequence[int], tokens: int | Sequence[int] | None = None
              ) -> list[int]:
         """One more request for each named one, after the others: it holds its
@@ -191,6 +210,7 @@ class PagedKVCache:
         once.  Whole pages are shared; the page in which the tokens end is
         copied.  Returns the new requests' indices."""
 
+        self._no_open_step()
         named = [int(r) for r in requests]
         if any(not 0 <= r < self.requests or r in self._released for r in named):
             raise ValueError("forked request is invalid or inactive")
@@ -300,6 +320,7 @@ class PagedKVCache:
 
         if headroom_pages < 0:
             raise ValueError("KV cache headroom cannot be negative")
+        self._no_open_step()
         pages = self.free_pages.numel()
         used = pages - self._free
         target = max(1, used + headroom_pages)
@@ -332,6 +353,7 @@ class PagedKVCache:
 
         if pages < 0:
             raise ValueError("added KV cache pages cannot be negative")
+        self._no_open_step()
         if not pages:
             return
         before = self.free_pages.numel()
@@ -421,7 +443,9 @@ class PagedAttention:
         self._step: PageTableStep | None = None
         self._next = 0              # the layer of the step that runs next
         self._prompt = False
+        self._whole = False         # within a step that the stack has opened
         self._before: tuple | None = None       # where the cache stood before the step
+        cache._blocks = [known for known in cache._blocks if known() is not None] + [ref(self)]
 
     # ------------------------------------------------------------- the steps
 
@@ -472,6 +496,7 @@ class PagedAttention:
     @contextmanager
     def _whole_step(self, begin: Callable[..., None], *args):
         begin(*args)
+        self._whole = True
         try:
             yield
             if self._unfinished():
@@ -479,6 +504,8 @@ class PagedAttention:
         except BaseException:
             self.abort()
             raise
+        finally:
+            self._whole = False
 
     def prefill_step(self, batch: int, time: int):
         """A context that opens the step of a prompt and takes it back when its
