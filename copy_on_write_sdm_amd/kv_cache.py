@@ -273,13 +273,17 @@ class PagedKVCache:
         if not named:
             return 0
         rows = torch.tensor(named, dtype=torch.int32, device=self.device)
-        # a launch takes so many; the pages of what comes first lie lowest
+        at = rows.long()
+        # a launch takes so many; the pages of what comes first lie lowest, above
+        # the count until all have gone
+        left = self.lengths, self.page_shares, self.free_count
+        self._before = None         # the stack holds no more what a step has taken off it
         for part in rows.split(MAX_REQUESTS):
-            left = release_page_tables(self.lengths, self.page_tables, self.page_shares,
-                                       self.free_pages, self.free_count, part,
-                                       page_tokens=self.page_tokens)
-            self.lengths, self.page_shares, self.free_count = left
-        self.page_tables.index_fill_(0, rows.long(), -1)
+            lengths, shares, count = left
+            left = release_page_tables(lengths, self.page_tables, shares, self.free_pages, count,
+                                       part, page_tokens=self.page_tokens)
+        self.lengths, self.page_shares, self.free_count = left
+        self.page_tables.index_fill_(0, at, -1)
         freed = 0
         for r in named:
             freed += self._pages(self._lengths[r]) - len(self._shared[r])
@@ -288,7 +292,6 @@ class PagedKVCache:
                 if not self._holders[page]:
                     del self._holders[page]
                     freed += 1
-        self._before = None
         for r in named:
             self._lengths[r] = 0
         self._shared = [() if r in gone else s for r, s in enumerate(self._shared)]
