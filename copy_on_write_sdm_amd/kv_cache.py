@@ -360,6 +360,8 @@ class PagedKVCache:
         if not pages:
             return
         before = self.free_pages.numel()
+        if (before + pages) * self.page_tokens >= 1 << 31:
+            raise ValueError("KV cache pages hold fewer than 2^31 tokens")
 
         def grown(t: torch.Tensor, value: int) -> torch.Tensor:
             bits = t.view(torch.uint8) if t.dtype is CODES else t

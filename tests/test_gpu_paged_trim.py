@@ -1,4 +1,4 @@
-"""What a trimmed pool gives up."""
+"""What a trimmed pool gives up, and how far one grows."""
 
 from __future__ import annotations
 
@@ -30,3 +30,20 @@ def test_trimmed_memory_is_given_up(device, layers):
                  "page_shares", "free_pages", "free_count"):
         t = getattr(cache, name)
         assert t.untyped_storage().nbytes() == t.numel() * t.element_size(), name
+
+
+def test_a_pool_grows_no_further_than_its_operators_count(device):
+    """Slots are 32-bit: past them no step, and no trim, would be taken any
+    more.  Refused before anything is allocated."""
+
+    cache = cow.PagedKVCache(1, 1, 32, capacity=64, pages=4, page_tokens=PAGE, device=device)
+    cache.admit(1)
+    cache.extend(20)
+    for more in ((1 << 31) // PAGE - 4, 1 << 40):
+        with pytest.raises(ValueError, match="fewer than 2\\^31 tokens"):
+            cache.grow_pages(more)
+    assert cache.free == 2 and cache.key_pages.shape[1] == 4
+    cache.take_back()                          # nothing has changed
+    cache.grow_pages(3)
+    assert cache.free == 7
+    assert_whole(cache)
