@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kHeadThreads) void rotate_heads_kernel(HeadParams p
 }
 
 template <typename T, int C>
-void launch_heads(HeadParams p, bool interleaved, hipStream_t s) {
+int32_t launch_heads(HeadParams p, bool interleaved, hipStream_t s) {
   const int need = p.width / (2 * C);
   p.lanes = 1;
   while (p.lanes < need) p.lanes *= 2;
@@ -190,6 +190,9 @@ void launch_heads(HeadParams p, bool interleaved, hipStream_t s) {
   if (p.rows > kHeadGroups * p.tokens && p.tokens < enough) p.tokens = enough;
   if (p.tokens > kHeadTokens) p.tokens = kHeadTokens;
   const int groups = (p.rows + p.tokens - 1) / p.tokens;
+  // a launch counts its threads in 32 bits
+  if (groups > static_cast<int>(UINT32_MAX / kHeadThreads))
+    return fail(COWSDM_ELIMIT, "rotate_heads: too large");
   const int bytes = 8 * p.width + 4 * p.tokens * p.rotated;
   if (interleaved)
     hipLaunchKernelGGL((rotate_heads_kernel<T, C, true>), dim3(groups), dim3(kHeadThreads), bytes,
@@ -197,6 +200,7 @@ void launch_heads(HeadParams p, bool interleaved, hipStream_t s) {
   else
     hipLaunchKernelGGL((rotate_heads_kernel<T, C, false>), dim3(groups), dim3(kHeadThreads),
                        bytes, s, p);
+  return launch_status("rotate_heads");
 }
 
 }  // namespace cowsdm_impl
@@ -218,7 +222,7 @@ extern "C" int32_t cowsdm_rotate_heads(const cowsdm_rotate_heads_t* heads, void*
     return fail(COWSDM_EARG, "rotate_heads: bad float type");
   if (!(a.eps >= 0.0f) || a.eps > 3.0e38f)
     return fail(COWSDM_EARG, "rotate_heads: eps cannot be negative");
-  // a launch counts its threads in 32 bits
+  // counted in 32 bits here, and a launch's threads by its workgroups
   if (a.rows >= (int64_t{1} << 24) * 3 || a.heads > 65535 || a.kv_heads > 65535)
     return fail(COWSDM_ELIMIT, "rotate_heads: too large");
   if (a.rows == 0) return 0;
@@ -254,13 +258,10 @@ extern "C" int32_t cowsdm_rotate_heads(const cowsdm_rotate_heads_t* heads, void*
   p.eps = a.eps;
   const auto s = static_cast<hipStream_t>(stream);
   const bool by_eight = a.width % 16 == 0 && a.rotated % 16 == 0;
-  if (a.float_type == COWSDM_FLOAT32) launch_heads<float, 4>(p, a.interleaved, s);
-  else if (a.float_type == COWSDM_FLOAT16) {
-    if (by_eight) launch_heads<_Float16, 8>(p, a.interleaved, s);
-    else launch_heads<_Float16, 4>(p, a.interleaved, s);
-  } else {
-    if (by_eight) launch_heads<__bf16, 8>(p, a.interleaved, s);
-    else launch_heads<__bf16, 4>(p, a.interleaved, s);
-  }
-  return launch_status("rotate_heads");
+  if (a.float_type == COWSDM_FLOAT32) return launch_heads<float, 4>(p, a.interleaved, s);
+  if (a.float_type == COWSDM_FLOAT16)
+    return by_eight ? launch_heads<_Float16, 8>(p, a.interleaved, s)
+                    : launch_heads<_Float16, 4>(p, a.interleaved, s);
+  return by_eight ? launch_heads<__bf16, 8>(p, a.interleaved, s)
+                  : launch_heads<__bf16, 4>(p, a.interleaved, s);
 }

@@ -1008,7 +1008,8 @@ int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace, int64_t wo
  * and then, of its first `rotated` elements, pair j (elements j and j +
  * rotated / 2, or 2 j and 2 j + 1 where interleaved) turned by position *
  * turns[j] / 2^64 of a full turn, which is exact in 64-bit integers at any
- * position.  The outputs are contiguous and none of the inputs. */
+ * position.  The outputs are contiguous and none of the inputs.  A workgroup
+ * takes a token or more: COWSDM_ELIMIT for 2^24 workgroups or more. */
 typedef struct cowsdm_rotate_heads {
   const void* query;
   const void* key;
