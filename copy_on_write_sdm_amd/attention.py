@@ -21,8 +21,9 @@ by which the codes count, [pages, heads].  The width is a head's, padded with
 zeros to 32, 64, 96, 128, 192 or 256 (``cache_width``).
 
 Kernels: csrc/prompt_attention.hip and csrc/kv_cache.hip.  Float32, float16
-and bfloat16; there is no backward pass (inputs that require a gradient are
-refused, where gradients are recorded) and no CPU path.
+and bfloat16; there is no derivative (inputs that require a gradient are
+refused, where gradients are recorded, and inputs with a tangent) and no CPU
+path.
 """
 
 from __future__ import annotations
@@ -31,6 +32,7 @@ import math
 from typing import NamedTuple, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -63,6 +65,12 @@ def _need_no_gradient(*tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise RuntimeError("the attention operators have no backward pass: call them under "
                            "torch.no_grad(), or with detached inputs")
+    # tangents, which no_grad() does not take away; the level first, as looking
+    # at each input takes half a microsecond
+    if forward_ad._current_level >= 0 and any(
+            [forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        raise RuntimeError("the attention operators have no forward-mode derivative: call them "
+                           "with the inputs' primals")
 
 
 def _float_type(dtype: torch.dtype) -> int:

@@ -3,8 +3,8 @@ over a projection's output: what stands between an attention layer's
 projection and its attention.
 
 Kernel: csrc/head_rotation.hip.  Float32, float16 and bfloat16; there is no
-backward pass (inputs that require a gradient are refused, where gradients are
-recorded) and no CPU path.
+derivative (inputs that require a gradient are refused, where gradients are
+recorded, and inputs with a tangent) and no CPU path.
 """
 
 from __future__ import annotations

@@ -2,9 +2,9 @@
 attention layer's projections and a block's MLP, for a token of each request
 and for whole prompts.
 
-Kernels: csrc/linear.hip.  Float32, float16 and bfloat16; there is no backward
-pass (inputs that require a gradient are refused, where gradients are
-recorded) and no CPU path.
+Kernels: csrc/linear.hip.  Float32, float16 and bfloat16; there is no
+derivative (inputs that require a gradient are refused, where gradients are
+recorded, and inputs with a tangent) and no CPU path.
 """
 
 from __future__ import annotations
@@ -12,6 +12,7 @@ from __future__ import annotations
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .attention import _need_no_gradient
@@ -70,7 +71,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             raise ValueError("linear residual must be [...,N]")
         alike = alike and residual.dtype is dtype
         together = together and residual.get_device() == index
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _need_no_gradient(*[t for t in (x, weight, bias, residual) if t is not None])
     float_type = nat.FLOAT_TYPES.get(dtype)
     if float_type is None:
