@@ -382,6 +382,18 @@ class Linear(ctypes.Structure):
     ]
 
 
+class LinearPlan(ctypes.Structure):
+    """cowsdm_linear_plan_t."""
+
+    _fields_ = [
+        ("workspace_bytes", ctypes.c_int64),
+        ("tile_rows", ctypes.c_int32),
+        ("tile_columns", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class RotateHeads(ctypes.Structure):
     """cowsdm_rotate_heads_t."""
 
@@ -515,6 +527,8 @@ SIGNATURES: dict[str, tuple] = {
     "cowsdm_page_tables_compact": (
         _I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "cowsdm_pages_copy": (_I32, [ctypes.POINTER(KVCache), _I64, _P, _P, _I64, _P]),
+    "cowsdm_linear_plan": (
+        _I32, [_I64, _I64, _I64, _I32, _I32, ctypes.POINTER(LinearPlan)]),
     "cowsdm_linear_workspace_bytes": (_I64, [_I64, _I64, _I64, _I32]),
     "cowsdm_linear": (_I32, [ctypes.POINTER(Linear), _P, _I64, _P]),
     "cowsdm_rotate_heads": (_I32, [ctypes.POINTER(RotateHeads), _P]),

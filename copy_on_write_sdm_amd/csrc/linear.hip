@@ -973,8 +973,6 @@ struct LinearPlan {
   int splits;
 };
 
-LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size);
-
 template <typename T, int BM, int BN, int MW, int NW, int kStages>
 int32_t launch_tiles(const LinearParams& p, hipStream_t s) {
   constexpr int kLines = kStages * (BM + BN) * kLineBytes;
@@ -991,7 +989,7 @@ int32_t launch_few(const LinearParams& p, hipStream_t s) {
 }
 
 template <typename T>
-int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipStream_t s) {
+int32_t launch_linear(LinearParams p, const LinearPlan& plan, hipStream_t s) {
   p.splits = 1;
   p.chunk = p.inner;
   if (plan.splits > 1) {
@@ -1001,7 +999,7 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
     p.chunk = (steps + plan.splits - 1) / plan.splits * kEach;
   }
   int32_t e = 0;
-  switch (aligned ? plan.form : LinearForm::kOdd) {
+  switch (plan.form) {
     case LinearForm::kOdd:
       e = launch_groups(&linear_odd_kernel<T>, tiles_of(p.rows, p.outer, 64, 64), p.splits, 256, 0,
                         p, s);
@@ -1029,8 +1027,10 @@ int32_t launch_linear(LinearParams p, bool aligned, const LinearPlan& plan, hipS
 // What a form takes of a call's sizes, in microseconds: rounds of workgroups,
 // each so long a step of 128 bytes and so long at its ends, or the memory's
 // time, and, where the summed axis is split, the join's launch and traffic.
-// The least one runs; where rows cannot all be aligned, the odd form's splits
-// are chosen the same way.  The constants are fitted to calls on one MI355X, which
+// The least one runs; where rows do not all start on 16 bytes, by their width,
+// stride or address, that is the odd form with the best of its own splits (a row
+// by 4096 x 1024 in bfloat16 at an odd address 7.8 us in 16 splits, 31.8 in the
+// one split of few rows).  The constants are fitted to calls on one MI355X, which
 // they give within some 20 %; in bfloat16, by the forms (splits):
 //   64 rows, 128 x 384: few 3.2, tiles of 64 3.8; 32 rows, 8192 x 512: few 23,
 //   64 (16) 9.6; a row, 4096 x 6144: few 12.7, 64 x 128 (5) 12.5; 64 rows: few
@@ -1057,10 +1057,12 @@ constexpr FormCost kFormCosts[] = {
 constexpr int64_t kChipCus = 256;
 constexpr int kMostSplits = 16;
 
-LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size) {
+// `aligned`: both operands' addresses and strides are multiples of 16 bytes.
+LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size, bool aligned) {
   const float memory =
       static_cast<float>((rows * inner + inner * outer + rows * outer) * size) * (1.0f / 5.0e6f);
-  LinearPlan best{LinearForm::k128, 1};
+  const bool odd = !aligned || inner * size % 16 != 0;
+  LinearPlan best{odd ? LinearForm::kOdd : LinearForm::k128, 1};   // of nothing to sum
   float least = 3.0e38f;
   auto consider = [&](LinearForm form, int splits, float us) {
     if (us < least) {
@@ -1068,7 +1070,6 @@ LinearPlan plan_linear(int64_t rows, int64_t inner, int64_t outer, int size) {
       best = {form, splits};
     }
   };
-  const bool odd = inner * size % 16 != 0;
   if (rows <= kFewRows && !odd) {
     const int64_t rounds = ((outer + 15) / 16 + kChipCus - 1) / kChipCus;
     const float us = static_cast<float>(rounds * (16 + rows) * inner * size) * (1.0f / 36.0e3f);
@@ -1112,21 +1113,52 @@ int64_t workspace_of(const LinearPlan& plan, int64_t rows, int64_t outer) {
   return plan.splits == 1 ? 0 : plan.splits * rows * ((outer + 3) / 4 * 16);
 }
 
-// 16-byte loads of both operands
+// 16-byte loads of both operands, as far as their inner size allows them
 bool linear_aligned(const cowsdm_linear_t& l) {
   const int64_t unit = l.float_type == COWSDM_FLOAT32 ? 4 : 8;
   return (reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.weight)) % 16 == 0 &&
-         l.inner % unit == 0 && l.x_row % unit == 0 && l.weight_row % unit == 0;
+         l.x_row % unit == 0 && l.weight_row % unit == 0;
 }
 
 }  // namespace
+
+extern "C" int32_t cowsdm_linear_plan(int64_t rows, int64_t inner, int64_t outer,
+                                      int32_t float_type, int32_t aligned,
+                                      cowsdm_linear_plan_t* plan) {
+  if (!plan) return fail(COWSDM_EARG, "linear_plan: null argument");
+  if (rows < 0 || inner < 0 || outer < 0)
+    return fail(COWSDM_EARG, "linear_plan: negative size");
+  if (float_type != COWSDM_FLOAT32 && float_type != COWSDM_FLOAT16 &&
+      float_type != COWSDM_BFLOAT16)
+    return fail(COWSDM_EARG, "linear_plan: bad float type");
+  if (inner > COWSDM_LINEAR_MOST || rows > INT32_MAX - 256 || outer > INT32_MAX - 256)
+    return fail(COWSDM_ELIMIT, "linear_plan: too large");
+  *plan = cowsdm_linear_plan_t{};
+  if (rows == 0 || outer == 0) return 0;
+  const LinearPlan p =
+      plan_linear(rows, inner, outer, float_type == COWSDM_FLOAT32 ? 4 : 2, aligned != 0);
+  plan->workspace_bytes = workspace_of(p, rows, outer);
+  plan->splits = p.splits;
+  if (p.form == LinearForm::kFew) {
+    plan->tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kFewRows;
+    plan->tile_columns = 16;
+  }
+  for (const FormCost& f : kFormCosts) {
+    if (f.form != p.form) continue;
+    plan->tile_rows = f.rows;
+    plan->tile_columns = f.columns;
+  }
+  return 0;
+}
 
 extern "C" int64_t cowsdm_linear_workspace_bytes(int64_t rows, int64_t inner, int64_t outer,
                                                  int32_t float_type) {
   if (rows < 0 || inner < 0 || outer < 0 || rows > INT32_MAX || outer > INT32_MAX) return -1;
   if (rows == 0 || outer == 0) return 0;
-  const LinearPlan plan = plan_linear(rows, inner, outer, float_type == COWSDM_FLOAT32 ? 4 : 2);
-  return workspace_of(plan, rows, outer);
+  const int size = float_type == COWSDM_FLOAT32 ? 4 : 2;
+  const int64_t aligned = workspace_of(plan_linear(rows, inner, outer, size, true), rows, outer);
+  const int64_t odd = workspace_of(plan_linear(rows, inner, outer, size, false), rows, outer);
+  return aligned > odd ? aligned : odd;
 }
 
 extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace,
@@ -1152,8 +1184,8 @@ extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace,
     return fail(COWSDM_EARG, "linear: null pointer argument");
   const int64_t size = l.float_type == COWSDM_FLOAT32 ? 4 : 2;
   auto address = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-  const bool aligned = linear_aligned(l);
-  const LinearPlan plan = plan_linear(l.rows, l.inner, l.outer, static_cast<int>(size));
+  const LinearPlan plan =
+      plan_linear(l.rows, l.inner, l.outer, static_cast<int>(size), linear_aligned(l));
   if (plan.splits > 1) {
     const int64_t need = workspace_of(plan, l.rows, l.outer);
     if (!workspace || workspace_bytes < need)
@@ -1177,7 +1209,7 @@ extern "C" int32_t cowsdm_linear(const cowsdm_linear_t* linear, void* workspace,
   p.activation = l.activation;
   p.parts = static_cast<float*>(workspace);
   const auto s = static_cast<hipStream_t>(stream);
-  if (l.float_type == COWSDM_FLOAT32) return launch_linear<float>(p, aligned, plan, s);
-  if (l.float_type == COWSDM_FLOAT16) return launch_linear<_Float16>(p, aligned, plan, s);
-  return launch_linear<__bf16>(p, aligned, plan, s);
+  if (l.float_type == COWSDM_FLOAT32) return launch_linear<float>(p, plan, s);
+  if (l.float_type == COWSDM_FLOAT16) return launch_linear<_Float16>(p, plan, s);
+  return launch_linear<__bf16>(p, plan, s);
 }

@@ -23,10 +23,13 @@ _MOST = 1 << 20          # elements of a row, and between rows
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(rows: int, inner: int, outer: int, float_type: int) -> int:
-    """By the sizes alone: asked for once."""
+def _workspace_bytes(rows: int, inner: int, outer: int, float_type: int, aligned: bool) -> int:
+    """By the sizes and the alignment alone: asked for once."""
 
-    return nat.lib().cowsdm_linear_workspace_bytes(rows, inner, outer, float_type)
+    plan = nat.LinearPlan()
+    nat.check(nat.lib().cowsdm_linear_plan(rows, inner, outer, float_type, aligned, plan),
+              "cowsdm_linear_plan")
+    return plan.workspace_bytes
 
 
 def _matrix(tensor: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
@@ -95,9 +98,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if residual is not None:
         residual, residual_row = _matrix(
             residual if residual.ndim == 2 else residual.reshape(rows, outer), outer)
-    need = _workspace_bytes(rows, inner, outer, float_type)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    a = nat.Linear(x.data_ptr(), weight.data_ptr(), nat.ptr(bias), nat.ptr(residual),
+    x_at, weight_at = x.data_ptr(), weight.data_ptr()
+    aligned = not ((x_at | weight_at) % 16 or (x_row | weight_row) % (8 if float_type else 4))
+    need = _workspace_bytes(rows, inner, outer, float_type, aligned)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    a = nat.Linear(x_at, weight_at, nat.ptr(bias), nat.ptr(residual),
                    out.data_ptr(), x_row, weight_row, residual_row, rows, inner, outer, float_type,
                    code)
     rc = nat.lib().cowsdm_linear(a, nat.ptr(workspace), need, nat.stream_handle(device))

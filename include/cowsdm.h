@@ -992,8 +992,24 @@ typedef struct cowsdm_linear {
   int32_t activation;
 } cowsdm_linear_t;
 
-/* Bytes of workspace that a call of cowsdm_linear needs (0: none), 16-byte
- * aligned. */
+/* What a call of cowsdm_linear runs: the output in tiles of so many rows and
+ * columns, the summed axis in so many splits, and the workspace that takes (0:
+ * none). */
+typedef struct cowsdm_linear_plan {
+  int64_t workspace_bytes;
+  int32_t tile_rows;
+  int32_t tile_columns;
+  int32_t splits;
+  int32_t reserved;
+} cowsdm_linear_plan_t;
+
+/* The plan of a call, from its sizes and whether the addresses of x and weight
+ * and the strides of their rows are multiples of 16 bytes. */
+int32_t cowsdm_linear_plan(int64_t rows, int64_t inner, int64_t outer, int32_t float_type,
+                           int32_t aligned, cowsdm_linear_plan_t* plan);
+
+/* Bytes of workspace that suffice for a call of cowsdm_linear whatever its
+ * operands' alignment (0: none needed); the workspace is 16-byte aligned. */
 int64_t cowsdm_linear_workspace_bytes(int64_t rows, int64_t inner, int64_t outer,
                                       int32_t float_type);
 
