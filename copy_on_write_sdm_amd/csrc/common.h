@@ -109,6 +109,12 @@ __device__ __forceinline__ float rlf(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
+// LDS written by lanes of one wave and read by others of the same wave
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Wave-inclusive sum over lanes (lane order), in DPP moves: shifts by 1, 2,
 // 4 and 8 lanes within each row of 16, then row 0's and row 1's last lanes
 // broadcast into the rows after them (a lane shifted in from outside its

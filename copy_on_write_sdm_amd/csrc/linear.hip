@@ -172,8 +172,9 @@ __device__ __forceinline__ void finish4(const LinearParams& p, int m, int n, f32
 
 // A wave's sums of 32 NT columns by 32 MT rows of the output, as the products
 // leave them, through LDS (32 rows of its own at a time, which `put` writes in
-// chunks of four columns), so that a store writes whole rows of its columns.
-// Chunks are permuted against the banks.  A lane keeps to four columns, whose
+// chunks of four columns), so that a store writes whole rows of its columns;
+// what other lanes have written is read, and written over, behind a fence of the
+// wave.  Chunks are permuted against the banks.  A lane keeps to four columns, whose
 // bias it loads once, at whatever address they lie: 1,671 rows by 288 x 11706 in
 // bfloat16 take 42 us, and 64 with a column a lane.
 template <typename T, int NT, int MT, typename Put>
@@ -190,6 +191,7 @@ __device__ __forceinline__ void finish_rows(const LinearParams& p, Put put, f32x
     put(u, [&](int r, int chunk) -> f32x4& {
       return turned[r * kChunks + (chunk ^ (r & (kChunks - 1)))];
     });
+    wave_lds_sync();
     const int first = m0 + u * 32;
     auto at = [&](int r) { return turned[r * kChunks + (c ^ (r & (kChunks - 1)))]; };
     if (p.splits > 1) {
@@ -220,6 +222,7 @@ __device__ __forceinline__ void finish_rows(const LinearParams& p, Put put, f32x
         if (m < p.rows) put4(static_cast<T*>(p.out) + static_cast<int64_t>(m) * p.outer + n, y);
       }
     }
+    wave_lds_sync();
   }
 }
 

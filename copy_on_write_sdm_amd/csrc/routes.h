@@ -65,12 +65,6 @@ __device__ __forceinline__ void wave_rank(const uint64_t (&key)[J], int (&rank)[
   }
 }
 
-// LDS written by lanes of one wave and read by others of the same wave
-__device__ __forceinline__ void wave_lds_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // Lane t < count ends with the t-th best (value, position) of the wave's
 // candidates (pos < 0: absent).  stage_val/stage_pos hold kRouteMaxSelected
 // entries of this wave.
