@@ -552,6 +552,7 @@ __global__ __launch_bounds__(kPromptThreads, DP <= 128 ? 2 : 1) void prompt_half
             turned + own % 32 * DP * 2 + place<DP>(own % 32, d * 4 + i) * 16 + own / 32 * 8) =
             __builtin_convertvector(x, vec4);
       }
+    wave_lds_sync();            // other lanes' columns
     T* const out = static_cast<T*>(p.out) +
                    ((static_cast<int64_t>(begin) + q0) * p.heads + w.head) * p.width;
 #pragma unroll
