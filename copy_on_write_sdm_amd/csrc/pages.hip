@@ -7,9 +7,10 @@
 // that pages which nothing shares need no care: extension does not write it.
 //
 // Every operator leaves its inputs as they are and writes new lengths,
-// tables, counts and shares (release pushes onto the free stack above its
-// count, where nothing reads), so that a step can be taken back by keeping
-// what was there.  Each runs in phases that need all of the one before.  Where
+// tables, counts and shares, so that a step can be taken back by keeping what
+// was there.  Only the free stack is written in place: a release pushes above
+// its count, over the numbers that forks and extensions have popped, so that
+// after it there is no way back to a larger count.  Each runs in phases that need all of the one before.  Where
 // the numbers are few, one workgroup runs them all with the pages' numbers in
 // LDS and its entries in registers, so that a phase costs a barrier and not a
 // launch or a round trip to memory; else they are launches of their own.

@@ -14,8 +14,11 @@ finished requests' pages, and the pool's pages moved together.
 ``page_shares`` [pages] counts the requests that hold a page beyond the first:
 zeros where nothing is shared.  A page that requests share is full, so that
 extension and cache writes never touch one.  What the table operators return
-is new: their inputs stay as they are (a release pushes onto the free stack
-above its count), so that a caller that keeps the former tensors can go back.
+is new, and their inputs stay as they are but for the free stack, onto which a
+release pushes above its count, over the numbers that forks and extensions have
+popped.  A caller that keeps the tensors from before a call can go back to them,
+but after a release only as far as the free count was no larger than the one that
+it was called with.
 
 Kernels: csrc/pages.hip.  All on the device, without a read by the host; there
 is no CPU path.

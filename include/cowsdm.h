@@ -905,8 +905,10 @@ int32_t cowsdm_cached_attention(const cowsdm_kv_cache_t* cache,
 /* The life of a cache's pages besides their extension.  page_shares[p] counts
  * the requests that hold page p beyond the first (zeros where nothing is
  * shared); pages that requests share are full.  Inputs stay as they are, but
- * for the free stack, which a release writes above its count: lengths, tables,
- * counts and shares come out new and are not the inputs themselves.  At most
+ * for the free stack, which a release writes above its count (over the numbers
+ * that forks and extensions have popped: a state from before those, of a larger
+ * count than the release's, is void after it).  Lengths, tables, counts and shares come
+ * out new and are not the inputs themselves.  At most
  * 4,096 requests are forked or released at once; page_tokens is 16, 32, 64,
  * 128 or 256. */
 
