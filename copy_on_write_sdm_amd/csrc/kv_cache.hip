@@ -163,8 +163,9 @@ __global__ __launch_bounds__(kTableThreads) void extend_tables_kernel(ExtendPara
 }
 
 // The pages of the named requests go back to the top of the free stack, in
-// the order of the list; one workgroup, and a request's pages one after another
-// in a thread: 64 requests of 40 pages 45 us, 4 of 8,192 pages 1,180.
+// the order of the list, whoever else holds them; one workgroup, and a
+// request's pages one after another in a thread: 64 requests of 40 pages 45 us,
+// 4 of 8,192 pages 1,180.
 __global__ __launch_bounds__(kTableThreads) void release_pages_kernel(
     int32_t* lengths, int32_t* page_tables, int32_t columns, const int32_t* named, int32_t n,
     int32_t requests, int32_t* free_pages, int32_t pages, int32_t* free_count, int page_shift) {

@@ -838,7 +838,10 @@ int32_t cowsdm_page_tables_extend(
     int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* overflow, void* stream);
 
 /* The pages of the n named requests (distinct) return to the top of the free
- * stack in that order; their lengths become 0 and their table entries -1. */
+ * stack in that order; their lengths become 0 and their table entries -1.  For
+ * caches none of whose pages is shared: it knows of no shares, and would free
+ * pages that other requests still hold.  Once cowsdm_page_tables_fork has run,
+ * requests go by cowsdm_page_tables_release. */
 int32_t cowsdm_pages_release(int32_t* lengths, int32_t* page_tables, int64_t requests,
                              int64_t columns, const int32_t* named, int64_t n,
                              int32_t* free_pages, int64_t pages, int32_t* free_count,
