@@ -1,6 +1,6 @@
-"""cowsdm_pages_release, the C entry that returns the pages of requests which
-share none, in place: against page by page Python, and against
-release_page_tables, which does the same where nothing is shared."""
+"""cowsdm_pages_release, which returns the pages of requests that share none in
+place: against page by page Python, and against release_page_tables, which gives
+the same where nothing is shared."""
 
 from __future__ import annotations
 
