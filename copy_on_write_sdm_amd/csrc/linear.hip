@@ -675,7 +675,7 @@ __global__ __launch_bounds__(512) void linear_large_float_kernel(LinearParams p)
 // What a CU takes in from beyond its L2 bounds it where there are few rows, some
 // 50 to 60 bytes a nanosecond whatever the stages' number, and else the steps'
 // round: 64 rows by 4096 x 6144 in bfloat16, in two splits of 64 x 64, 14.2 us
-// with the join; 1,111 rows by 2304 x 1544 in float16, 64 x 128, 18 us.
+// with the join; 1,111 rows by 2304 x 1544 in float16, 64 x 128, 18.6 us.
 template <typename T, int BM, int BN, int MW, int NW, int kStages>
 __global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearParams p) {
   constexpr int kThreads = MW * NW * kWave;
@@ -780,7 +780,7 @@ __global__ __launch_bounds__(MW * NW * kWave) void linear_tile_kernel(LinearPara
 // the summed axis, from memory into registers, which a load of 16 bytes reaches
 // from any address, and on into LDS, a step ahead of the products.  What one
 // step ahead brings in bounds it: a row by 4095 x 6144 in bfloat16 14.7 us, 64
-// rows 30 (4096: 12.7 and 15), 1,111 rows by 2303 x 1544 in float16 34 (2304:
+// rows 30 (4096: 11.7 and 15), 1,111 rows by 2303 x 1544 in float16 34 (2304:
 // 18).  Element by element and nothing ahead they took 125, 173 and 117.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_odd_kernel(LinearParams p) {
@@ -890,7 +890,7 @@ constexpr int kFewRows = 64;
 // these are used; the waves' sums meet in LDS.
 //
 // What a CU can have on its way bounds it: some 36 bytes a nanosecond, of W
-// and of x.  bfloat16, a row by 4096 x 6144: 12.7 us, 4.0 TB/s.
+// and of x.  bfloat16, a row by 4096 x 6144: 11.7 us, 4.3 TB/s.
 template <typename T, int MT>
 __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(LinearParams p) {
   constexpr int kEach = 16 / static_cast<int>(sizeof(T));   // columns a lane
@@ -1035,16 +1035,18 @@ int32_t launch_linear(LinearParams p, const LinearPlan& plan, hipStream_t s) {
 // by 4096 x 1024 in bfloat16 at an odd address 7.8 us in 16 splits, 31.8 in the
 // one split of few rows).  The constants are fitted to calls on one MI355X, which
 // they give within some 20 %; in bfloat16, by the forms (splits):
-//   64 rows, 128 x 384: few 3.2, tiles of 64 3.8; 32 rows, 8192 x 512: few 23,
-//   64 (16) 9.6; a row, 4096 x 6144: few 12.7, 64 x 128 (5) 12.5; 64 rows: few
-//   38, 64 (2) 15.3, 64 x 128 (4) 15.0, 64 x 128 (1) 24
-//   100 rows, 4000 x 100: 64 (16) 7.4, 64 (1) 19
-//   2,910 rows, 7848 x 1420: 128 148, 128 (3) 121, 256 151, 256 (3) 76
-//   1,111 rows, 2304 x 1544: 64 16.7, 64 x 128 16.4, 128 23, 256 46
-//   2,048 rows, 2048 x 2048: 64 29, 64 x 128 29, 128 23, 256 44
-//   4,096 rows, 4096 x 4096: 64 209, 64 x 128 197, 128 153, 256 100
-//   and in float32 4,000 rows, 4000 x 4000: 64 962, 64 x 128 909, 128 704, 256
-//   579; 256 rows, 2048 x 2048: 64 42, 64 (4) 26, 64 x 128 (4) 25.
+//   64 rows, 128 x 384: few 3.2, tiles of 64 3.7; 32 rows, 8192 x 512: few 23,
+//   64 (16) 8.9; a row, 4096 x 6144: few 11.7, 64 x 128 (5) 12.7; 64 rows: few
+//   38, 64 (2) 15.0, 64 x 128 (4) 15.2, 64 x 128 (1) 25
+//   100 rows, 4000 x 100: 64 (16) 7.6, 64 (1) 19
+//   2,910 rows, 7848 x 1420: 128 150, 128 (3) 119, 256 150, 256 (3) 80
+//   1,111 rows, 2304 x 1544: 64 17.8, 64 x 128 17.9, 128 24, 256 47
+//   2,048 rows, 2048 x 2048: 64 31, 64 x 128 32, 128 25, 256 44
+//   4,096 rows, 4096 x 4096: 64 206, 64 x 128 197, 128 155, 256 99
+//   and in float32 4,000 rows, 4000 x 4000: 64 930, 64 x 128 875, 128 677, 256
+//   561; 256 rows, 2048 x 2048: 64 39, 64 (4) 25, 64 x 128 (4) 24; 64 rows, 4096 x
+//   6144: few 73, 64 x 128 106, 64 x 128 (5) 34
+//   and of rows that are not aligned 64 rows, 4095 x 6144: 49, (2) 30.
 struct FormCost {
   LinearForm form;
   int rows, columns;               // of a tile
